@@ -1,0 +1,432 @@
+// rmsnorm.cu -- root-mean-square norm with the residual's addition, forward and backward.
+//
+//   h = a + r  (rounded to the type it is stored in: the residual stream),   y = h * rstd * gamma,   rstd = (mean(h^2) + eps)^(-1/2)
+//   g = dy * gamma,   dh = rstd * (g - h * rstd^2 * mean(g h)) + dsum,   dgamma = sum over rows of dy * h * rstd
+//
+// dsum is the gradient that reaches h past the norm; dh is the gradient of a and of r.  Statistics, products and sums are held in 32 bits;
+// y, dh and dgamma are rounded once, when they are stored.
+//
+// What bounds it: HBM.  A row is read once into registers and written once: forward 4, backward 4 row's worth of bytes.  A row belongs to
+// one warp (WARPS 1, shuffles only) or to a block of eight (WARPS 8, one exchange through shared memory); a thread holds N pieces
+// of V elements (16 bytes, or one element where the width or an address does not allow that).  Backward's blocks stay for many rows: a
+// thread keeps the columns it owns of dgamma in registers and the block leaves one partial row, which the fold adds in a fixed order.
+// Rows too wide for registers take the kernels at the end, which read a row twice.
+#include "common.cuh"
+
+namespace {
+
+template <typename T> __device__ __forceinline__ float rms_ld(const T *p);
+template <> __device__ __forceinline__ float rms_ld<float>(const float *p) { return *p; }
+template <> __device__ __forceinline__ float rms_ld<bf16>(const bf16 *p) { return bf2f(*p); }
+__device__ __forceinline__ void rms_st(float *p, float v) { *p = v; }
+__device__ __forceinline__ void rms_st(bf16 *p, float v) { *p = f2bf(v); }
+__device__ __forceinline__ float rms_round(float v, const float *) { return v; }
+__device__ __forceinline__ float rms_round(float v, const bf16 *) { return bf2f(f2bf(v)); }
+
+// V elements as they lie in memory
+template <typename T, int V> struct Piece;
+template <> struct Piece<float, 1> {
+  float u;
+  __device__ __forceinline__ void load(const float *p) { u = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = u; }
+  __device__ __forceinline__ void set(const float (&v)[1]) { u = v[0]; }
+  __device__ __forceinline__ void store(float *p) const { *p = u; }
+  __device__ __forceinline__ void zero() { u = 0.f; }
+};
+template <> struct Piece<bf16, 1> {
+  bf16 u;
+  __device__ __forceinline__ void load(const bf16 *p) { u = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = bf2f(u); }
+  __device__ __forceinline__ void set(const float (&v)[1]) { u = f2bf(v[0]); }
+  __device__ __forceinline__ void store(bf16 *p) const { *p = u; }
+  __device__ __forceinline__ void zero() { u = f2bf(0.f); }
+};
+template <> struct Piece<float, 4> {
+  float4 u;
+  __device__ __forceinline__ void load(const float *p) { u = *reinterpret_cast<const float4 *>(p); }
+  __device__ __forceinline__ void get(float (&v)[4]) const { v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w; }
+  __device__ __forceinline__ void set(const float (&v)[4]) { u = make_float4(v[0], v[1], v[2], v[3]); }
+  __device__ __forceinline__ void store(float *p) const { *reinterpret_cast<float4 *>(p) = u; }
+  __device__ __forceinline__ void zero() { u = make_float4(0.f, 0.f, 0.f, 0.f); }
+};
+template <> struct Piece<bf16, 8> {
+  uint4 u;
+  __device__ __forceinline__ void load(const bf16 *p) { u = *reinterpret_cast<const uint4 *>(p); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const float2 a = unpack_bf162(u.x), b = unpack_bf162(u.y), c = unpack_bf162(u.z), d = unpack_bf162(u.w);
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    u = make_uint4(pack_bf162(v[0], v[1]), pack_bf162(v[2], v[3]), pack_bf162(v[4], v[5]), pack_bf162(v[6], v[7]));
+  }
+  __device__ __forceinline__ void store(bf16 *p) const { *reinterpret_cast<uint4 *>(p) = u; }
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+};
+
+// sum over the warps that share a row; `red`: two sets of WARPS floats that successive rows use in turn
+template <int WARPS>
+__device__ __forceinline__ float row_sum(float v, float *red, int parity) {
+  v = warp_sum(v);
+  if constexpr (WARPS > 1) {
+    float *r = red + parity * WARPS;
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) v += r[w];
+  }
+  return v;
+}
+
+// a, r, xsum and y are read and written element by element by the same thread: y or xsum may be a or r
+template <typename T, int V, int N, int WARPS>
+__global__ void __launch_bounds__(256) rms_fwd_kernel(const T *a, const T *b, const T *gamma, T *xsum, T *y, float *__restrict__ rstd, int rows,
+                                                      int cols, float eps) {
+  pdl_entry(xsum, y);
+  __shared__ float red[2 * (WARPS > 1 ? WARPS : 1)];
+  const int slot = WARPS > 1 ? threadIdx.x : threadIdx.x & 31;
+  const int per_block = WARPS > 1 ? 1 : (int)(blockDim.x >> 5);
+  const float inv = 1.f / (float)cols;
+  int parity = 0;
+  for (long long row = (long long)blockIdx.x * per_block + (WARPS > 1 ? 0 : threadIdx.x >> 5); row < rows; row += (long long)gridDim.x * per_block) {
+    const long long base = row * cols;
+    Piece<T, V> pa[N], pb[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * WARPS * 32 + slot) * V;
+      pa[i].zero();
+      pb[i].zero();
+      if (c < cols) {
+        pa[i].load(a + base + c);
+        if (b) pb[i].load(b + base + c);
+      }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float u[V], w[V];
+      pa[i].get(u);
+      if (b) {
+        pb[i].get(w);
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] += w[j];
+        pa[i].set(u);
+        pa[i].get(u);                        // the sum as it is stored
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) ss = fmaf(u[j], u[j], ss);
+    }
+    ss = row_sum<WARPS>(ss, red, parity);
+    parity ^= 1;
+    const float rs = rsqrtf(ss * inv + eps);
+    if (slot == 0 && rstd) rstd[row] = rs;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * WARPS * 32 + slot) * V;
+      if (c < cols) {
+        if (b && xsum) pa[i].store(xsum + base + c);
+        float u[V], g[V];
+        Piece<T, V> pg;
+        pg.load(gamma + c);
+        pg.get(g);
+        pa[i].get(u);
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] = u[j] * rs * g[j];
+        pa[i].set(u);
+        pa[i].store(y + base + c);
+      }
+    }
+  }
+}
+
+// dh may be dy or dsum.  `partial`: [gridDim.x][cols]
+template <typename T, int V, int N, int WARPS>
+__global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, const T *gamma, const float *rstd, const T *dsum, T *dh,
+                                                      float *__restrict__ partial, int rows, int cols) {
+  pdl_entry(dh);
+  __shared__ float red[2 * (WARPS > 1 ? WARPS : 1)];
+  extern __shared__ float part[];            // WARPS 1: the block's sum of dgamma, [cols]
+  const int warp = threadIdx.x >> 5;
+  const int slot = WARPS > 1 ? threadIdx.x : threadIdx.x & 31;
+  const int per_block = WARPS > 1 ? 1 : (int)(blockDim.x >> 5);
+  const float inv = 1.f / (float)cols;
+  float acc[N][V];
+  Piece<T, V> pg[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = (i * WARPS * 32 + slot) * V;
+    pg[i].zero();
+    if (c < cols) pg[i].load(gamma + c);
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[i][j] = 0.f;
+  }
+  int parity = 0;
+  for (long long row = (long long)blockIdx.x * per_block + (WARPS > 1 ? 0 : warp); row < rows; row += (long long)gridDim.x * per_block) {
+    const long long base = row * cols;
+    Piece<T, V> py[N], ph[N], ps[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * WARPS * 32 + slot) * V;
+      py[i].zero();
+      ph[i].zero();
+      ps[i].zero();
+      if (c < cols) {
+        py[i].load(dy + base + c);
+        ph[i].load(h + base + c);
+        if (N * V < 64 && dsum) ps[i].load(dsum + base + c);
+      }
+    }
+    const float rs = rstd[row];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float y[V], x[V], g[V];
+      py[i].get(y);
+      ph[i].get(x);
+      pg[i].get(g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float yx = y[j] * x[j];
+        dot = fmaf(yx, g[j], dot);
+        acc[i][j] = fmaf(yx, rs, acc[i][j]);
+      }
+    }
+    dot = row_sum<WARPS>(dot, red, parity);
+    parity ^= 1;
+    const float k = dot * inv * rs * rs;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * WARPS * 32 + slot) * V;
+      if (c < cols) {
+        float y[V], x[V], g[V], s[V];
+        py[i].get(y);
+        ph[i].get(x);
+        pg[i].get(g);
+        if (N * V >= 64 && dsum) ps[i].load(dsum + base + c);      // the widest rows: the other three fill the registers
+        ps[i].get(s);
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = fmaf(rs, fmaf(y[j], g[j], -x[j] * k), s[j]);
+        py[i].set(y);
+        py[i].store(dh + base + c);
+      }
+    }
+  }
+  if (!partial) return;
+  float *out = partial + (long long)blockIdx.x * cols;
+  if constexpr (WARPS > 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = (i * WARPS * 32 + slot) * V;
+      if (c < cols) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[c + j] = acc[i][j];
+      }
+    }
+  } else {
+    // the warps add up their columns one after the other
+    for (int w = 0; w < per_block; ++w) {
+      if (warp == w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = (i * 32 + slot) * V;
+          if (c < cols) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) part[c + j] = w == 0 ? acc[i][j] : part[c + j] + acc[i][j];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) out[c] = part[c];
+  }
+}
+
+// dgamma (+)= column sums of the `parts` partial rows, in their order: 32 columns a block, 32 threads a column
+template <typename T>
+__global__ void __launch_bounds__(1024) rms_fold_kernel(const float *partial, int parts, int cols, T *dgamma, int accumulate) {
+  pdl_entry(dgamma);
+  __shared__ float sum[32][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < cols)
+    for (int p = threadIdx.y; p < parts; p += 32) s += partial[(long long)p * cols + c];
+  sum[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < cols) {
+    s = 0.f;
+#pragma unroll
+    for (int p = 0; p < 32; ++p) s += sum[p][threadIdx.x];
+    if (accumulate) s += rms_ld(dgamma + c);
+    rms_st(dgamma + c, s);
+  }
+}
+
+// ---- rows too wide for registers: a block per row, two passes
+template <typename T>
+__global__ void __launch_bounds__(512) rms_fwd_wide_kernel(const T *a, const T *b, const T *gamma, T *xsum, T *y, float *__restrict__ rstd, int rows,
+                                                           int cols, float eps) {
+  pdl_entry(xsum, y);
+  __shared__ float red[32];
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const long long base = row * cols;
+    float ss = 0.f;
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      const float v = b ? rms_round(rms_ld(a + base + c) + rms_ld(b + base + c), a) : rms_ld(a + base + c);
+      ss = fmaf(v, v, ss);
+    }
+    ss = block_sum(ss, red);
+    const float rs = rsqrtf(ss / (float)cols + eps);
+    if (threadIdx.x == 0 && rstd) rstd[row] = rs;
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      const float v = b ? rms_round(rms_ld(a + base + c) + rms_ld(b + base + c), a) : rms_ld(a + base + c);
+      if (b && xsum) rms_st(xsum + base + c, v);
+      rms_st(y + base + c, v * rs * rms_ld(gamma + c));
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) rms_bwd_wide_kernel(const T *dy, const T *h, const T *gamma, const float *rstd, const T *dsum, T *dh,
+                                                           float *partial, int rows, int cols) {
+  pdl_entry(dh, partial);
+  __shared__ float red[32];
+  float *out = partial ? partial + (long long)blockIdx.x * cols : nullptr;
+  bool first = true;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x, first = false) {
+    const long long base = row * cols;
+    float dot = 0.f;
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) dot = fmaf(rms_ld(dy + base + c) * rms_ld(h + base + c), rms_ld(gamma + c), dot);
+    dot = block_sum(dot, red);
+    const float rs = rstd[row], k = dot / (float)cols * rs * rs;
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      const float y = rms_ld(dy + base + c), x = rms_ld(h + base + c);
+      const float s = dsum ? rms_ld(dsum + base + c) : 0.f;
+      if (out) out[c] = (first ? 0.f : out[c]) + y * x * rs;      // a column belongs to one thread of the block
+      rms_st(dh + base + c, fmaf(rs, fmaf(y, rms_ld(gamma + c), -x * k), s));
+    }
+    __syncthreads();
+  }
+}
+
+// How a row is spread: warps (1 or 8) and pieces per thread (1, 2, 4, 8); pieces 0: too wide for registers
+struct RmsForm { int v, warps, n; };
+RmsForm rms_form(int rows, int cols, int es, bool whole) {
+  const int v = whole && cols % (16 / es) == 0 ? 16 / es : 1;
+  const int pieces = (cols + v * 32 - 1) / (v * 32);       // of a warp
+  RmsForm f = {v, 1, 0};
+  if (pieces > 64) return f;
+  if (pieces > 4) { f.warps = 8; }
+  const int need = f.warps == 8 ? (pieces + 7) / 8 : pieces;
+  f.n = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
+  (void)rows;
+  return f;
+}
+int rms_fwd_grid(const RmsForm &f, int rows, int &threads) {
+  if (f.n == 0) { threads = 512; return rows < 148 * 4 ? rows : 148 * 4; }
+  if (f.warps == 8) { threads = 256; return rows < 148 * 8 ? rows : 148 * 8; }
+  threads = rows >= 148 * 8 ? 256 : 64;
+  const int per = threads / 32, want = (rows + per - 1) / per;
+  return want < 148 * 8 ? want : 148 * 8;
+}
+int rms_bwd_grid(const RmsForm &f, int rows) {
+  if (f.n == 0) return rows < 148 * 2 ? rows : 148 * 2;
+  const int want = f.warps == 8 ? rows : (rows + 7) / 8, most = 148 * 4;
+  return want < most ? want : most;
+}
+bool rms_aligned(const void *p) { return (((uintptr_t)p) & 15) == 0; }
+
+template <typename T, int V, int N, int WARPS>
+int rms_fwd_run(const void *a, const void *b, const void *gamma, void *xsum, void *y, float *rstd, int rows, int cols, float eps, int grid, int threads,
+                cudaStream_t st) {
+  return ffk_launch(rms_fwd_kernel<T, V, N, WARPS>, grid, threads, 0, st, (const T *)a, (const T *)b, (const T *)gamma, (T *)xsum, (T *)y, rstd, rows,
+                    cols, eps);
+}
+template <typename T, int V, int N, int WARPS>
+int rms_bwd_run(const void *dy, const void *h, const void *gamma, const float *rstd, const void *dsum, void *dh, float *partial, int rows, int cols,
+                int grid, cudaStream_t st) {
+  return ffk_launch(rms_bwd_kernel<T, V, N, WARPS>, grid, 256, WARPS == 1 ? (size_t)cols * 4 : 0, st, (const T *)dy, (const T *)h, (const T *)gamma,
+                    rstd, (const T *)dsum, (T *)dh, partial, rows, cols);
+}
+#define RMS_FORMS(RUN, T, V, ...)                                                                              \
+  if (f.warps == 1) switch (f.n) {                                                                            \
+      case 1: return RUN<T, V, 1, 1>(__VA_ARGS__);                                                            \
+      case 2: return RUN<T, V, 2, 1>(__VA_ARGS__);                                                            \
+      default: return RUN<T, V, 4, 1>(__VA_ARGS__);                                                           \
+    }                                                                                                         \
+  switch (f.n) {                                                                                              \
+    case 1: return RUN<T, V, 1, 8>(__VA_ARGS__);                                                              \
+    case 2: return RUN<T, V, 2, 8>(__VA_ARGS__);                                                              \
+    case 4: return RUN<T, V, 4, 8>(__VA_ARGS__);                                                              \
+    default: return RUN<T, V, 8, 8>(__VA_ARGS__);                                                             \
+  }
+
+template <typename T, int WHOLE>
+int rms_fwd_typed(const RmsForm &f, const void *a, const void *b, const void *gamma, void *xsum, void *y, float *rstd, int rows, int cols, float eps,
+                  int grid, int threads, cudaStream_t st) {
+  if (f.n == 0)
+    return ffk_launch(rms_fwd_wide_kernel<T>, grid, threads, 0, st, (const T *)a, (const T *)b, (const T *)gamma, (T *)xsum, (T *)y, rstd, rows, cols, eps);
+  if (f.v == 1) { RMS_FORMS(rms_fwd_run, T, 1, a, b, gamma, xsum, y, rstd, rows, cols, eps, grid, threads, st) }
+  RMS_FORMS(rms_fwd_run, T, WHOLE, a, b, gamma, xsum, y, rstd, rows, cols, eps, grid, threads, st)
+}
+template <typename T, int WHOLE>
+int rms_bwd_typed(const RmsForm &f, const void *dy, const void *h, const void *gamma, const float *rstd, const void *dsum, void *dh, float *partial,
+                  int rows, int cols, int grid, cudaStream_t st) {
+  if (f.n == 0)
+    return ffk_launch(rms_bwd_wide_kernel<T>, grid, 512, 0, st, (const T *)dy, (const T *)h, (const T *)gamma, rstd, (const T *)dsum, (T *)dh, partial,
+                      rows, cols);
+  if (f.v == 1) { RMS_FORMS(rms_bwd_run, T, 1, dy, h, gamma, rstd, dsum, dh, partial, rows, cols, grid, st) }
+  RMS_FORMS(rms_bwd_run, T, WHOLE, dy, h, gamma, rstd, dsum, dh, partial, rows, cols, grid, st)
+}
+
+}  // namespace
+
+// dt: 0 fp32, 1 bf16 (gamma too).  b, xsum, rstd may be null; b is the residual, xsum receives a + b.
+FFK_API int ffk_rmsnorm_fwd(const void *a, const void *b, const void *gamma, void *xsum, void *y, float *rstd, int rows, int cols, float eps, int dt,
+                            cudaStream_t st) {
+  if (dt != 0 && dt != 1) return -2;
+  if (rows <= 0) return 0;
+  if (cols <= 0) return -2;
+  const int es = dt == 1 ? 2 : 4;
+  FfkTraffic traffic((long long)rows * cols * es * (b ? xsum ? 4 : 3 : 2));
+  const RmsForm f = rms_form(rows, cols, es, rms_aligned(a) && rms_aligned(b) && rms_aligned(gamma) && rms_aligned(xsum) && rms_aligned(y));
+  int threads = 0;
+  const int grid = rms_fwd_grid(f, rows, threads);
+  return dt == 1 ? rms_fwd_typed<bf16, 8>(f, a, b, gamma, xsum, y, rstd, rows, cols, eps, grid, threads, st)
+                 : rms_fwd_typed<float, 4>(f, a, b, gamma, xsum, y, rstd, rows, cols, eps, grid, threads, st);
+}
+
+// floats of scratch: the partial rows of dgamma, for either form of the addresses
+FFK_API long long ffk_rmsnorm_bwd_scratch(int rows, int cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  long long most = 0;
+  for (int es = 2; es <= 4; es += 2)
+    for (int whole = 0; whole < 2; ++whole) {
+      const long long g = rms_bwd_grid(rms_form(rows, cols, es, whole), rows);
+      most = g > most ? g : most;
+    }
+  return most * cols;
+}
+
+// dsum, dgamma and (without dgamma) partial may be null
+FFK_API int ffk_rmsnorm_bwd(const void *dy, const void *h, const void *gamma, const float *rstd, const void *dsum, void *dh, void *dgamma, float *partial,
+                            int rows, int cols, int dt, int accumulate_params, cudaStream_t st) {
+  if (dt != 0 && dt != 1) return -2;
+  if (cols <= 0) return rows <= 0 ? 0 : -2;
+  const int es = dt == 1 ? 2 : 4;
+  int grid = 0;
+  if (dgamma && rows > 0 && !partial) return -2;
+  if (rows > 0) {
+    FfkTraffic traffic((long long)rows * cols * es * (dsum ? 4 : 3));
+    const RmsForm f = rms_form(rows, cols, es, rms_aligned(dy) && rms_aligned(h) && rms_aligned(gamma) && rms_aligned(dsum) && rms_aligned(dh));
+    grid = rms_bwd_grid(f, rows);
+    float *part = dgamma ? partial : nullptr;
+    const int e = dt == 1 ? rms_bwd_typed<bf16, 8>(f, dy, h, gamma, rstd, dsum, dh, part, rows, cols, grid, st)
+                          : rms_bwd_typed<float, 4>(f, dy, h, gamma, rstd, dsum, dh, part, rows, cols, grid, st);
+    if (e) return e;
+  }
+  if (!dgamma) return 0;
+  const dim3 block(32, 32);
+  if (dt == 1) return ffk_launch(rms_fold_kernel<bf16>, (cols + 31) / 32, block, 0, st, partial, grid, cols, (bf16 *)dgamma, accumulate_params);
+  return ffk_launch(rms_fold_kernel<float>, (cols + 31) / 32, block, 0, st, partial, grid, cols, (float *)dgamma, accumulate_params);
+}

@@ -1,0 +1,880 @@
+// span_attention_bwd.cu -- backward pass of attention over spans of keys (span_attention.cuh has the forward mathematics).
+//
+//   P = exp(x - lse),  delta_q = dO_q . O_q,  dS = P o (dO V^T - delta) o f'(u),  f'(u) = 1 - tanh(u / cap)^2 (1 without a cap)
+//   dV = P^T dO,   dK = scale dS^T Q  (both summed over the query heads of the key head),   dQ = scale dS K
+//
+// Two kernels recompute the scores, one per accumulator that has to stay on chip: seven products a tile pair where one kernel with all three
+// gradients needs five, but no gradient is added to in global memory, so there are no atomics, no 32-bit copy of dQ to clear and convert, and
+// the same inputs give the same bits.
+//   span_attn_prep_kernel  delta, and what each 128 queries of a batch row see together
+//   span_attn_dkv_kernel   CTA = 128 keys of one key head, over the query tiles that see them, of all its query heads.  Scores are produced
+//                          transposed (lanes = keys), so that P^T and dS^T, written back to tensor memory as bf16, are the A operands of
+//                          dV += P^T dO and dK += dS^T Q where they lie.
+//   span_attn_dq_kernel    CTA = 128 queries of one head, over the key tiles that they see; lanes = queries, dS is the A operand of dQ += dS K.
+// Roles in both (384 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 clears rows that nothing sees, warps 4-11 the element-wise
+// part (thread = one row and half of the columns); in the first kernel warp 3 brings each query tile's lse, delta and spans.
+//
+// Every wait is bounded (tcgen05.cuh).
+#include "span_attention.cuh"
+
+namespace {
+
+constexpr int SAB_THREADS = 384;
+
+// ---------------------------------------------------------------------------------------------- delta and summaries
+// L lanes (16 bytes each) per (row, head); blocks from `delta_blocks` on: a warp per 128 queries.  Summary: smallest first key and largest
+// last key of the queries that see any, largest first key and smallest last key of all (an empty span among them: nothing is seen by all).
+template <int L>
+__global__ void __launch_bounds__(256) span_attn_prep_kernel(const bf16 *dO, long long lddo, const bf16 *O, long long ldo, float *__restrict__ delta,
+                                                             int4 *__restrict__ summary, int delta_blocks, const SpanArgs p) {
+  pdl_entry();
+  const int lane = threadIdx.x & 31;
+  if ((int)blockIdx.x < delta_blocks) {
+    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / L, total = (long long)p.B * p.S * p.H;
+    const int c = (threadIdx.x % L) * 8;
+    const bool here = at < total;
+    const int h = (int)(at % p.H);
+    const long long row = at / p.H;
+    float s = 0.f;
+    if (here && c < p.D) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(dO + row * lddo + (long long)h * p.D + c);
+      const uint4 w = *reinterpret_cast<const uint4 *>(O + row * ldo + (long long)h * p.D + c);
+      const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = unpack_bf162(uu[i]), o = unpack_bf162(ww[i]);
+        s = fmaf(a.x, o.x, fmaf(a.y, o.y, s));
+      }
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (here && c == 0) {
+      const long long b = row / p.S, q = row - b * p.S;
+      delta[(b * p.H + h) * p.S + q] = s;
+    }
+    return;
+  }
+  const int nqt = (p.S + SA_T - 1) / SA_T;
+  const long long w = (long long)(blockIdx.x - delta_blocks) * 8 + (threadIdx.x >> 5);
+  if (w >= (long long)p.B * nqt) return;
+  const int b = (int)(w / nqt), i = (int)(w % nqt);
+  int lo = 0x7fffffff, hi = -1, lo_all = -1, hi_all = 0x7fffffff;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int q = i * SA_T + r * 32 + lane;
+    if (q < p.S) {
+      const int2 s = sa_span(p, b, q);
+      if (s.x <= s.y) {
+        lo = min(lo, s.x); hi = max(hi, s.y); lo_all = max(lo_all, s.x); hi_all = min(hi_all, s.y);
+      } else {
+        lo_all = 0x7fffffff;
+      }
+    }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo); hi = __reduce_max_sync(0xffffffffu, hi);
+  lo_all = __reduce_max_sync(0xffffffffu, lo_all); hi_all = __reduce_min_sync(0xffffffffu, hi_all);
+  if (lane == 0) summary[w] = make_int4(lo, hi, lo_all, hi_all);
+}
+
+// ---------------------------------------------------------------------------------------------- dK, dV
+template <int DT>
+struct DkvCfg {
+  static constexpr int PANELS = DT / 64;
+  static constexpr int TILE = SA_T * DT * 2;
+  static constexpr int NQ = 2;                                     // stages of (Q, dO)
+  static constexpr int OFF_K = 0;
+  static constexpr int OFF_V = OFF_K + TILE;
+  static constexpr int OFF_Q = OFF_V + TILE;                       // [NQ]
+  static constexpr int OFF_DO = OFF_Q + NQ * TILE;                 // [NQ]
+  static constexpr int OFF_LSE = OFF_DO + NQ * TILE;               // [NQ][128] float
+  static constexpr int OFF_DELTA = OFF_LSE + NQ * 512;             // [NQ][128] float
+  static constexpr int OFF_SPAN = OFF_DELTA + NQ * 512;            // [NQ][128] int2
+  static constexpr int OFF_BAR = OFF_SPAN + NQ * 1024;
+  static constexpr int SLACK = 1024;
+  static constexpr int SMEM = OFF_BAR + 256 + SLACK;
+  static constexpr int TM_S = 0, TM_DP = 128, TM_DK = 256, TM_DV = 256 + DT;
+  static_assert(SMEM <= 232448, "tiles exceed the shared memory of a CTA");
+};
+
+template <int DT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(SAB_THREADS, 1)
+span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const __grid_constant__ CUtensorMap tmDO, const SpanArgs p) {
+  using C = DkvCfg<DT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t *bars = (uint64_t *)(smem + C::OFF_BAR);
+  uint64_t *kv_full = bars;
+  uint64_t *qd_full = bars + 1;       // [2]
+  uint64_t *qd_ready = bars + 3;      // [2]
+  uint64_t *qd_empty = bars + 5;      // [2]
+  uint64_t *st_full = bars + 7;       // [2]
+  uint64_t *st_empty = bars + 9;      // [2] eight warps
+  uint64_t *s_full = bars + 11;
+  uint64_t *dp_full = bars + 12;
+  uint64_t *p_full = bars + 13;       // eight warps
+  uint64_t *ds_full = bars + 14;      // eight warps
+  uint64_t *dkv_full = bars + 15;
+  uint32_t *tmem_slot = (uint32_t *)(bars + 16);
+  volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+  int *walk = (int *)(tmem_slot + 2);                             // first and last query tile
+  volatile int *full_flag = (volatile int *)(tmem_slot + 4);      // [2] every query of the stage sees every key
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {
+    pdl_entry();
+    if (threadIdx.x == 0 && p.err) atomicCAS(p.err, 0, (int)FFK_ERR_BAD_ARG);
+    return;
+  }
+  const int group = p.H / p.KH;
+  const int bh = blockIdx.x % (p.B * p.KH);
+  const int kb = blockIdx.x / (p.B * p.KH);                       // the first keys, which most queries see under a causal mask, first
+  const int kh = bh % p.KH, b = bh / p.KH;
+  const int k0 = kb * SA_T, k1 = min(k0 + SA_T, p.S) - 1;
+  const int nqt = (p.S + SA_T - 1) / SA_T;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int s = 0; s < 2; ++s) { mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 8); }
+    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_full, 8); mbar_init(ds_full, 8); mbar_init(dkv_full, 1);
+    *abort_flag = 0;
+    walk[0] = 0x7fffffff;
+    walk[1] = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_entry();
+  __syncthreads();
+  const int4 *summary = p.summary + (long long)b * nqt;
+  for (int i = threadIdx.x; i < nqt; i += SAB_THREADS) {
+    const int4 s = summary[i];
+    if (s.x <= k1 && s.y >= k0) {
+      atomicMin(&walk[0], i);
+      atomicMax(&walk[1], i);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int i0 = walk[0], ni = walk[1] < 0 ? 0 : walk[1] - i0 + 1;
+  const int n = ni * group;                                       // steps: (head, query tile)
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0 && n > 0) {
+      mbar_expect_tx(kv_full, 2 * C::TILE);
+#pragma unroll
+      for (int c = 0; c < C::PANELS; ++c) {
+        tma_load_4d(smem_u32(smem + C::OFF_K + c * SA_PANEL), &tmK, kv_full, c * 64, k0, kh, b);
+        tma_load_4d(smem_u32(smem + C::OFF_V + c * SA_PANEL), &tmV, kv_full, c * 64, k0, kh, b);
+      }
+      int g = 0, i = i0;
+      for (int it = 0; it < n; ++it) {
+        const int s = it & 1;
+        if (!mbar_wait(&qd_empty[s], ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_PRODUCER)) break;
+        mbar_expect_tx(&qd_full[s], 2 * C::TILE);
+#pragma unroll
+        for (int c = 0; c < C::PANELS; ++c) {
+          tma_load_4d(smem_u32(smem + C::OFF_Q + s * C::TILE + c * SA_PANEL), &tmQ, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
+          tma_load_4d(smem_u32(smem + C::OFF_DO + s * C::TILE + c * SA_PANEL), &tmDO, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
+        }
+        if (++i == i0 + ni) { i = i0; ++g; }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer: the whole warp runs, one lane issues
+    const bool leader = elect_one();
+    const uint64_t dk = make_smem_desc(smem_u32(smem + C::OFF_K), 16, 1024), dv = make_smem_desc(smem_u32(smem + C::OFF_V), 16, 1024);
+    const uint64_t q_k0 = make_smem_desc(smem_u32(smem + C::OFF_Q), 16, 1024), q_n0 = make_smem_desc(smem_u32(smem + C::OFF_Q), SA_PANEL, 1024);
+    const uint64_t o_k0 = make_smem_desc(smem_u32(smem + C::OFF_DO), 16, 1024), o_n0 = make_smem_desc(smem_u32(smem + C::OFF_DO), SA_PANEL, 1024);
+    const int ksteps = (p.D + 15) / 16;
+    const uint32_t id_s = sa_idesc(128, SA_T, 0, 0), id_g = sa_idesc(128, ksteps * 16, 0, 1);
+    // [keys x queries] = A (keys x D) B (queries x D)^T
+    auto issue_t = [&](uint32_t d, uint64_t a, uint64_t bq, uint64_t *bar) {
+      if (leader) {
+        tc_mma_bf16<false>(d, a, bq, id_s);
+        for (int s = 1; s < ksteps; ++s) {
+          const uint32_t off = (uint32_t)((s >> 2) * SA_PANEL + (s & 3) * 32);
+          tc_mma_bf16<true>(d, desc_advance(a, off), desc_advance(bq, off), id_s);
+        }
+        tc_commit(bar);
+      }
+      __syncwarp();
+    };
+    // [keys x D] += A (bf16 in tensor memory: keys x queries, 64 queries in the first 32 columns of either half) B (queries x D)
+    auto issue_g = [&](uint32_t d, uint32_t a, uint64_t bn, bool first) {
+      if (leader) {
+        if (first) tc_mma_ts_bf16<false>(d, a, bn, id_g);
+        else tc_mma_ts_bf16<true>(d, a, bn, id_g);
+#pragma unroll
+        for (int s = 1; s < SA_T / 16; ++s)
+          tc_mma_ts_bf16<true>(d, a + (uint32_t)((s >> 2) * 64 + (s & 3) * 8), desc_advance(bn, (uint32_t)(s * 2048)), id_g);
+      }
+      __syncwarp();
+    };
+    auto wait_qd = [&](int it) -> bool {
+      return mbar_wait_warp(&qd_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
+             mbar_wait_warp(&qd_ready[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    };
+    bool ok = n > 0 && mbar_wait_warp(kv_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && wait_qd(0);
+    if (ok) {
+      tc_fence_after();
+      issue_t(tmem_base + C::TM_S, dk, q_k0, s_full);
+      issue_t(tmem_base + C::TM_DP, dv, o_k0, dp_full);
+    }
+    for (int it = 0; it < n && ok; ++it) {
+      const uint32_t ph = (uint32_t)it & 1u, off = (uint32_t)((it & 1) * C::TILE), next = (uint32_t)(((it + 1) & 1) * C::TILE);
+      ok = mbar_wait_warp(p_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+      if (!ok) break;
+      tc_fence_after();
+      issue_g(tmem_base + C::TM_DV, tmem_base + C::TM_S, desc_advance(o_n0, off), it == 0);
+      if (it + 1 < n) {                   // the next scores take the columns that P^T is read from: products run in issue order
+        ok = wait_qd(it + 1);
+        if (!ok) break;
+        tc_fence_after();
+        issue_t(tmem_base + C::TM_S, dk, desc_advance(q_k0, next), s_full);
+      }
+      ok = mbar_wait_warp(ds_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+      if (!ok) break;
+      tc_fence_after();
+      issue_g(tmem_base + C::TM_DK, tmem_base + C::TM_DP, desc_advance(q_n0, off), it == 0);
+      if (leader) tc_commit(&qd_empty[it & 1]);
+      __syncwarp();
+      if (it + 1 < n) issue_t(tmem_base + C::TM_DP, dv, desc_advance(o_k0, next), dp_full);
+    }
+    if (ok && leader) tc_commit(dkv_full);
+    __syncwarp();
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ rows of Q and dO that see none of these keys
+    bool ok = true;
+    int i = i0;
+    for (int it = 0; it < n && ok; ++it) {
+      const int s = it & 1;
+      const int4 all = summary[i];
+      uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+      if (all.z > k0 || all.w < k1) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int q = i * SA_T + w * 32 + lane;
+          bool sees = true;                                       // rows behind the sequence arrive as zeros
+          if (q < p.S) {
+            const int2 sp = sa_span(p, b, q);
+            sees = sp.x <= sp.y && sp.x <= k1 && sp.y >= k0;
+          }
+          keep[w] = __ballot_sync(0xffffffffu, sees);
+        }
+      }
+      ok = sa_wait(&qd_full[s], (uint32_t)(it >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+        sa_clear_rows(smem + C::OFF_Q + s * C::TILE, C::PANELS, keep, lane);
+        sa_clear_rows(smem + C::OFF_DO + s * C::TILE, C::PANELS, keep, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      sa_warp_arrive(&qd_ready[s], lane);
+      if (++i == i0 + ni) i = i0;
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ statistics of each query tile
+    bool ok = true;
+    int g = 0, i = i0;
+    for (int it = 0; it < n && ok; ++it) {
+      const int s = it & 1;
+      float *lse = (float *)(smem + C::OFF_LSE) + s * SA_T, *dlt = (float *)(smem + C::OFF_DELTA) + s * SA_T;
+      int2 *sp = (int2 *)(smem + C::OFF_SPAN) + s * SA_T;
+      const long long base = ((long long)b * p.H + kh * group + g) * p.S;
+      const int4 all = summary[i];
+      float vl[4], vd[4];
+      int2 vs[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int q = i * SA_T + r * 32 + lane;
+        // a query that sees nothing, or does not exist: probabilities of 0
+        vl[r] = INFINITY; vd[r] = 0.f; vs[r] = make_int2(1, 0);
+        if (q < p.S) {
+          const int2 t = sa_span(p, b, q);
+          if (t.x <= t.y) {
+            vs[r] = t;
+            vl[r] = p.lse[base + q];
+            vd[r] = p.delta[base + q];
+          }
+        }
+      }
+      ok = sa_wait(&st_empty[s], ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        lse[r * 32 + lane] = vl[r];
+        dlt[r * 32 + lane] = vd[r];
+        sp[r * 32 + lane] = vs[r];
+      }
+      if (lane == 0) full_flag[s] = all.z <= k0 && all.w >= k1;
+      sa_warp_arrive(&st_full[s], lane);
+      if (++i == i0 + ni) { i = i0; ++g; }
+    }
+  } else {
+    // ------------------------------------------------------------------ P^T and dS^T: thread = key x 64 of the tile's queries
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int r = quarter * 32 + lane, key = k0 + r;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
+    bool ok = true;
+    int g = 0, i = i0;
+    for (int it = 0; it < n && ok; ++it) {
+      const int s = it & 1;
+      const uint32_t ph = (uint32_t)it & 1u;
+      const float *lse = (const float *)(smem + C::OFF_LSE) + s * SA_T + half * 64, *dlt = (const float *)(smem + C::OFF_DELTA) + s * SA_T + half * 64;
+      const int4 *sp = (const int4 *)(smem + C::OFF_SPAN) + (s * SA_T + half * 64) / 2;
+      ok = sa_wait(&st_full[s], (uint32_t)(it >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE) &&
+           sa_wait(s_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      tc_fence_after();
+      const bool full = full_flag[s] != 0;
+      uint32_t x[64];
+      tmem_ld32(lane_base + C::TM_S, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+      tmem_ld32(lane_base + C::TM_S + 32u, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
+      tmem_ld_wait();
+      if (CAP && !full) {                 // what masked scores hold does not choose the way tanh is taken
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          const int4 t = sp[c / 2];
+          if (key < t.x || key > t.y) x[c] = 0u;
+          if (key < t.z || key > t.w) x[c + 1] = 0u;
+        }
+      }
+      const float f = sa_capped<64, CAP>(x, p, true);
+      const pair32 ff = pair_of(f, f);
+      uint32_t pk[32];
+      {
+        float slope = 0.f;
+        if constexpr (BIAS) slope = -p.slopes[kh * group + g] * SA_LOG2E;
+        const pair32 ss = pair_of(slope, slope), two = pair_of(2.f, 2.f);
+        const float d0 = (float)(i * SA_T + half * 64 - key);
+        pair32 d = pair_of(d0, d0 + 1.f);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 w = *reinterpret_cast<const float4 *>(lse + c);
+          float e[4];
+#pragma unroll
+          for (int u = 0; u < 4; u += 2) {
+            pair32 y = pair_fma(pair_get(&x[c + u]), ff, u == 0 ? pair_of(-w.x, -w.y) : pair_of(-w.z, -w.w));
+            if constexpr (BIAS) {
+              y = pair_fma(ss, d & 0x7fffffff7fffffffull, y);
+              d = pair_add(d, two);
+            }
+            pair_to(y, e[u], e[u + 1]);
+          }
+          if (!full) {
+            const int4 a = sp[c / 2], z = sp[c / 2 + 1];
+            if (key < a.x || key > a.y) e[0] = -INFINITY;
+            if (key < a.z || key > a.w) e[1] = -INFINITY;
+            if (key < z.x || key > z.y) e[2] = -INFINITY;
+            if (key < z.z || key > z.w) e[3] = -INFINITY;
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) e[u] = sa_exp2(e[u]);
+          pk[c >> 1] = pack_bf162(e[0], e[1]);
+          pk[(c >> 1) + 1] = pack_bf162(e[2], e[3]);
+          // what dS needs of P: times the cap's derivative
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if constexpr (CAP) {
+              const float t = __uint_as_float(x[c + u]);
+              const float k = e[u] * fmaf(-t, t, 1.f);
+              x[c + u] = __float_as_uint(k);
+            } else {
+              x[c + u] = __float_as_uint(e[u]);
+            }
+          }
+        }
+      }
+      tmem_st32(lane_base + C::TM_S, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      sa_warp_arrive(p_full, lane);
+      ok = sa_wait(dp_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int hc = 0; hc < 64; hc += 32) {
+        uint32_t y[32];
+        tmem_ld32(lane_base + C::TM_DP + (uint32_t)hc, y);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 w = *reinterpret_cast<const float4 *>(dlt + hc + c);
+          float e[4];
+          pair_to(pair_mul(pair_get(&x[hc + c]), pair_add(pair_get(&y[c]), pair_of(-w.x, -w.y))), e[0], e[1]);
+          pair_to(pair_mul(pair_get(&x[hc + c + 2]), pair_add(pair_get(&y[c + 2]), pair_of(-w.z, -w.w))), e[2], e[3]);
+          if (!full) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (__uint_as_float(x[hc + c + u]) == 0.f) e[u] = 0.f;            // whatever dO and delta hold there
+          }
+          pk[(hc + c) >> 1] = pack_bf162(e[0], e[1]);
+          pk[((hc + c) >> 1) + 1] = pack_bf162(e[2], e[3]);
+        }
+      }
+      tmem_st32(lane_base + C::TM_DP, pk);
+      tmem_st_wait();
+      tc_fence_before();
+      sa_warp_arrive(ds_full, lane);
+      if (lane == 0) mbar_arrive(&st_empty[s]);
+      if (++i == i0 + ni) { i = i0; ++g; }
+    }
+    if (ok && n > 0) {
+      ok = sa_wait(dkv_full, 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      tc_fence_after();
+    }
+    if (ok) {
+      constexpr int DH = DT / 2;
+      const long long row = (long long)b * p.S + key;
+      const uint32_t t_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      for (int w = 0; w < 2; ++w) {
+        const float f = w == 0 ? p.scale : 1.f;
+        bf16 *orow = (w == 0 ? p.dK + row * p.lddk : p.dV + row * p.lddv) + (long long)kh * p.D + half * DH;
+#pragma unroll 1
+        for (int c = 0; c < DH / 32; ++c) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld32(t_base + (uint32_t)((w == 0 ? C::TM_DK : C::TM_DV) + half * DH + c * 32), o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int u = 0; u < 32; ++u) o[u] = 0u;
+          }
+          if (key < p.S) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (half * DH + c * 32 + 8 * u < p.D)
+                *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) =
+                    make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * f, __uint_as_float(o[8 * u + 1]) * f),
+                               pack_bf162(__uint_as_float(o[8 * u + 2]) * f, __uint_as_float(o[8 * u + 3]) * f),
+                               pack_bf162(__uint_as_float(o[8 * u + 4]) * f, __uint_as_float(o[8 * u + 5]) * f),
+                               pack_bf162(__uint_as_float(o[8 * u + 6]) * f, __uint_as_float(o[8 * u + 7]) * f));
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- dQ
+template <int DT>
+struct DqCfg {
+  static constexpr int PANELS = DT / 64;
+  static constexpr int TILE = SA_T * DT * 2;
+  static constexpr int NK = 3, NV = 2;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_DO = OFF_Q + TILE;
+  static constexpr int OFF_K = OFF_DO + TILE;
+  static constexpr int OFF_V = OFF_K + NK * TILE;
+  static constexpr int OFF_SPAN = OFF_V + NV * TILE;               // [128] int2
+  static constexpr int OFF_RANGE = OFF_SPAN + 1024;                // [4] int2
+  static constexpr int OFF_BAR = OFF_RANGE + 32;
+  static constexpr int SLACK = 1024;
+  static constexpr int SMEM = OFF_BAR + 256 + SLACK;
+  static constexpr int TM_S = 0, TM_DP = 256, TM_DQ = 384;         // two score buffers
+  static_assert(SMEM <= 232448, "tiles exceed the shared memory of a CTA");
+};
+
+template <int DT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(SAB_THREADS, 1)
+span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ CUtensorMap tmDO, const SpanArgs p) {
+  using C = DqCfg<DT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  int2 *span = (int2 *)(smem + C::OFF_SPAN);
+  int2 *range = (int2 *)(smem + C::OFF_RANGE);
+  uint64_t *bars = (uint64_t *)(smem + C::OFF_BAR);
+  uint64_t *q_full = bars;
+  uint64_t *k_full = bars + 1;        // [NK]
+  uint64_t *k_ready = bars + 4;       // [NK]
+  uint64_t *k_empty = bars + 7;       // [NK]
+  uint64_t *v_full = bars + 10;       // [NV]
+  uint64_t *v_empty = bars + 12;      // [NV]
+  uint64_t *s_full = bars + 14;       // [2]
+  uint64_t *dp_full = bars + 16;
+  uint64_t *dp_free = bars + 17;      // eight warps
+  uint64_t *ds_full = bars + 18;      // eight warps
+  uint64_t *dq_full = bars + 19;
+  uint32_t *tmem_slot = (uint32_t *)(bars + 20);
+  volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {
+    pdl_entry();
+    if (threadIdx.x == 0 && p.err) atomicCAS(p.err, 0, (int)FFK_ERR_BAD_ARG);
+    return;
+  }
+  const int nqb = (p.S + SA_T - 1) / SA_T;
+  const int bh = blockIdx.x % (p.B * p.H);
+  const int qb = nqb - 1 - blockIdx.x / (p.B * p.H);
+  const int h = bh % p.H, b = bh / p.H, kh = h / (p.H / p.KH);
+  const int q0 = qb * SA_T;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_ready[s], 1); mbar_init(&k_empty[s], 1); }
+    for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+    mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1); mbar_init(dp_free, 8); mbar_init(ds_full, 8); mbar_init(dq_full, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_entry();
+  if (threadIdx.x < SA_T) {
+    const int q = q0 + (int)threadIdx.x;
+    const int2 s = q < p.S ? sa_span(p, b, q) : make_int2(1, 0);
+    span[threadIdx.x] = s;
+    const bool sees = s.x <= s.y;
+    const int lo = __reduce_min_sync(0xffffffffu, sees ? s.x : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, sees ? s.y : -1);
+    if (lane == 0) range[warp] = make_int2(lo, hi);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  int first = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) { first = min(first, range[w].x); last = max(last, range[w].y); }
+  const int j0 = last < 0 ? 0 : first / SA_T;
+  const int n = last < 0 ? 0 : last / SA_T - j0 + 1;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0 && n > 0) {
+      mbar_expect_tx(q_full, 2 * C::TILE);
+#pragma unroll
+      for (int c = 0; c < C::PANELS; ++c) {
+        tma_load_4d(smem_u32(smem + C::OFF_Q + c * SA_PANEL), &tmQ, q_full, c * 64, q0, h, b);
+        tma_load_4d(smem_u32(smem + C::OFF_DO + c * SA_PANEL), &tmDO, q_full, c * 64, q0, h, b);
+      }
+      int ki = 0, vi = 0;
+      uint64_t t0 = ffk_globaltimer();
+      uint32_t spins = 0;
+      while (ki < n || vi < n) {
+        bool progress = false;
+        if (ki < n) {
+          const int s = ki % C::NK;
+          if (mbar_try_wait(&k_empty[s], ((uint32_t)(ki / C::NK) & 1u) ^ 1u)) {
+            mbar_expect_tx(&k_full[s], C::TILE);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              tma_load_4d(smem_u32(smem + C::OFF_K + s * C::TILE + c * SA_PANEL), &tmK, &k_full[s], c * 64, (j0 + ki) * SA_T, kh, b);
+            ++ki;
+            progress = true;
+          }
+        }
+        if (vi < n) {
+          const int s = vi % C::NV;
+          if (mbar_try_wait(&v_empty[s], ((uint32_t)(vi / C::NV) & 1u) ^ 1u)) {
+            mbar_expect_tx(&v_full[s], C::TILE);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              tma_load_4d(smem_u32(smem + C::OFF_V + s * C::TILE + c * SA_PANEL), &tmV, &v_full[s], c * 64, (j0 + vi) * SA_T, kh, b);
+            ++vi;
+            progress = true;
+          }
+        }
+        if (progress) {
+          t0 = ffk_globaltimer();
+        } else if ((++spins & 63u) == 0) {
+          if (*abort_flag) break;
+          if (ffk_globaltimer() - t0 > WAIT_LIMIT_NS) {
+            *abort_flag = 1;
+            if (p.err) atomicCAS(p.err, 0, (int)FFK_ERR_TIMEOUT_PRODUCER);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    const uint64_t dq = make_smem_desc(smem_u32(smem + C::OFF_Q), 16, 1024), dd = make_smem_desc(smem_u32(smem + C::OFF_DO), 16, 1024);
+    const uint64_t k_k0 = make_smem_desc(smem_u32(smem + C::OFF_K), 16, 1024), k_n0 = make_smem_desc(smem_u32(smem + C::OFF_K), SA_PANEL, 1024);
+    const uint64_t v_k0 = make_smem_desc(smem_u32(smem + C::OFF_V), 16, 1024);
+    const int ksteps = (p.D + 15) / 16;
+    const uint32_t id_s = sa_idesc(128, SA_T, 0, 0), id_g = sa_idesc(128, ksteps * 16, 0, 1);
+    auto issue_t = [&](uint32_t d, uint64_t a, uint64_t bk) {
+      if (leader) {
+        tc_mma_bf16<false>(d, a, bk, id_s);
+        for (int s = 1; s < ksteps; ++s) {
+          const uint32_t off = (uint32_t)((s >> 2) * SA_PANEL + (s & 3) * 32);
+          tc_mma_bf16<true>(d, desc_advance(a, off), desc_advance(bk, off), id_s);
+        }
+      }
+    };
+    auto issue_s = [&](int i) -> bool {
+      const int s = i % C::NK;
+      if (!mbar_wait_warp(&k_full[s], (uint32_t)(i / C::NK) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) ||
+          !mbar_wait_warp(&k_ready[s], (uint32_t)(i / C::NK) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA))
+        return false;
+      tc_fence_after();
+      issue_t(tmem_base + (uint32_t)(C::TM_S + (i & 1) * SA_T), dq, desc_advance(k_k0, (uint32_t)(s * C::TILE)));
+      if (leader) tc_commit(&s_full[i & 1]);
+      __syncwarp();
+      return true;
+    };
+    auto issue_dp = [&](int i) -> bool {
+      const int s = i % C::NV;
+      if (!mbar_wait_warp(&v_full[s], (uint32_t)(i / C::NV) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA)) return false;
+      tc_fence_after();
+      issue_t(tmem_base + (uint32_t)C::TM_DP, dd, desc_advance(v_k0, (uint32_t)(s * C::TILE)));
+      if (leader) {
+        tc_commit(dp_full);
+        tc_commit(&v_empty[s]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = n > 0 && mbar_wait_warp(q_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && issue_s(0) && issue_dp(0);
+    for (int i = 0; i < n && ok; ++i) {
+      const uint32_t ph = (uint32_t)i & 1u;
+      if (i + 1 < n) {
+        ok = issue_s(i + 1) && mbar_wait_warp(dp_free, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && issue_dp(i + 1);
+        if (!ok) break;
+      }
+      ok = mbar_wait_warp(ds_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+        const uint32_t d = tmem_base + (uint32_t)C::TM_DQ, a = tmem_base + (uint32_t)(C::TM_S + (i & 1) * SA_T);
+        const uint64_t bn = desc_advance(k_n0, (uint32_t)((i % C::NK) * C::TILE));
+        if (i == 0) tc_mma_ts_bf16<false>(d, a, bn, id_g);
+        else tc_mma_ts_bf16<true>(d, a, bn, id_g);
+#pragma unroll
+        for (int s = 1; s < SA_T / 16; ++s)
+          tc_mma_ts_bf16<true>(d, a + (uint32_t)((s >> 2) * 64 + (s & 3) * 8), desc_advance(bn, (uint32_t)(s * 2048)), id_g);
+        tc_commit(&k_empty[i % C::NK]);
+        if (i + 1 == n) tc_commit(dq_full);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ rows of K that no query of the block sees
+    bool ok = true;
+    for (int i = 0; i < n && ok; ++i) {
+      const int k0 = (j0 + i) * SA_T, s = i % C::NK;
+      uint32_t keep[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int2 t = span[r * 32 + lane];
+        if (t.x <= t.y) sa_add_bits(keep, t.x - k0, t.y - k0);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) keep[w] = __reduce_or_sync(0xffffffffu, keep[w]);
+      ok = sa_wait(&k_full[s], (uint32_t)(i / C::NK) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+        sa_clear_rows(smem + C::OFF_K + s * C::TILE, C::PANELS, keep, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      sa_warp_arrive(&k_ready[s], lane);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ dS: thread = query x 64 of the tile's keys
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int r = quarter * 32 + lane, q = q0 + r;
+    const int2 mine = span[r];
+    const bool empty = mine.x > mine.y;
+    const int lo = empty ? -1 : mine.x, hi = empty ? 0x7ffffff0 : mine.y;      // see the forward kernel
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
+    const float slope = BIAS ? -p.slopes[h] * SA_LOG2E : 0.f;
+    const long long stat = ((long long)b * p.H + h) * p.S + q;
+    const float neg_lse = empty ? -INFINITY : -p.lse[stat], neg_delta = empty ? 0.f : -p.delta[stat];
+    const pair32 nl = pair_of(neg_lse, neg_lse), nd = pair_of(neg_delta, neg_delta);
+    bool ok = true;
+    for (int i = 0; i < n && ok; ++i) {
+      const uint32_t ph = (uint32_t)i & 1u;
+      const int k0 = (j0 + i) * SA_T + half * 64;
+      const uint32_t t_s = lane_base + (uint32_t)(C::TM_S + (i & 1) * SA_T);
+      ok = sa_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[64];
+      tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+      tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
+      tmem_ld_wait();
+      const bool full = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + 63);
+      const int a = lo - k0, w = hi - lo;
+      if (CAP && !full) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if ((unsigned)(c - a) > (unsigned)w) x[c] = 0u;
+      }
+      const float f = sa_capped<64, CAP>(x, p, !empty);
+      const pair32 ff = pair_of(f, f), ss = pair_of(slope, slope), two = pair_of(2.f, 2.f);
+      pair32 d = pair_of((float)(k0 - q), (float)(k0 - q + 1));
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        float e[4];
+#pragma unroll
+        for (int u = 0; u < 4; u += 2) {
+          pair32 y = pair_fma(pair_get(&x[c + u]), ff, nl);
+          if constexpr (BIAS) {
+            y = pair_fma(ss, d & 0x7fffffff7fffffffull, y);
+            d = pair_add(d, two);
+          }
+          pair_to(y, e[u], e[u + 1]);
+        }
+        if (!full) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if ((unsigned)(c + u - a) > (unsigned)w) e[u] = -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          e[u] = sa_exp2(e[u]);
+          if constexpr (CAP) {
+            const float t = __uint_as_float(x[c + u]);
+            const float k = e[u] * fmaf(-t, t, 1.f);
+            x[c + u] = __float_as_uint(k);
+          } else {
+            x[c + u] = __float_as_uint(e[u]);
+          }
+        }
+      }
+      ok = sa_wait(dp_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t y[64];
+      tmem_ld32(lane_base + C::TM_DP, *reinterpret_cast<uint32_t(*)[32]>(&y[0]));
+      tmem_ld32(lane_base + C::TM_DP + 32u, *reinterpret_cast<uint32_t(*)[32]>(&y[32]));
+      tmem_ld_wait();
+      tc_fence_before();
+      sa_warp_arrive(dp_free, lane);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float e0, e1;
+        pair_to(pair_mul(pair_get(&x[c]), pair_add(pair_get(&y[c]), nd)), e0, e1);
+        if (!full) {
+          if (__uint_as_float(x[c]) == 0.f) e0 = 0.f;
+          if (__uint_as_float(x[c + 1]) == 0.f) e1 = 0.f;
+        }
+        y[c >> 1] = pack_bf162(e0, e1);
+      }
+      tmem_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&y[0]));
+      tmem_st_wait();
+      tc_fence_before();
+      sa_warp_arrive(ds_full, lane);
+    }
+    if (ok && n > 0) {
+      ok = sa_wait(dq_full, 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      tc_fence_after();
+    }
+    if (ok) {
+      constexpr int DH = DT / 2;
+      const uint32_t t_q = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(C::TM_DQ + half * DH);
+      bf16 *orow = p.dQ + ((long long)b * p.S + q) * p.lddq + (long long)h * p.D + half * DH;
+#pragma unroll 1
+      for (int c = 0; c < DH / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(t_q + (uint32_t)(c * 32), o);
+          tmem_ld_wait();
+        }
+        if (q < p.S) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (half * DH + c * 32 + 8 * u < p.D) {
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (!empty)
+                v = make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * p.scale, __uint_as_float(o[8 * u + 1]) * p.scale),
+                               pack_bf162(__uint_as_float(o[8 * u + 2]) * p.scale, __uint_as_float(o[8 * u + 3]) * p.scale),
+                               pack_bf162(__uint_as_float(o[8 * u + 4]) * p.scale, __uint_as_float(o[8 * u + 5]) * p.scale),
+                               pack_bf162(__uint_as_float(o[8 * u + 6]) * p.scale, __uint_as_float(o[8 * u + 7]) * p.scale));
+              *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) = v;
+            }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+struct SpanMaps { CUtensorMap q, k, v, dout; };
+
+template <int DT, bool CAP, bool BIAS>
+int launch_bwd(const SpanMaps &m, const SpanArgs &a, cudaStream_t st) {
+  static unsigned long long done_kv = 0, done_q = 0;
+  cudaError_t e = ffk_allow_smem(span_attn_dkv_kernel<DT, CAP, BIAS>, DkvCfg<DT>::SMEM, done_kv);
+  if (e != cudaSuccess) return (int)e;
+  e = ffk_allow_smem(span_attn_dq_kernel<DT, CAP, BIAS>, DqCfg<DT>::SMEM, done_q);
+  if (e != cudaSuccess) return (int)e;
+  const long long tiles = (a.S + SA_T - 1) / SA_T;
+  int r = ffk_launch(span_attn_dkv_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.KH), SAB_THREADS, DkvCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, a);
+  if (r) return r;
+  return ffk_launch(span_attn_dq_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.H), SAB_THREADS, DqCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, a);
+}
+
+long long delta_floats(long long B, long long H, long long S) { return (B * H * S + 3) / 4 * 4; }
+
+}  // namespace
+
+FFK_API long long ffk_span_attention_bwd_scratch_floats(int B, int H, int S) {
+  if (B <= 0 || H <= 0 || S <= 0) return 0;
+  return delta_floats(B, H, S) + 4ll * B * ((S + SA_T - 1) / SA_T);
+}
+
+FFK_API int ffk_span_attention_bwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
+  if (d->B <= 0 || d->H <= 0 || d->S <= 0) return 0;
+  if (!sa_shape_ok(d)) return -2;
+  if (!sa_aligned(d->Q, d->ldq) || !sa_aligned(d->K, d->ldk) || !sa_aligned(d->V, d->ldv) || !sa_aligned(d->O, d->ldo) || !sa_aligned(d->dO, d->lddo) ||
+      !sa_aligned(d->dQ, d->lddq) || !sa_aligned(d->dK, d->lddk) || !sa_aligned(d->dV, d->lddv) || (((uintptr_t)d->scratch) & 15) || !d->lse)
+    return -2;
+  const long long tiles = (d->S + SA_T - 1) / SA_T, rows = (long long)d->B * d->S * d->H;
+  const int lanes = d->D <= 64 ? 8 : 16;
+  const long long delta_blocks = (rows * lanes + 255) / 256, sum_blocks = (d->B * tiles + 7) / 8;
+  if (tiles * d->B * d->H > 0x7fffffffll || delta_blocks + sum_blocks > 0x7fffffffll) return -2;
+  SpanMaps m;
+  int r;
+  if ((r = sa_head_map(&m.q, d->Q, d->D, d->S, d->ldq, d->H, d->B))) return r;
+  if ((r = sa_head_map(&m.k, d->K, d->D, d->S, d->ldk, d->KH, d->B))) return r;
+  if ((r = sa_head_map(&m.v, d->V, d->D, d->S, d->ldv, d->KH, d->B))) return r;
+  if ((r = sa_head_map(&m.dout, d->dO, d->D, d->S, d->lddo, d->H, d->B))) return r;
+  SpanArgs a = {};
+  sa_args(d, a, ffk_span_attention_err());
+  float *delta = d->scratch;
+  int4 *summary = reinterpret_cast<int4 *>(d->scratch + delta_floats(d->B, d->H, d->S));
+  a.delta = delta;
+  a.summary = summary;
+  a.dQ = (bf16 *)d->dQ; a.lddq = d->lddq; a.dK = (bf16 *)d->dK; a.lddk = d->lddk; a.dV = (bf16 *)d->dV; a.lddv = d->lddv;
+  FfkTraffic traffic((long long)d->B * d->S * d->D * 4 * (d->H + d->KH));
+  const unsigned blocks = (unsigned)(delta_blocks + sum_blocks);
+  r = lanes == 8 ? ffk_launch(span_attn_prep_kernel<8>, blocks, 256, 0, st, (const bf16 *)d->dO, d->lddo, (const bf16 *)d->O, d->ldo, delta, summary,
+                              (int)delta_blocks, a)
+                 : ffk_launch(span_attn_prep_kernel<16>, blocks, 256, 0, st, (const bf16 *)d->dO, d->lddo, (const bf16 *)d->O, d->ldo, delta, summary,
+                              (int)delta_blocks, a);
+  if (r) return r;
+  const bool cap = d->cap > 0.f, bias = d->slopes != nullptr;
+  if (d->D <= 64) {
+    if (cap) return bias ? launch_bwd<64, true, true>(m, a, st) : launch_bwd<64, true, false>(m, a, st);
+    return bias ? launch_bwd<64, false, true>(m, a, st) : launch_bwd<64, false, false>(m, a, st);
+  }
+  if (cap) return bias ? launch_bwd<128, true, true>(m, a, st) : launch_bwd<128, true, false>(m, a, st);
+  return bias ? launch_bwd<128, false, true>(m, a, st) : launch_bwd<128, false, false>(m, a, st);
+}

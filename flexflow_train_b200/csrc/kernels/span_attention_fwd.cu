@@ -1,0 +1,467 @@
+// span_attention_fwd.cu -- forward pass of attention over spans of keys (span_attention.cuh has the mathematics).
+//
+// A CTA (384 threads) takes one or two tiles of 128 queries of one (batch row, head) and walks over the key tiles from the first
+// to the last that any of its queries sees; scores and probabilities exist in tensor memory and registers only:
+//   warp 0      TMA producer: Q once, then the K and V tiles through rings
+//   warp 1      MMA issuer: S_t = Q_t K_j^T (two products ahead of nothing but the other tile's softmax), O_t += P_t V_j
+//   warp 2      clears the rows of V_j that no query of the CTA sees (only where a tile holds such rows)
+//   warps 4-11  softmax, thread = query row: four warps per query tile.  P_t overwrites the first columns of S_t as bf16 and is the A operand of
+//               the second product from there.  The reference maximum of a row moves only when the true one has grown by 2^8, and then the
+//               thread rescales its row of O in tensor memory: the common step has no correction pass.
+// While one tile's softmax runs, the tensor core works on the other tile's products.
+//
+// Every wait is bounded (tcgen05.cuh).
+#include "span_attention.cuh"
+
+namespace {
+
+constexpr int SAF_THREADS = 384;
+constexpr float SAF_GAP = 8.f;          // log-2 units by which a row's maximum may exceed the reference in use
+
+template <int DT>                       // columns of a tile: 64 or 128
+struct SafCfg {
+  static constexpr int PANELS = DT / 64;
+  static constexpr int TILE = SA_T * DT * 2;
+  static constexpr int NK = 2, NV = DT == 128 ? 3 : 4;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + 2 * TILE;
+  static constexpr int OFF_V = OFF_K + NK * TILE;
+  static constexpr int OFF_SPAN = OFF_V + NV * TILE;              // [256] int2
+  static constexpr int OFF_RANGE = OFF_SPAN + 256 * 8;            // [8] int2: smallest first and largest last of 32 rows
+  static constexpr int OFF_BAR = OFF_RANGE + 64;
+  static constexpr int SMEM = OFF_BAR + 256 + 640;                // the base is aligned to 1024 (checked in the kernel)
+  static constexpr int SLACK = 640;
+  static_assert(SMEM <= 232448, "tiles exceed the shared memory of a CTA");
+  static constexpr int TM_S = 0;                                  // S_t at t * 128
+  static constexpr int TM_O = 256;                                // O_t at 256 + t * DT
+};
+
+template <int DT, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(SAF_THREADS, 1)
+span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const SpanArgs p) {
+  using C = SafCfg<DT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  int2 *span = (int2 *)(smem + C::OFF_SPAN);
+  int2 *range = (int2 *)(smem + C::OFF_RANGE);
+  uint64_t *bars = (uint64_t *)(smem + C::OFF_BAR);
+  uint64_t *q_full = bars;            // [2]
+  uint64_t *k_full = bars + 2;        // [NK]
+  uint64_t *k_empty = bars + 4;       // [NK]
+  uint64_t *v_full = bars + 6;        // [NV]
+  uint64_t *v_ready = bars + 10;      // [NV]
+  uint64_t *v_empty = bars + 14;      // [NV]
+  uint64_t *s_full = bars + 18;       // [2]
+  uint64_t *p_full = bars + 20;       // [2] four warps
+  uint64_t *o_full = bars + 22;       // [2]
+  uint32_t *tmem_slot = (uint32_t *)(bars + 24);
+  volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {      // the launch did not leave room to align the tiles: refuse
+    pdl_entry();
+    if (threadIdx.x == 0 && p.err) atomicCAS(p.err, 0, (int)FFK_ERR_BAD_ARG);
+    return;
+  }
+  // the query blocks of all heads in turn, the last ones (which see most keys under a causal mask) first
+  const int rows_cta = SA_T * p.tiles;
+  const int nqb = (p.S + rows_cta - 1) / rows_cta;
+  const int bh = blockIdx.x % (p.B * p.H);
+  const int qb = nqb - 1 - blockIdx.x / (p.B * p.H);
+  const int h = bh % p.H, b = bh / p.H, kh = h / (p.H / p.KH);
+  const int q0 = qb * rows_cta;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) { mbar_init(&q_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+    for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+    for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_ready[s], 1); mbar_init(&v_empty[s], 1); }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_entry();  // the set-up above ran under the previous kernel's tail
+  // spans of the CTA's queries, and what each 32 of them see together
+  if (threadIdx.x < 256) {
+    const int q = q0 + (int)threadIdx.x;
+    int2 s = make_int2(1, 0);
+    if ((int)threadIdx.x < rows_cta && q < p.S) s = sa_span(p, b, q);
+    span[threadIdx.x] = s;
+    const bool sees = s.x <= s.y;
+    const int lo = __reduce_min_sync(0xffffffffu, sees ? s.x : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, sees ? s.y : -1);
+    if (lane == 0) range[warp] = make_int2(lo, hi);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  // key tiles of each query tile: from[t] .. to[t], none where from > to
+  int from[2], to[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    int lo = 0x7fffffff, hi = -1;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { lo = min(lo, range[t * 4 + w].x); hi = max(hi, range[t * 4 + w].y); }
+    from[t] = hi < 0 ? 1 : lo / SA_T;
+    to[t] = hi < 0 ? 0 : hi / SA_T;
+  }
+  const bool any0 = from[0] <= to[0], any1 = from[1] <= to[1];
+  const int j0 = any0 ? (any1 ? min(from[0], from[1]) : from[0]) : from[1];
+  const int j1 = any0 ? (any1 ? max(to[0], to[1]) : to[0]) : to[1];
+  const int n = j1 - j0 + 1;               // 0 where no query sees a key
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0 && n > 0) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (from[t] <= to[t]) {
+          mbar_expect_tx(&q_full[t], C::TILE);
+#pragma unroll
+          for (int c = 0; c < C::PANELS; ++c)
+            tma_load_4d(smem_u32(smem + C::OFF_Q + t * C::TILE + c * SA_PANEL), &tmQ, &q_full[t], c * 64, q0 + t * SA_T, h, b);
+        }
+      // the K and the V ring advance independently; the wait for progress on either is bounded
+      int ki = 0, vi = 0;
+      uint64_t t0 = ffk_globaltimer();
+      uint32_t spins = 0;
+      while (ki < n || vi < n) {
+        bool progress = false;
+        if (ki < n) {
+          const int s = ki % C::NK;
+          if (mbar_try_wait(&k_empty[s], ((uint32_t)(ki / C::NK) & 1u) ^ 1u)) {
+            mbar_expect_tx(&k_full[s], C::TILE);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              tma_load_4d(smem_u32(smem + C::OFF_K + s * C::TILE + c * SA_PANEL), &tmK, &k_full[s], c * 64, (j0 + ki) * SA_T, kh, b);
+            ++ki;
+            progress = true;
+          }
+        }
+        if (vi < n) {
+          const int s = vi % C::NV;
+          if (mbar_try_wait(&v_empty[s], ((uint32_t)(vi / C::NV) & 1u) ^ 1u)) {
+            mbar_expect_tx(&v_full[s], C::TILE);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c)
+              tma_load_4d(smem_u32(smem + C::OFF_V + s * C::TILE + c * SA_PANEL), &tmV, &v_full[s], c * 64, (j0 + vi) * SA_T, kh, b);
+            ++vi;
+            progress = true;
+          }
+        }
+        if (progress) {
+          t0 = ffk_globaltimer();
+        } else if ((++spins & 63u) == 0) {
+          if (*abort_flag) break;
+          if (ffk_globaltimer() - t0 > WAIT_LIMIT_NS) {
+            *abort_flag = 1;
+            if (p.err) atomicCAS(p.err, 0, (int)FFK_ERR_TIMEOUT_PRODUCER);
+            break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer: the whole warp runs, one lane issues
+    const bool leader = elect_one();
+    const uint64_t dq0 = make_smem_desc(smem_u32(smem + C::OFF_Q), 16, 1024);
+    const uint64_t dk0 = make_smem_desc(smem_u32(smem + C::OFF_K), 16, 1024);
+    const uint64_t dv0 = make_smem_desc(smem_u32(smem + C::OFF_V), SA_PANEL, 1024);
+    const int ksteps = (p.D + 15) / 16;                                   // of Q K^T; the columns beyond D are zeros
+    const uint32_t id_s = sa_idesc(128, SA_T, 0, 0), id_o = sa_idesc(128, ksteps * 16, 0, 1);
+    bool ok = true;
+    // i: number of the key tile in the walk.  S_t overwrites the buffer that P_t(i - 1) was read from: products run in issue order
+    auto issue_s = [&](int t, int i) {
+      if (leader) {
+        const uint64_t a = desc_advance(dq0, (uint32_t)(t * C::TILE)), k = desc_advance(dk0, (uint32_t)((i % C::NK) * C::TILE));
+        const uint32_t d = tmem_base + (uint32_t)(C::TM_S + t * SA_T);
+        tc_mma_bf16<false>(d, a, k, id_s);
+        for (int s = 1; s < ksteps; ++s) {
+          const uint32_t off = (uint32_t)((s >> 2) * SA_PANEL + (s & 3) * 32);
+          tc_mma_bf16<true>(d, desc_advance(a, off), desc_advance(k, off), id_s);
+        }
+        tc_commit(&s_full[t]);
+      }
+      __syncwarp();
+    };
+    auto wait_k = [&](int i) -> bool { return mbar_wait_warp(&k_full[i % C::NK], (uint32_t)(i / C::NK) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA); };
+    if (any0) ok = mbar_wait_warp(&q_full[0], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    if (any1 && ok) ok = mbar_wait_warp(&q_full[1], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    if (ok && n > 0) {
+      ok = wait_k(0);
+      if (ok) {
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (from[t] == j0 && from[t] <= to[t]) issue_s(t, 0);
+        if (leader) tc_commit(&k_empty[0]);
+      }
+    }
+    uint32_t done[2] = {0, 0};              // products P V issued for each query tile
+    for (int i = 0; i < n && ok; ++i) {
+      const int j = j0 + i;
+      const bool more = i + 1 < n;
+      bool k_here = false, v_here = false;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (ok && j >= from[t] && j <= to[t]) {
+          if (!v_here) {
+            ok = mbar_wait_warp(&v_full[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
+                 mbar_wait_warp(&v_ready[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+            v_here = true;
+          }
+          if (ok) ok = mbar_wait_warp(&p_full[t], done[t] & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+          if (ok) {
+            tc_fence_after();
+            if (leader) {
+              const uint64_t v = desc_advance(dv0, (uint32_t)((i % C::NV) * C::TILE));
+              const uint32_t d = tmem_base + (uint32_t)(C::TM_O + t * DT), a = tmem_base + (uint32_t)(C::TM_S + t * SA_T);
+              if (done[t] == 0) tc_mma_ts_bf16<false>(d, a, v, id_o);
+              else tc_mma_ts_bf16<true>(d, a, v, id_o);
+#pragma unroll
+              for (int s = 1; s < SA_T / 16; ++s) tc_mma_ts_bf16<true>(d, a + (uint32_t)(s * 8), desc_advance(v, (uint32_t)(s * 2048)), id_o);
+              if (j == to[t]) tc_commit(&o_full[t]);
+            }
+            __syncwarp();
+            ++done[t];
+          }
+        }
+        if (ok && more && j + 1 >= from[t] && j + 1 <= to[t]) {
+          if (!k_here) {
+            ok = wait_k(i + 1);
+            k_here = true;
+          }
+          if (ok) {
+            tc_fence_after();
+            issue_s(t, i + 1);
+          }
+        }
+      }
+      // a key tile that neither query tile takes (between two documents) is waited for all the same: its stage is given back below
+      if (ok && !v_here) ok = mbar_wait_warp(&v_ready[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+      if (ok && more && !k_here) ok = wait_k(i + 1);
+      if (ok && leader) {
+        tc_commit(&v_empty[i % C::NV]);
+        if (more) tc_commit(&k_empty[(i + 1) % C::NK]);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ rows of V that nothing sees
+    bool ok = true;
+    for (int i = 0; i < n && ok; ++i) {
+      const int k0 = (j0 + i) * SA_T;
+      uint32_t keep[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int2 s = span[r * 32 + lane];
+        if (s.x <= s.y) sa_add_bits(keep, s.x - k0, s.y - k0);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) keep[w] = __reduce_or_sync(0xffffffffu, keep[w]);
+      ok = sa_wait(&v_full[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+        sa_clear_rows(smem + C::OFF_V + (i % C::NV) * C::TILE, C::PANELS, keep, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      sa_warp_arrive(&v_ready[i % C::NV], lane);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ softmax: thread = query row
+    const int t = (warp - 4) >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const int q = q0 + t * SA_T + r;
+    const int2 mine = span[t * SA_T + r];
+    const bool empty = mine.x > mine.y;
+    // a row that sees nothing computes what it likes and stores zeros: it does not keep its warp from the unmasked path
+    const int lo = empty ? -1 : mine.x, hi = empty ? 0x7ffffff0 : mine.y;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t t_s = lane_base + (uint32_t)(C::TM_S + t * SA_T), t_o = lane_base + (uint32_t)(C::TM_O + t * DT);
+    const float slope = BIAS ? -p.slopes[h] * SA_LOG2E : 0.f;
+    float m = -INFINITY, l = 0.f;          // m: what the row's exponentials are taken against; -infinity until the row has seen a key
+    bool ok = true;
+    const int steps = to[t] - from[t] + 1;
+    for (int i = 0; i < steps && ok; ++i) {
+      const int k0 = (from[t] + i) * SA_T;
+      ok = sa_wait(&s_full[t], (uint32_t)i & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + (uint32_t)(c * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
+      tmem_ld_wait();
+      const bool full = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + SA_T - 1);
+      const int a = lo - k0, w = hi - lo;
+      if (CAP && !full) {                 // what masked scores hold does not choose the way tanh is taken
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if ((unsigned)(c - a) > (unsigned)w) x[c] = 0u;
+      }
+      float f = sa_capped<128, CAP>(x, p, !empty);
+      if constexpr (BIAS) {
+        const pair32 ff = pair_of(f, f), ss = pair_of(slope, slope), two = pair_of(2.f, 2.f);
+        pair32 d = pair_of((float)(k0 - q), (float)(k0 - q + 1));       // whole numbers: exact
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          pair_set(&x[c], pair_fma(ss, d & 0x7fffffff7fffffffull, pair_mul(pair_get(&x[c]), ff)));
+          d = pair_add(d, two);
+        }
+        f = 1.f;
+      }
+      if (!full) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if ((unsigned)(c - a) > (unsigned)w) x[c] = 0xff800000u;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], fmaxf(__uint_as_float(x[c + u]), __uint_as_float(x[c + 4 + u])));
+      }
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+      const bool need = top > m + SAF_GAP;
+      if (i == 0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, need)) {
+        // the scores were issued after P V of the tile before, and have arrived: O holds all earlier tiles and nothing is under way
+        const float alpha = need ? (m == -INFINITY ? 0.f : sa_exp2(m - top)) : 1.f;
+#pragma unroll 1
+        for (int c = 0; c < DT / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + (uint32_t)(c * 32), o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int u = 0; u < 32; ++u) o[u] = __float_as_uint(__uint_as_float(o[u]) * alpha);
+          tmem_st32(t_o + (uint32_t)(c * 32), o);
+        }
+        l *= alpha;
+        if (need) m = top;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      const pair32 ff = pair_of(f, f), neg = pair_of(-ref, -ref);
+      pair32 sum0 = pair_of(l, 0.f), sum1 = pair_of(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 128; c += 16) {
+        float e[16];
+#pragma unroll
+        for (int u = 0; u < 16; u += 2) pair_to(pair_fma(pair_get(&x[c + u]), ff, neg), e[u], e[u + 1]);
+#pragma unroll
+        for (int u = 0; u < 12; ++u) e[u] = sa_exp2(e[u]);
+        sa_exp2_pair(e[12], e[13]);
+        sa_exp2_pair(e[14], e[15]);
+#pragma unroll
+        for (int u = 0; u < 16; u += 4) {
+          sum0 = pair_add(sum0, pair_of(e[u], e[u + 1]));
+          sum1 = pair_add(sum1, pair_of(e[u + 2], e[u + 3]));
+        }
+#pragma unroll
+        for (int u = 0; u < 16; u += 2) x[(c + u) >> 1] = pack_bf162(e[u], e[u + 1]);
+      }
+      float s0, s1, s2, s3;
+      pair_to(sum0, s0, s1);
+      pair_to(sum1, s2, s3);
+      l = (s0 + s1) + (s2 + s3);
+      tmem_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+      tmem_st32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
+      tmem_st_wait();
+      tc_fence_before();
+      sa_warp_arrive(&p_full[t], lane);
+    }
+    if (ok && steps > 0) {
+      ok = sa_wait(&o_full[t], 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+      tc_fence_after();
+    }
+    if (ok) {
+      const bool stored = t * SA_T + r < rows_cta && q < p.S;
+      const float inv = empty || !(l != 0.f) ? 0.f : 1.f / l;
+      if (stored && p.lse) p.lse[((long long)b * p.H + h) * p.S + q] = empty ? 0.f : m + __log2f(l);
+      bf16 *orow = p.O + ((long long)b * p.S + q) * p.ldo + (long long)h * p.D;
+#pragma unroll 1
+      for (int c = 0; c < DT / 32; ++c) {
+        uint32_t o[32];
+        if (steps > 0) {
+          tmem_ld32(t_o + (uint32_t)(c * 32), o);      // warp-wide: rows past the end read too and store nothing
+          tmem_ld_wait();
+        }
+        if (stored) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (c * 32 + 8 * u < p.D) {
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (!empty)
+                v = make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * inv, __uint_as_float(o[8 * u + 1]) * inv),
+                               pack_bf162(__uint_as_float(o[8 * u + 2]) * inv, __uint_as_float(o[8 * u + 3]) * inv),
+                               pack_bf162(__uint_as_float(o[8 * u + 4]) * inv, __uint_as_float(o[8 * u + 5]) * inv),
+                               pack_bf162(__uint_as_float(o[8 * u + 6]) * inv, __uint_as_float(o[8 * u + 7]) * inv));
+              *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) = v;
+            }
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+__device__ int g_span_attn_err = 0;
+
+template <int DT, bool CAP, bool BIAS>
+int launch_fwd(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const SpanArgs &a, long long grid, cudaStream_t st) {
+  static unsigned long long done = 0;
+  const cudaError_t e = ffk_allow_smem(span_attn_fwd_kernel<DT, CAP, BIAS>, SafCfg<DT>::SMEM, done);
+  if (e != cudaSuccess) return (int)e;
+  return ffk_launch(span_attn_fwd_kernel<DT, CAP, BIAS>, (unsigned)grid, SAF_THREADS, SafCfg<DT>::SMEM, st, tq, tk, tv, a);
+}
+
+}  // namespace
+
+int *ffk_span_attention_err() {
+  void *p = nullptr;
+  return cudaGetSymbolAddress(&p, g_span_attn_err) == cudaSuccess ? (int *)p : nullptr;
+}
+
+FFK_API int ffk_span_attention_fwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
+  if (d->B <= 0 || d->H <= 0 || d->S <= 0) return 0;
+  if (!sa_shape_ok(d)) return -2;
+  if (!sa_aligned(d->Q, d->ldq) || !sa_aligned(d->K, d->ldk) || !sa_aligned(d->V, d->ldv) || !sa_aligned(d->O, d->ldo)) return -2;
+  CUtensorMap tq, tk, tv;
+  int r;
+  if ((r = sa_head_map(&tq, d->Q, d->D, d->S, d->ldq, d->H, d->B))) return r;
+  if ((r = sa_head_map(&tk, d->K, d->D, d->S, d->ldk, d->KH, d->B))) return r;
+  if ((r = sa_head_map(&tv, d->V, d->D, d->S, d->ldv, d->KH, d->B))) return r;
+  SpanArgs a = {};
+  sa_args(d, a, ffk_span_attention_err());
+  // two query tiles per CTA share the K and V tiles and the tensor core; one where that would leave SMs without work
+  const long long heads = (long long)d->B * d->H;
+  a.tiles = heads * ((d->S + 255) / 256) >= 148 ? 2 : 1;
+  const long long grid = heads * ((d->S + SA_T * a.tiles - 1) / (SA_T * a.tiles));
+  if (heads > 0x7fffffffll || grid > 0x7fffffffll) return -2;
+  FfkTraffic traffic((long long)d->B * d->S * d->D * 2 * (2 * d->H + 2 * d->KH));
+  const bool cap = d->cap > 0.f, bias = d->slopes != nullptr;
+  if (d->D <= 64) {
+    if (cap) return bias ? launch_fwd<64, true, true>(tq, tk, tv, a, grid, st) : launch_fwd<64, true, false>(tq, tk, tv, a, grid, st);
+    return bias ? launch_fwd<64, false, true>(tq, tk, tv, a, grid, st) : launch_fwd<64, false, false>(tq, tk, tv, a, grid, st);
+  }
+  if (cap) return bias ? launch_fwd<128, true, true>(tq, tk, tv, a, grid, st) : launch_fwd<128, true, false>(tq, tk, tv, a, grid, st);
+  return bias ? launch_fwd<128, false, true>(tq, tk, tv, a, grid, st) : launch_fwd<128, false, false>(tq, tk, tv, a, grid, st);
+}
+
+// Reads (and clears) the error word of the bounded waits of both directions.  Synchronises the device.
+FFK_API int ffk_span_attention_last_error() {
+  int v = 0, z = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
+  cudaMemcpyFromSymbol(&v, g_span_attn_err, sizeof(int));
+  cudaMemcpyToSymbol(g_span_attn_err, &z, sizeof(int));
+  return v;
+}

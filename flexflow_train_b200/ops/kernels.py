@@ -76,6 +76,18 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class SpanAttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int), ("H", c_int), ("KH", c_int), ("S", c_int), ("D", c_int), ("scale", c_float), ("cap", c_float),
+        ("spans", c_void_p), ("slopes", c_void_p),
+        ("Q", c_void_p), ("ldq", c_longlong), ("K", c_void_p), ("ldk", c_longlong), ("V", c_void_p), ("ldv", c_longlong),
+        ("O", c_void_p), ("ldo", c_longlong), ("lse", c_void_p),
+        ("dO", c_void_p), ("lddo", c_longlong),
+        ("dQ", c_void_p), ("lddq", c_longlong), ("dK", c_void_p), ("lddk", c_longlong), ("dV", c_void_p), ("lddv", c_longlong),
+        ("scratch", c_void_p),
+    ]
+
+
 class ConvDesc(ctypes.Structure):
     _fields_ = [
         ("N", c_int), ("H", c_int), ("W", c_int), ("C", c_int), ("OC", c_int), ("KH", c_int), ("KW", c_int),
@@ -377,6 +389,145 @@ def attention_keep_mask(B, H, Sq, Sk, p, salt, seed=None, device="cpu"):
     return keep.reshape(B, H, Sq, Sk)
 
 
+# --------------------------------------------------------------------------- attention over spans of keys
+def attention_spans(documents, prompt=None, *, causal=True, out=None):
+    """The first and last token that each token of packed sequences sees: int32 [B, S, 2], the mask of `span_attention_fwd`.
+
+    documents [B, S] int32: a document is a run of equal numbers in a row; a negative number is padding, which sees nothing (first 0,
+    last -1).  A token sees its own document: up to itself if `causal`, to the end otherwise.  prompt [B, S] (bool or uint8, with
+    `causal` only): the flagged tokens that a document begins with are seen by all of its tokens."""
+    if documents.dim() != 2 or documents.dtype != torch.int32:
+        raise KernelError("attention_spans: documents is an int32 [batch, sequence] tensor")
+    B, S = documents.shape
+    if prompt is not None:
+        if prompt.dtype not in (torch.bool, torch.uint8) or prompt.shape != documents.shape:
+            raise KernelError("attention_spans: prompt holds one bool or uint8 flag per token")
+        if not causal:
+            raise KernelError("attention_spans: a prompt is seen by all of its document anyway unless the mask is causal")
+    if out is None:
+        out = torch.empty(B, S, 2, dtype=torch.int32, device=documents.device)
+    if out.dtype != torch.int32 or tuple(out.shape) != (B, S, 2):
+        raise KernelError("attention_spans: out is an int32 [batch, sequence, 2] tensor")
+    if B > 2**31 - 1 or S > 2**31 - 4096:
+        raise KernelError("attention_spans: sequence too long")
+    _apart("attention_spans", ("documents", documents), ("out", out))
+    _apart("attention_spans", ("prompt", prompt), ("out", out))
+    _cuda_contig(documents, prompt, out)
+    _same_device(documents, prompt, out)
+    _check(_nlib().ffk_attention_spans(documents.data_ptr(), _p(prompt), out.data_ptr(), B, S, int(bool(causal)), _stream()), "ffk_attention_spans")
+    return out
+
+
+def span_attention_supported(head_dim: int) -> bool:
+    """True when `span_attention_fwd` / `_bwd` cover this head dimension: multiples of 8 up to 128."""
+    return 8 <= int(head_dim) <= 128 and int(head_dim) % 8 == 0
+
+
+def span_attention_last_error() -> int:
+    """Error word of the span attention kernels' bounded waits (0: none ran out).  Synchronises the device."""
+    return _nlib().ffk_span_attention_last_error()
+
+
+def _span_operand(what, name, t, rows, heads, D):
+    """A [B*S, >= heads*D] bf16 matrix with unit column stride whose rows TMA can address -> (pointer, leading dimension)."""
+    if t is None or t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < heads * D or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
+    ld = t.stride(0) if rows > 1 else max(t.stride(0), (heads * D + 7) // 8 * 8)
+    if ld < heads * D or ld % 8 or t.data_ptr() % 16:
+        raise KernelError(f"{what}: {name} must start on a 16-byte boundary, at a pitch of a multiple of 8 elements that holds its heads")
+    return t.data_ptr(), ld
+
+
+def _span_desc(what, spans, B, S, H, KH, D, scale, cap, slopes):
+    if min(B, S) < 0 or H < 1 or KH < 1 or H % KH:
+        raise KernelError(f"{what}: every key head serves the same number of query heads (H {H}, KH {KH}, B {B}, S {S})")
+    if not span_attention_supported(D):
+        raise KernelError(f"{what}: head dim {D} (a multiple of 8 up to 128 expected)")
+    if not (0.0 < scale < float("inf") and 0.0 <= cap < float("inf")):
+        raise KernelError(f"{what}: scale must be positive and cap not negative")
+    if spans is None or spans.dtype != torch.int32 or tuple(spans.shape) != (B, S, 2) or not spans.is_contiguous() or spans.data_ptr() % 8:
+        raise KernelError(f"{what}: spans is a contiguous int32 [B, S, 2] tensor (attention_spans)")
+    if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous()):
+        raise KernelError(f"{what}: slopes holds one fp32 value per query head")
+    d = SpanAttnDesc()
+    d.B, d.H, d.KH, d.S, d.D, d.scale, d.cap = B, H, KH, S, D, float(scale), float(cap)
+    d.spans, d.slopes = spans.data_ptr(), _p(slopes)
+    return d
+
+
+def _span_apart(what, d, outs, ins, rows, widths):
+    """Refuses outputs that share memory with an input or with one another.  Two matrices of one pitch may lie side by side (views into a
+    packed buffer); `widths`: columns in use."""
+    def place(name):
+        return getattr(d, name), getattr(d, "ld" + name.lower()) * 2, widths[name] * 2
+
+    plain = {"Q": "q", "K": "k", "V": "v", "O": "out", "dO": "dout", "dQ": "dq", "dK": "dk", "dV": "dv"}
+    for i, a in enumerate(outs):
+        for b in outs[i + 1:] + ins:
+            (pa, la, wa), (pb, lb, wb) = place(a), place(b)
+            if pa + (rows - 1) * la + wa <= pb or pb + (rows - 1) * lb + wb <= pa:
+                continue
+            gap = (pb - pa) % la
+            if la == lb and gap >= wa and gap + wb <= la:
+                continue
+            raise KernelError(f"{what}: {plain[a]} and {plain[b]} share memory")
+
+
+def span_attention_fwd(q, k, v, out, lse, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None):
+    """out[b, q, h] = softmax over the keys of q's span of x[q, k], times v, with
+    x = f(scale * q . k) - slopes[h] * |q - k| and f(u) = cap * tanh(u / cap) (u itself where cap is 0).
+
+    q / out [B*S, >= H*D] and k / v [B*S, >= KH*D] are bf16 matrices with head h in columns [h*D, (h+1)*D) (views into a packed QKV
+    buffer are fine); query head h reads key head h // (H // KH).  spans [B, S, 2] int32: the first and last key that each query sees
+    (`attention_spans`, or any: what lies outside the sequence is cut off).  A query whose span is empty gets zeros.  lse [B, H, S]
+    fp32 receives the base-2 log-sum-exp of x (0 for an empty span), which `span_attention_bwd` needs.  What tokens hold that no query
+    sees does not matter, NaN included."""
+    d = _span_desc("span_attention_fwd", spans, B, S, H, KH, D, scale, cap, slopes)
+    rows = B * S
+    for f, ldf, name, t, heads in (("Q", "ldq", "q", q, H), ("K", "ldk", "k", k, KH), ("V", "ldv", "v", v, KH), ("O", "ldo", "out", out, H)):
+        ptr, ld = _span_operand("span_attention_fwd", name, t, rows, heads, D)
+        setattr(d, f, ptr)
+        setattr(d, ldf, ld)
+    if lse is None or lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or not lse.is_contiguous():
+        raise KernelError("span_attention_fwd: lse must be a contiguous fp32 [B, H, S] tensor")
+    if rows:
+        _span_apart("span_attention_fwd", d, ["O"], ["Q", "K", "V"], rows, {"Q": H * D, "K": KH * D, "V": KH * D, "O": H * D})
+    d.lse = lse.data_ptr()
+    _same_device(q, k, v, out, lse, spans, slopes)
+    _check(_nlib().ffk_span_attention_fwd(ctypes.byref(d), _stream()), "ffk_span_attention_fwd")
+    return out
+
+
+def span_attention_bwd_scratch_floats(B, H, S) -> int:
+    """fp32 elements of scratch `span_attention_bwd` needs."""
+    return int(_nlib().ffk_span_attention_bwd_scratch_floats(B, H, S))
+
+
+def span_attention_bwd(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None):
+    """Gradients of `span_attention_fwd` with respect to q, k and v (same layouts; dk and dv are summed over the query heads that share a
+    key head).  out and lse are the forward pass's.  Every sum is taken in a fixed order: the same inputs give the same bits.  scratch:
+    span_attention_bwd_scratch_floats(B, H, S) fp32 elements on a 16-byte boundary.  The slopes have no gradient."""
+    d = _span_desc("span_attention_bwd", spans, B, S, H, KH, D, scale, cap, slopes)
+    rows = B * S
+    for f, ldf, name, t, heads in (("Q", "ldq", "q", q, H), ("K", "ldk", "k", k, KH), ("V", "ldv", "v", v, KH), ("O", "ldo", "out", out, H),
+                                   ("dO", "lddo", "dout", dout, H), ("dQ", "lddq", "dq", dq, H), ("dK", "lddk", "dk", dk, KH),
+                                   ("dV", "lddv", "dv", dv, KH)):
+        ptr, ld = _span_operand("span_attention_bwd", name, t, rows, heads, D)
+        setattr(d, f, ptr)
+        setattr(d, ldf, ld)
+    if lse is None or lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or not lse.is_contiguous():
+        raise KernelError("span_attention_bwd: lse must be a contiguous fp32 [B, H, S] tensor")
+    if scratch is None or scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.data_ptr() % 16 or \
+            scratch.numel() < span_attention_bwd_scratch_floats(B, H, S):
+        raise KernelError("span_attention_bwd: scratch must hold span_attention_bwd_scratch_floats(B, H, S) fp32 elements")
+    if rows:
+        wide = {n: (KH if n[-1] in "KV" else H) * D for n in ("Q", "K", "V", "O", "dO", "dQ", "dK", "dV")}
+        _span_apart("span_attention_bwd", d, ["dQ", "dK", "dV"], ["Q", "K", "V", "O", "dO"], rows, wide)
+    d.lse, d.scratch = lse.data_ptr(), scratch.data_ptr()
+    _same_device(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, slopes)
+    _check(_nlib().ffk_span_attention_bwd(ctypes.byref(d), _stream()), "ffk_span_attention_bwd")
+
+
 def _es(t):
     if t.dtype == torch.bfloat16:
         return 2
@@ -594,6 +745,206 @@ def loss_fwd(kind: str, pred, target, loss_rows):
     ldt = _dt(target) if target is not None and target.dtype in (torch.int32, torch.int64) else DT_I32
     _check(lib().ffk_loss_fwd(LOSS_KINDS[kind], pred.data_ptr(), _p(target), loss_rows.data_ptr(), rows, cols,
                               _dt(pred), ldt, _stream()), "ffk_loss_fwd")
+
+
+def _same_device(*ts):
+    """Tensors of a call live on one device, which is the current one: the kernel is launched on its current stream."""
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) > 1:
+        raise KernelError(f"operands on different devices: {sorted(map(str, devices))}")
+    for d in devices:
+        if d.type != "cuda":
+            raise KernelError("kernel called with a CPU tensor")
+        if d.index != torch.cuda.current_device():
+            raise KernelError(f"operands on {d}, but cuda:{torch.cuda.current_device()} is the current device")
+
+
+def _new_ops_decl(l):
+    P, I, L, F, S = c_void_p, c_int, c_longlong, c_float, c_void_p
+    sig = {
+        "ffk_rmsnorm_fwd": ([P, P, P, P, P, P, I, I, F, I, S], c_int),
+        "ffk_rmsnorm_bwd": ([P, P, P, P, P, P, P, P, I, I, I, I, S], c_int),
+        "ffk_rmsnorm_bwd_scratch": ([I, I], c_longlong),
+        "ffk_attention_spans": ([P, P, P, I, I, I, S], c_int),
+        "ffk_span_attention_fwd": ([ctypes.POINTER(SpanAttnDesc), S], c_int),
+        "ffk_span_attention_bwd": ([ctypes.POINTER(SpanAttnDesc), S], c_int),
+        "ffk_span_attention_bwd_scratch_floats": ([I, I, I], c_longlong),
+        "ffk_span_attention_last_error": ([], c_int),
+        "ffk_grad_piece_elements": ([], c_int),
+        "ffk_grad_partials": ([], c_int),
+        "ffk_grad_norm": ([P, I, P, P, L, S], c_int),
+        "ffk_grad_clip": ([P, I, P, F, P, L, S], c_int),
+    }
+    for name, (args, res) in sig.items():
+        fn = getattr(l, name)
+        fn.argtypes = args
+        fn.restype = res
+
+
+_new_ops_declared = [False]
+
+
+def _nlib():
+    l = lib()
+    if not _new_ops_declared[0]:
+        _new_ops_decl(l)
+        _new_ops_declared[0] = True
+    return l
+
+
+def _rms_check(what, a, gamma, same, rstd):
+    """Checks of the RMS norm's operands: `a` [rows, cols], gamma [cols], tensors of a's shape, rstd [rows]."""
+    if a.dim() != 2:
+        raise KernelError(f"{what}: rows are a 2-D [rows, cols] tensor")
+    rows, cols = a.shape
+    if a.dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"{what}: bf16 or fp32 rows expected, got {a.dtype}")
+    if cols < 1 or rows > 2**31 - 1 or cols > 2**31 - 1:
+        raise KernelError(f"{what}: rows of {cols} elements")
+    for t in same:
+        if t is not None and (t.shape != a.shape or t.dtype != a.dtype):
+            raise KernelError(f"{what}: tensors of the rows' shape and dtype expected")
+    if gamma is None or gamma.dtype != a.dtype or tuple(gamma.shape) != (cols,):
+        raise KernelError(f"{what}: gamma must hold one value of the rows' dtype per column")
+    if rstd is not None and (rstd.dtype != torch.float32 or rstd.numel() != rows):
+        raise KernelError(f"{what}: rstd must be fp32 with one value per row")
+
+
+def _apart(what, *named):
+    """Refuses outputs that share memory with one another or with an input they may not replace: (name, tensor) pairs."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), n) for n, t in named if t is not None and t.numel())
+    for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
+        if start < end:
+            raise KernelError(f"{what}: {a} and {b} share memory")
+
+
+def _same_or_apart(what, out_name, out, others):
+    """An output that is read and written element by element may be one of the inputs, but not a part of one."""
+    for name, t in others:
+        if out is None or t is None or (out.data_ptr() == t.data_ptr() and out.numel() == t.numel()):
+            continue
+        _apart(what, (out_name, out), (name, t))
+
+
+def rmsnorm_fwd(a, gamma, eps, residual=None, xsum=None, out=None, rstd=None):
+    """out = h / sqrt(mean(h^2) + eps) * gamma over the rows of h = a + residual (h = a without a residual), h rounded to the rows'
+    dtype.  xsum receives h, rstd (fp32, one per row) the reciprocal root, which `rmsnorm_bwd` needs.  `out` and `xsum` may be `a` or
+    `residual` themselves."""
+    _rms_check("rmsnorm_fwd", a, gamma, (residual, xsum, out), rstd)
+    out = torch.empty_like(a) if out is None else out
+    if xsum is not None and residual is None:
+        raise KernelError("rmsnorm_fwd: xsum is the sum with a residual")
+    ins = (("a", a), ("residual", residual))
+    _same_or_apart("rmsnorm_fwd", "out", out, ins)
+    _same_or_apart("rmsnorm_fwd", "xsum", xsum, ins)
+    _apart("rmsnorm_fwd", ("out", out), ("xsum", xsum), ("gamma", gamma), ("rstd", rstd))
+    _cuda_contig(a, residual, gamma, xsum, out, rstd)
+    _same_device(a, residual, gamma, xsum, out, rstd)
+    rows, cols = a.shape
+    _check(_nlib().ffk_rmsnorm_fwd(a.data_ptr(), _p(residual), gamma.data_ptr(), _p(xsum), out.data_ptr(), _p(rstd), rows, cols, eps, _dt(a),
+                                   _stream()), "ffk_rmsnorm_fwd")
+    return out
+
+
+def rmsnorm_bwd_scratch(rows, cols) -> int:
+    """fp32 elements of scratch `rmsnorm_bwd` needs for [rows, cols]."""
+    return int(_nlib().ffk_rmsnorm_bwd_scratch(rows, cols))
+
+
+def rmsnorm_bwd(dy, x, gamma, rstd, dx, dgamma, scratch, dsum=None, accumulate_params=False):
+    """Gradients of `rmsnorm_fwd`: x is what was normalized (`xsum` where there was a residual).  dx = gradient of x, to which `dsum`,
+    the gradient that reaches x past the norm, is added: it is the gradient of both addends.  dgamma (None: not computed) (+)= its column
+    sums, added in a fixed order.  dx may be dy or dsum themselves.  scratch: rmsnorm_bwd_scratch(rows, cols) fp32 elements."""
+    _rms_check("rmsnorm_bwd", dy, gamma, (x, dx, dsum), rstd)
+    rows, cols = dy.shape
+    if rstd is None or x is None or dx is None:
+        raise KernelError("rmsnorm_bwd: x, rstd and dx are needed")
+    if dgamma is not None:
+        if dgamma.dtype != dy.dtype or tuple(dgamma.shape) != (cols,):
+            raise KernelError("rmsnorm_bwd: dgamma must be like gamma")
+        if rows and (scratch is None or scratch.dtype != torch.float32 or scratch.numel() < rmsnorm_bwd_scratch(rows, cols)):
+            raise KernelError("rmsnorm_bwd: scratch smaller than rmsnorm_bwd_scratch(rows, cols)")
+    _same_or_apart("rmsnorm_bwd", "dx", dx, (("dy", dy), ("x", x), ("dsum", dsum)))
+    _apart("rmsnorm_bwd", ("dx", dx), ("gamma", gamma), ("rstd", rstd), ("dgamma", dgamma), ("scratch", scratch if dgamma is not None else None))
+    _cuda_contig(dy, x, gamma, rstd, dx, dsum, dgamma, scratch)
+    _same_device(dy, x, gamma, rstd, dx, dsum, dgamma, scratch)
+    _check(_nlib().ffk_rmsnorm_bwd(dy.data_ptr(), x.data_ptr(), gamma.data_ptr(), rstd.data_ptr(), _p(dsum), dx.data_ptr(), _p(dgamma),
+                                   _p(scratch) if dgamma is not None else None, rows, cols, _dt(dy), int(accumulate_params), _stream()),
+           "ffk_rmsnorm_bwd")
+
+
+# --------------------------------------------------------------------------- gradient norm and clipping
+_GRAD_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class GradientList:
+    """Gradient tensors that `gradient_norm` and `clip_gradients` take as one vector: contiguous fp32, bf16 or fp16 tensors of one
+    device, any sizes (empty ones too).  `out`: where `clip_gradients` leaves the clipped gradients, one tensor per gradient of its
+    shape and dtype, sharing no memory with any gradient but its own (default: in place).
+
+    The list of their pieces lies in device memory from here on (a captured graph may address it while the list lives), and so does the
+    scratch of the passes: calls on one list run one after another, on one stream or ordered by the caller; two lists may be used at
+    once."""
+
+    def __init__(self, tensors, out=None):
+        self.tensors = list(tensors)
+        self.out = list(out) if out is not None else self.tensors
+        if not self.tensors:
+            raise KernelError("GradientList: no gradients")
+        if len(self.out) != len(self.tensors):
+            raise KernelError("GradientList: one output per gradient")
+        for t, o in zip(self.tensors, self.out):
+            if t.dtype not in _GRAD_TYPES:
+                raise KernelError(f"GradientList: unsupported dtype {t.dtype}")
+            if o.dtype != t.dtype or o.shape != t.shape:
+                raise KernelError("GradientList: an output has its gradient's shape and dtype")
+        bounds = lambda t: (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())  # noqa: E731
+        held = [bounds(t) for t in self.tensors] + [bounds(o) for t, o in zip(self.tensors, self.out) if bounds(o) != bounds(t)]
+        held = sorted(b for b in held if b[0] < b[1])
+        if any(start < end for (_, end), (start, _) in zip(held, held[1:])):
+            raise KernelError("GradientList: gradients or outputs that share memory")
+        _cuda_contig(*self.tensors, *self.out)
+        self.check_device()
+        piece = _nlib().ffk_grad_piece_elements()
+        tables = []
+        for t, o in zip(self.tensors, self.out):
+            es, n = t.element_size(), t.numel()
+            at = torch.arange(0, n, piece, dtype=torch.int64)
+            tables.append(torch.stack([t.data_ptr() + at * es, o.data_ptr() + at * es, (n - at).clamp_max(piece) | _dt(t) << 32], 1))
+        table = torch.cat(tables)
+        self.pieces = table.shape[0]
+        if self.pieces > 2**31 - 1:
+            raise KernelError("GradientList: too many elements")
+        device = self.tensors[0].device
+        self.bytes = sum(t.numel() * t.element_size() for t in self.tensors)
+        self._table = (table if self.pieces else torch.zeros(1, 3, dtype=torch.int64)).to(device)
+        self._partial = torch.empty(_nlib().ffk_grad_partials(), dtype=torch.float64, device=device)
+        self.norm = torch.zeros(1, dtype=torch.float32, device=device)
+
+    def check_device(self):
+        _same_device(*self.tensors, *self.out)
+
+
+def gradient_norm(grads: GradientList):
+    """The 2-norm of all gradients of the list taken as one vector: an fp32 device tensor of one element, the list's own, which the next
+    call on the list overwrites.  The sum does not depend on the order in which blocks run."""
+    grads.check_device()
+    _check(_nlib().ffk_grad_norm(grads._table.data_ptr(), grads.pieces, grads._partial.data_ptr(), grads.norm.data_ptr(), grads.bytes, _stream()),
+           "ffk_grad_norm")
+    return grads.norm
+
+
+def clip_gradients(grads: GradientList, max_norm: float):
+    """Every gradient of the list times min(1, max_norm / norm), in place or into the list's outputs, without a host synchronisation;
+    returns the norm before clipping (see `gradient_norm`).  A norm that is not finite leaves the values as they are: read the norm to
+    skip such a step."""
+    max_norm = float(max_norm)
+    if not 0.0 <= max_norm < float("inf"):
+        raise KernelError("clip_gradients: max_norm is a finite number that is not negative")
+    grads.check_device()
+    _check(_nlib().ffk_grad_clip(grads._table.data_ptr(), grads.pieces, grads._partial.data_ptr(), max_norm, grads.norm.data_ptr(), 2 * grads.bytes,
+                                 _stream()), "ffk_grad_clip")
+    return grads.norm
 
 
 # --------------------------------------------------------------------------- optimizers / embedding
