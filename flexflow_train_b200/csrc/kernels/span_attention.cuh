@@ -39,9 +39,10 @@ struct SpanArgs {
   int B, H, KH, S, D;
   const int2 *spans;
   const float *slopes;
-  float mul;                       // to the log-2 domain: scale * log2(e), or with a cap scale / cap
-  float cap2;                      // cap * log2(e)
-  float scale;
+  float scale, factor;             // factor = scale * log2(e): a score in log-2 units is factor * y, see sa_scores
+  float to_z, from_z;              // with a cap: scale / cap and cap / scale
+  float lim2, lim4;                // |raw score| up to which tanh is a polynomial of degree 2 or 4 in its square; negative: nowhere
+  float t2[3], t4[5];              // the polynomials' coefficients, for raw scores
   bf16 *O;
   long long ldo;
   float *lse;
@@ -94,56 +95,86 @@ __device__ __forceinline__ float sa_exp2(float x) {
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^x of a pair on the FMA pipe: x = n + f, |f| <= 1/2, a polynomial of degree 4 for 2^f (least squares on the relative error, 2.6e-6),
-// n added to the exponent.  x below -126 counts as -126.
-__device__ __forceinline__ void sa_exp2_pair(float &a, float &b) {
-  const float magic = 12582912.f;                        // 1.5 * 2^23: the sum holds round(x) in its low bits
-  const pair32 x = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const pair32 t = pair_add(x, pair_of(magic, magic));
-  const pair32 n = pair_add(t, pair_of(-magic, -magic));
-  const pair32 f = pair_fma(n, pair_of(-1.f, -1.f), x);
-  pair32 p = pair_fma(f, pair_of(0.009570101276f, 0.009570101276f), pair_of(0.05591785908f, 0.05591785908f));
-  p = pair_fma(p, f, pair_of(0.2402474433f, 0.2402474433f));
-  p = pair_fma(p, f, pair_of(0.6931217909f, 0.6931217909f));
-  p = pair_fma(p, f, pair_of(0.9999992847f, 0.9999992847f));
-  float p0, p1, t0, t1;
-  pair_to(p, p0, p1);
-  pair_to(t, t0, t1);
-  a = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  b = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
-// tanh(z) for |z| <= SA_TANH_SMALL: z times a polynomial of degree 4 in z^2 (least squares on the relative error, 1.1e-7)
-constexpr float SA_TANH_SMALL = 0.625f;
-__device__ __forceinline__ pair32 sa_tanh_small(pair32 z) {
-  const pair32 w = pair_mul(z, z);
-  pair32 p = pair_fma(w, pair_of(0.01505094394f, 0.01505094394f), pair_of(-0.05182186514f, -0.05182186514f));
-  p = pair_fma(p, w, pair_of(0.1330452561f, 0.1330452561f));
-  p = pair_fma(p, w, pair_of(-0.3333195448f, -0.3333195448f));
-  p = pair_fma(p, w, pair_of(0.9999998808f, 0.9999998808f));
-  return pair_mul(z, p);
-}
 // tanh(z) = 1 - 2 / (1 + e^2z), everywhere, to 2e-7 of 1
 __device__ __forceinline__ float sa_tanh_any(float z) { return 1.f - __fdividef(2.f, 1.f + sa_exp2(fminf(z * (2.f * SA_LOG2E), 120.f))); }
 
-// `x` (N raw scores of one row) becomes tanh(mul * x) with a cap; the score in log-2 units is x times what is returned.  All lanes of the
-// warp; a row that does not `count` has no say in the way tanh is taken.
-template <int N, bool CAP>
-__device__ __forceinline__ float sa_capped(uint32_t (&x)[N], const SpanArgs &p, bool count) {
-  if constexpr (!CAP) return p.mul;
-  float most = 0.f;
+// Scores of N columns of a row, in place: raw products s become y with  (score in log-2 units) = factor * y:
+//   y = s, with a cap tanh(a s) / a (a = scale / cap), with a bias less slope / scale * |distance|.
+// The special-function unit has its hands full with the exponentials (8 cycles a warp instruction), and the FMA pipe takes one element a
+// cycle whether packed or not, so tanh(a s) / a = s T((a s)^2) is a polynomial as short as the warp's largest |s| allows: degree 2 up to |a s| =
+// 1/4, degree 4 up to 5/8 (least squares on the relative error: 4e-7 and 1.1e-7), the exponential form beyond.  `count`: whether the row has a
+// say in that (one that sees nothing may hold anything).  d0: position of the first column less the row's, side: -1 / 1 where no column of
+// the warp lies right / left of its row, 0 otherwise.  All lanes of the warp.
+template <bool CAP, bool BIAS, int N>
+__device__ __forceinline__ void sa_scores(uint32_t (&x)[N], const SpanArgs &p, bool count, float slope, float d0, int side) {
+  if constexpr (CAP) {
+    float most[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < N; i += 2) most = fmaxf(most, fmaxf(fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1]))));
-  if (__all_sync(0xffffffffu, !count || most * p.mul <= SA_TANH_SMALL)) {
-    const pair32 a = pair_of(p.mul, p.mul);
+    for (int i = 0; i < N; i += 2) {
+      most[0] = fmaxf(most[0], fabsf(__uint_as_float(x[i])));
+      most[1] = fmaxf(most[1], fabsf(__uint_as_float(x[i + 1])));
+    }
+    const float top = fmaxf(most[0], most[1]);
+    if (__all_sync(0xffffffffu, !count || top <= p.lim2)) {
+      const pair32 c0 = pair_of(p.t2[0], p.t2[0]), c1 = pair_of(p.t2[1], p.t2[1]), c2 = pair_of(p.t2[2], p.t2[2]);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) pair_set(&x[i], sa_tanh_small(pair_mul(pair_get(&x[i]), a)));
-  } else {
+      for (int i = 0; i < N; i += 2) {
+        const pair32 s = pair_get(&x[i]), w = pair_mul(s, s);
+        pair_set(&x[i], pair_mul(s, pair_fma(pair_fma(w, c2, c1), w, c0)));
+      }
+    } else if (__all_sync(0xffffffffu, !count || top <= p.lim4)) {
+      const pair32 c0 = pair_of(p.t4[0], p.t4[0]), c1 = pair_of(p.t4[1], p.t4[1]), c2 = pair_of(p.t4[2], p.t4[2]), c3 = pair_of(p.t4[3], p.t4[3]),
+                   c4 = pair_of(p.t4[4], p.t4[4]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = __float_as_uint(sa_tanh_any(__uint_as_float(x[i]) * p.mul));
+      for (int i = 0; i < N; i += 2) {
+        const pair32 s = pair_get(&x[i]), w = pair_mul(s, s);
+        pair_set(&x[i], pair_mul(s, pair_fma(pair_fma(pair_fma(pair_fma(w, c4, c3), w, c2), w, c1), w, c0)));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = __float_as_uint(sa_tanh_any(__uint_as_float(x[i]) * p.to_z) * p.from_z);
+    }
   }
-  return p.cap2;
+  if constexpr (BIAS) {
+    // distances are whole numbers: exact
+    pair32 d = pair_of(d0, d0 + 1.f);
+    const pair32 two = pair_of(2.f, 2.f);
+    if (side != 0) {
+      const float k = side > 0 ? -slope : slope;
+      const pair32 kk = pair_of(k, k);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        pair_set(&x[i], pair_fma(kk, d, pair_get(&x[i])));
+        d = pair_add(d, two);
+      }
+    } else {
+      const pair32 kk = pair_of(-slope, -slope);
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        pair_set(&x[i], pair_fma(kk, d & 0x7fffffff7fffffffull, pair_get(&x[i])));
+        d = pair_add(d, two);
+      }
+    }
+  }
 }
+// The distance bias of successive pairs of columns in log-2 units, added to `to` (backward: the cap's derivative needs the score without it)
+struct SaBias {
+  pair32 d, k, bits;
+  __device__ __forceinline__ SaBias(float slope, float d0, int side) {
+    const float kk = side < 0 ? slope : -slope;
+    d = pair_of(d0, d0 + 1.f);
+    k = pair_of(kk * SA_LOG2E, kk * SA_LOG2E);
+    bits = side != 0 ? ~0ull : 0x7fffffff7fffffffull;
+  }
+  __device__ __forceinline__ pair32 next(pair32 to) {
+    const pair32 r = pair_fma(k, d & bits, to);
+    d = pair_add(d, pair_of(2.f, 2.f));
+    return r;
+  }
+};
+// 32 of a thread's registers
+template <int N>
+__device__ __forceinline__ uint32_t (&sa_group(uint32_t (&x)[N], int g))[32] { return *reinterpret_cast<uint32_t(*)[32]>(&x[g * 32]); }
 
 __device__ __forceinline__ void sa_warp_arrive(uint64_t *bar, int lane) {
   __syncwarp();
@@ -159,6 +190,25 @@ __device__ __forceinline__ int2 sa_span(const SpanArgs &p, int b, int q) {
   s.x = max(s.x, 0);
   s.y = min(s.y, p.S - 1);
   return s;
+}
+
+// How a warp's 32 rows see columns [c, c + 31], as spans [lo, hi] of each lane: bits of `none` and `part` by column group of 32.  All lanes.
+template <int GROUPS>
+__device__ __forceinline__ void sa_kinds(int lo, int hi, int c, uint32_t &none, uint32_t &part) {
+  none = part = 0;
+  if (__all_sync(0xffffffffu, lo <= c && hi >= c + GROUPS * 32 - 1)) return;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int a = c + g * 32, z = a + 31;
+    if (!__any_sync(0xffffffffu, lo <= z && hi >= a)) none |= 1u << g;
+    else if (!__all_sync(0xffffffffu, lo <= a && hi >= z)) part |= 1u << g;
+  }
+}
+// columns before `a` and behind `z` (of 32) become `v`
+__device__ __forceinline__ void sa_mask(uint32_t (&x)[32], int a, int z, uint32_t v) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (i < a || i > z) x[i] = v;
 }
 
 // Clears the rows of a tile (panels of 64 columns, 128 bytes a row) whose bit in `keep` (four words, 32 rows each) is not set.  One warp.
@@ -216,9 +266,25 @@ inline bool sa_shape_ok(const FfkSpanAttnDesc *d) {
 inline void sa_args(const FfkSpanAttnDesc *d, SpanArgs &a, int *err) {
   a.B = d->B; a.H = d->H; a.KH = d->KH; a.S = d->S; a.D = d->D;
   a.spans = (const int2 *)d->spans; a.slopes = d->slopes;
-  a.mul = d->cap > 0.f ? d->scale / d->cap : d->scale * SA_LOG2E;
-  a.cap2 = d->cap * SA_LOG2E;
   a.scale = d->scale;
+  a.factor = d->scale * SA_LOG2E;
+  a.lim2 = a.lim4 = -1.f;
+  if (d->cap > 0.f) {
+    const float z = d->scale / d->cap, w = z * z;
+    a.to_z = z;
+    a.from_z = d->cap / d->scale;
+    const float t2[3] = {0.9999996043f, -0.3332190822f, 0.1284161341f};
+    const float t4[5] = {0.9999998808f, -0.3333195448f, 0.1330452561f, -0.05182186514f, 0.01505094394f};
+    float f = 1.f;
+    for (int i = 0; i < 5; ++i, f *= w) {
+      if (i < 3) a.t2[i] = t2[i] * f;
+      a.t4[i] = t4[i] * f;
+    }
+    if (z >= 1.f / 4096 && z <= 1024.f) {      // z^8 within the range of 32 bits
+      a.lim2 = 0.25f / z;
+      a.lim4 = 0.625f / z;
+    }
+  }
   a.O = (bf16 *)d->O; a.ldo = d->ldo; a.lse = d->lse;
   a.err = err;
 }

@@ -21,6 +21,12 @@ namespace {
 
 constexpr int SAB_THREADS = 384;
 
+// y[c], y[c + 1] (scores, see sa_scores) become e0, e1 times the cap's derivative 1 - (a y)^2
+__device__ __forceinline__ void sa_times_slope(uint32_t (&y)[32], int c, float e0, float e1, float a) {
+  const pair32 e = pair_of(e0, e1), z = pair_mul(pair_get(&y[c]), pair_of(a, a));
+  pair_set(&y[c], pair_fma(pair_mul(z, pair_of(-e0, -e1)), z, e));
+}
+
 // ---------------------------------------------------------------------------------------------- delta and summaries
 // L lanes (16 bytes each) per (row, head); blocks from `delta_blocks` on: a warp per 128 queries.  Summary: smallest first key and largest
 // last key of the queries that see any, largest first key and smallest last key of all (an empty span among them: nothing is seen by all).
@@ -89,7 +95,8 @@ struct DkvCfg {
   static constexpr int OFF_LSE = OFF_DO + NQ * TILE;               // [NQ][128] float
   static constexpr int OFF_DELTA = OFF_LSE + NQ * 512;             // [NQ][128] float
   static constexpr int OFF_SPAN = OFF_DELTA + NQ * 512;            // [NQ][128] int2
-  static constexpr int OFF_BAR = OFF_SPAN + NQ * 1024;
+  static constexpr int OFF_GROUP = OFF_SPAN + NQ * 1024;           // [NQ][4] int4: summary of each 32 queries
+  static constexpr int OFF_BAR = OFF_GROUP + NQ * 64;
   static constexpr int SLACK = 1024;
   static constexpr int SMEM = OFF_BAR + 256 + SLACK;
   static constexpr int TM_S = 0, TM_DP = 128, TM_DK = 256, TM_DV = 256 + DT;
@@ -162,6 +169,9 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int i0 = walk[0], ni = walk[1] < 0 ? 0 : walk[1] - i0 + 1;
   const int n = ni * group;                                       // steps: (head, query tile)
 
+  // the element-wise warps hold half a row of a tile each: registers go from the warps that move data to them (128 x 104 + 256 x 200)
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -196,7 +206,9 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     auto issue_t = [&](uint32_t d, uint64_t a, uint64_t bq, uint64_t *bar) {
       if (leader) {
         tc_mma_bf16<false>(d, a, bq, id_s);
-        for (int s = 1; s < ksteps; ++s) {
+#pragma unroll
+        for (int s = 1; s < DT / 16; ++s) {
+          if (s >= ksteps) break;
           const uint32_t off = (uint32_t)((s >> 2) * SA_PANEL + (s & 3) * 32);
           tc_mma_bf16<true>(d, desc_advance(a, off), desc_advance(bq, off), id_s);
         }
@@ -311,11 +323,23 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         dlt[r * 32 + lane] = vd[r];
         sp[r * 32 + lane] = vs[r];
       }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {       // rows behind the sequence count as seeing all: their probabilities are zeros
+        const bool there = i * SA_T + r * 32 + lane < p.S, sees = vs[r].x <= vs[r].y;
+        int4 t;
+        t.x = __reduce_min_sync(0xffffffffu, sees ? vs[r].x : 0x7fffffff);
+        t.y = __reduce_max_sync(0xffffffffu, sees ? vs[r].y : -1);
+        t.z = __reduce_max_sync(0xffffffffu, sees ? vs[r].x : there ? 0x7fffffff : -1);
+        t.w = __reduce_min_sync(0xffffffffu, sees ? vs[r].y : there ? -1 : 0x7fffffff);
+        if (lane == 0) *(int4 *)(smem + C::OFF_GROUP + (s * 4 + r) * 16) = t;
+      }
       if (lane == 0) full_flag[s] = all.z <= k0 && all.w >= k1;
       sa_warp_arrive(&st_full[s], lane);
       if (++i == i0 + ni) { i = i0; ++g; }
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------------ P^T and dS^T: thread = key x 64 of the tile's queries
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane, key = k0 + r;
@@ -326,48 +350,62 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const int s = it & 1;
       const uint32_t ph = (uint32_t)it & 1u;
       const float *lse = (const float *)(smem + C::OFF_LSE) + s * SA_T + half * 64, *dlt = (const float *)(smem + C::OFF_DELTA) + s * SA_T + half * 64;
-      const int4 *sp = (const int4 *)(smem + C::OFF_SPAN) + (s * SA_T + half * 64) / 2;
+      const int4 *sp = (const int4 *)(smem + C::OFF_SPAN) + (s * SA_T + half * 64) / 2;     // two spans each
       ok = sa_wait(&st_full[s], (uint32_t)(it >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE) &&
            sa_wait(s_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       tc_fence_after();
-      const bool full = full_flag[s] != 0;
-      uint32_t x[64];
-      tmem_ld32(lane_base + C::TM_S, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-      tmem_ld32(lane_base + C::TM_S + 32u, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
-      tmem_ld_wait();
-      if (CAP && !full) {                 // what masked scores hold does not choose the way tanh is taken
+      // how this warp's 32 keys are seen by each 32 of the tile's queries
+      uint32_t none = 0, part = 0;
+      if (full_flag[s] == 0) {
+        const int a = k0 + quarter * 32;
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const int4 t = sp[c / 2];
-          if (key < t.x || key > t.y) x[c] = 0u;
-          if (key < t.z || key > t.w) x[c + 1] = 0u;
+        for (int gq = 0; gq < 2; ++gq) {
+          const int4 t = *(const int4 *)(smem + C::OFF_GROUP + (s * 4 + half * 2 + gq) * 16);
+          if (t.x > a + 31 || t.y < a) none |= 1u << gq;
+          else if (t.z > a || t.w < a + 31) part |= 1u << gq;
         }
       }
-      const float f = sa_capped<64, CAP>(x, p, true);
-      const pair32 ff = pair_of(f, f);
+      uint32_t x[64];
+      tmem_ld32(lane_base + C::TM_S, sa_group(x, 0));
+      tmem_ld32(lane_base + C::TM_S + 32u, sa_group(x, 1));
+      tmem_ld_wait();
       uint32_t pk[32];
-      {
-        float slope = 0.f;
-        if constexpr (BIAS) slope = -p.slopes[kh * group + g] * SA_LOG2E;
-        const pair32 ss = pair_of(slope, slope), two = pair_of(2.f, 2.f);
-        const float d0 = (float)(i * SA_T + half * 64 - key);
-        pair32 d = pair_of(d0, d0 + 1.f);
+      float slope = 0.f;
+      if constexpr (BIAS) slope = p.slopes[kh * group + g];
+      const pair32 ff = pair_of(p.factor, p.factor);
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const float4 w = *reinterpret_cast<const float4 *>(lse + c);
-          float e[4];
+      for (int gq = 0; gq < 2; ++gq) {
+        uint32_t(&y)[32] = sa_group(x, gq);
+        if (none >> gq & 1u) {
 #pragma unroll
-          for (int u = 0; u < 4; u += 2) {
-            pair32 y = pair_fma(pair_get(&x[c + u]), ff, u == 0 ? pair_of(-w.x, -w.y) : pair_of(-w.z, -w.w));
-            if constexpr (BIAS) {
-              y = pair_fma(ss, d & 0x7fffffff7fffffffull, y);
-              d = pair_add(d, two);
-            }
-            pair_to(y, e[u], e[u + 1]);
+          for (int c = 0; c < 32; ++c) y[c] = 0u;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) pk[gq * 16 + c] = 0u;
+          continue;
+        }
+        const bool masked = part >> gq & 1u;
+        const int qg = i * SA_T + half * 64 + gq * 32, kw = k0 + quarter * 32;
+        if (CAP && masked) {              // masked scores do not choose the way tanh is taken
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const int4 t = sp[gq * 16 + c / 2];
+            if (key < t.x || key > t.y) y[c] = 0u;
+            if (key < t.z || key > t.w) y[c + 1] = 0u;
           }
-          if (!full) {
-            const int4 a = sp[c / 2], z = sp[c / 2 + 1];
+        }
+        sa_scores<CAP, false>(y, p, true, 0.f, 0.f, 0);
+        SaBias bias(slope, (float)(qg - key), qg >= kw + 31 ? 1 : qg + 31 <= kw ? -1 : 0);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 w = *reinterpret_cast<const float4 *>(lse + gq * 32 + c);
+          float e[4];
+          pair32 w0 = pair_of(-w.x, -w.y), w1 = pair_of(-w.z, -w.w);
+          if constexpr (BIAS) { w0 = bias.next(w0); w1 = bias.next(w1); }
+          pair_to(pair_fma(pair_get(&y[c]), ff, w0), e[0], e[1]);
+          pair_to(pair_fma(pair_get(&y[c + 2]), ff, w1), e[2], e[3]);
+          if (masked) {
+            const int4 a = sp[gq * 16 + c / 2], z = sp[gq * 16 + c / 2 + 1];
             if (key < a.x || key > a.y) e[0] = -INFINITY;
             if (key < a.z || key > a.w) e[1] = -INFINITY;
             if (key < z.x || key > z.y) e[2] = -INFINITY;
@@ -375,18 +413,15 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           }
 #pragma unroll
           for (int u = 0; u < 4; ++u) e[u] = sa_exp2(e[u]);
-          pk[c >> 1] = pack_bf162(e[0], e[1]);
-          pk[(c >> 1) + 1] = pack_bf162(e[2], e[3]);
+          pk[gq * 16 + (c >> 1)] = pack_bf162(e[0], e[1]);
+          pk[gq * 16 + (c >> 1) + 1] = pack_bf162(e[2], e[3]);
           // what dS needs of P: times the cap's derivative
+          if constexpr (CAP) {
+            sa_times_slope(y, c, e[0], e[1], p.to_z);
+            sa_times_slope(y, c + 2, e[2], e[3], p.to_z);
+          } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if constexpr (CAP) {
-              const float t = __uint_as_float(x[c + u]);
-              const float k = e[u] * fmaf(-t, t, 1.f);
-              x[c + u] = __float_as_uint(k);
-            } else {
-              x[c + u] = __float_as_uint(e[u]);
-            }
+            for (int u = 0; u < 4; ++u) y[c + u] = __float_as_uint(e[u]);
           }
         }
       }
@@ -398,23 +433,25 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
-      for (int hc = 0; hc < 64; hc += 32) {
+      for (int gq = 0; gq < 2; ++gq) {
+        if (none >> gq & 1u) continue;    // zeros already
+        const uint32_t(&e)[32] = sa_group(x, gq);
         uint32_t y[32];
-        tmem_ld32(lane_base + C::TM_DP + (uint32_t)hc, y);
+        tmem_ld32(lane_base + C::TM_DP + (uint32_t)(gq * 32), y);
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          const float4 w = *reinterpret_cast<const float4 *>(dlt + hc + c);
-          float e[4];
-          pair_to(pair_mul(pair_get(&x[hc + c]), pair_add(pair_get(&y[c]), pair_of(-w.x, -w.y))), e[0], e[1]);
-          pair_to(pair_mul(pair_get(&x[hc + c + 2]), pair_add(pair_get(&y[c + 2]), pair_of(-w.z, -w.w))), e[2], e[3]);
-          if (!full) {
+          const float4 w = *reinterpret_cast<const float4 *>(dlt + gq * 32 + c);
+          float v[4];
+          pair_to(pair_mul(pair_get(&e[c]), pair_add(pair_get(&y[c]), pair_of(-w.x, -w.y))), v[0], v[1]);
+          pair_to(pair_mul(pair_get(&e[c + 2]), pair_add(pair_get(&y[c + 2]), pair_of(-w.z, -w.w))), v[2], v[3]);
+          if (part >> gq & 1u) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              if (__uint_as_float(x[hc + c + u]) == 0.f) e[u] = 0.f;            // whatever dO and delta hold there
+              if (__uint_as_float(e[c + u]) == 0.f) v[u] = 0.f;                 // whatever dO and delta hold there
           }
-          pk[(hc + c) >> 1] = pack_bf162(e[0], e[1]);
-          pk[((hc + c) >> 1) + 1] = pack_bf162(e[2], e[3]);
+          pk[gq * 16 + (c >> 1)] = pack_bf162(v[0], v[1]);
+          pk[gq * 16 + (c >> 1) + 1] = pack_bf162(v[2], v[3]);
         }
       }
       tmem_st32(lane_base + C::TM_DP, pk);
@@ -508,9 +545,11 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t *s_full = bars + 14;       // [2]
   uint64_t *dp_full = bars + 16;
   uint64_t *dp_free = bars + 17;      // eight warps
-  uint64_t *ds_full = bars + 18;      // eight warps
-  uint64_t *dq_full = bars + 19;
-  uint32_t *tmem_slot = (uint32_t *)(bars + 20);
+  // two, for the warps may be a tile apart (dP of the next one is there as soon as all have read this one's): an arrival for the next tile
+  // must not count for this one
+  uint64_t *ds_full = bars + 18;      // [2] eight warps
+  uint64_t *dq_full = bars + 20;
+  uint32_t *tmem_slot = (uint32_t *)(bars + 21);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {
@@ -529,7 +568,8 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_ready[s], 1); mbar_init(&k_empty[s], 1); }
     for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
     mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
-    mbar_init(dp_full, 1); mbar_init(dp_free, 8); mbar_init(ds_full, 8); mbar_init(dq_full, 1);
+    mbar_init(&ds_full[0], 8); mbar_init(&ds_full[1], 8);
+    mbar_init(dp_full, 1); mbar_init(dp_free, 8); mbar_init(dq_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -556,6 +596,9 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   const int j0 = last < 0 ? 0 : first / SA_T;
   const int n = last < 0 ? 0 : last / SA_T - j0 + 1;
 
+  // the element-wise warps hold half a row of a tile each: registers go from the warps that move data to them (128 x 104 + 256 x 200)
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -615,7 +658,9 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     auto issue_t = [&](uint32_t d, uint64_t a, uint64_t bk) {
       if (leader) {
         tc_mma_bf16<false>(d, a, bk, id_s);
-        for (int s = 1; s < ksteps; ++s) {
+#pragma unroll
+        for (int s = 1; s < DT / 16; ++s) {
+          if (s >= ksteps) break;
           const uint32_t off = (uint32_t)((s >> 2) * SA_PANEL + (s & 3) * 32);
           tc_mma_bf16<true>(d, desc_advance(a, off), desc_advance(bk, off), id_s);
         }
@@ -651,7 +696,7 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         ok = issue_s(i + 1) && mbar_wait_warp(dp_free, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && issue_dp(i + 1);
         if (!ok) break;
       }
-      ok = mbar_wait_warp(ds_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+      ok = mbar_wait_warp(&ds_full[i & 1], (uint32_t)(i >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
       if (!ok) break;
       tc_fence_after();
       if (leader) {
@@ -688,7 +733,9 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       }
       sa_warp_arrive(&k_ready[s], lane);
     }
-  } else if (warp >= 4) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ------------------------------------------------------------------ dS: thread = query x 64 of the tile's keys
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     const int r = quarter * 32 + lane, q = q0 + r;
@@ -696,10 +743,11 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const bool empty = mine.x > mine.y;
     const int lo = empty ? -1 : mine.x, hi = empty ? 0x7ffffff0 : mine.y;      // see the forward kernel
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
-    const float slope = BIAS ? -p.slopes[h] * SA_LOG2E : 0.f;
+    const float slope = BIAS ? p.slopes[h] : 0.f;
+    const int q_low = q - lane;
     const long long stat = ((long long)b * p.H + h) * p.S + q;
     const float neg_lse = empty ? -INFINITY : -p.lse[stat], neg_delta = empty ? 0.f : -p.delta[stat];
-    const pair32 nl = pair_of(neg_lse, neg_lse), nd = pair_of(neg_delta, neg_delta);
+    const pair32 nl = pair_of(neg_lse, neg_lse), nd = pair_of(neg_delta, neg_delta), ff = pair_of(p.factor, p.factor);
     bool ok = true;
     for (int i = 0; i < n && ok; ++i) {
       const uint32_t ph = (uint32_t)i & 1u;
@@ -709,45 +757,37 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (!ok) break;
       tc_fence_after();
       uint32_t x[64];
-      tmem_ld32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-      tmem_ld32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
+      tmem_ld32(t_s, sa_group(x, 0));
+      tmem_ld32(t_s + 32u, sa_group(x, 1));
       tmem_ld_wait();
-      const bool full = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + 63);
-      const int a = lo - k0, w = hi - lo;
-      if (CAP && !full) {
+      uint32_t none, part;
+      sa_kinds<2>(lo, hi, k0, none, part);
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if ((unsigned)(c - a) > (unsigned)w) x[c] = 0u;
-      }
-      const float f = sa_capped<64, CAP>(x, p, !empty);
-      const pair32 ff = pair_of(f, f), ss = pair_of(slope, slope), two = pair_of(2.f, 2.f);
-      pair32 d = pair_of((float)(k0 - q), (float)(k0 - q + 1));
+      for (int g = 0; g < 2; ++g) {
+        if (none >> g & 1u) continue;
+        const int kg = k0 + g * 32;
+        uint32_t(&y)[32] = sa_group(x, g);
+        if (CAP && (part >> g & 1u)) sa_mask(y, lo - kg, hi - kg, 0u);
+        sa_scores<CAP, false>(y, p, !empty, 0.f, 0.f, 0);
+        SaBias bias(slope, (float)(kg - q), kg + 31 <= q_low ? -1 : kg >= q_low + 31 ? 1 : 0);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        float e[4];
+        for (int c = 0; c < 32; c += 4) {
+          float e[4];
+          pair_to(pair_fma(pair_get(&y[c]), ff, BIAS ? bias.next(nl) : nl), e[0], e[1]);
+          pair_to(pair_fma(pair_get(&y[c + 2]), ff, BIAS ? bias.next(nl) : nl), e[2], e[3]);
+          if (part >> g & 1u) {
 #pragma unroll
-        for (int u = 0; u < 4; u += 2) {
-          pair32 y = pair_fma(pair_get(&x[c + u]), ff, nl);
-          if constexpr (BIAS) {
-            y = pair_fma(ss, d & 0x7fffffff7fffffffull, y);
-            d = pair_add(d, two);
+            for (int u = 0; u < 4; ++u)
+              if (c + u < lo - kg || c + u > hi - kg) e[u] = -INFINITY;
           }
-          pair_to(y, e[u], e[u + 1]);
-        }
-        if (!full) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if ((unsigned)(c + u - a) > (unsigned)w) e[u] = -INFINITY;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          e[u] = sa_exp2(e[u]);
+          for (int u = 0; u < 4; ++u) e[u] = sa_exp2(e[u]);
           if constexpr (CAP) {
-            const float t = __uint_as_float(x[c + u]);
-            const float k = e[u] * fmaf(-t, t, 1.f);
-            x[c + u] = __float_as_uint(k);
+            sa_times_slope(y, c, e[0], e[1], p.to_z);
+            sa_times_slope(y, c + 2, e[2], e[3], p.to_z);
           } else {
-            x[c + u] = __float_as_uint(e[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) y[c + u] = __float_as_uint(e[u]);
           }
         }
       }
@@ -761,19 +801,27 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       tc_fence_before();
       sa_warp_arrive(dp_free, lane);
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float e0, e1;
-        pair_to(pair_mul(pair_get(&x[c]), pair_add(pair_get(&y[c]), nd)), e0, e1);
-        if (!full) {
-          if (__uint_as_float(x[c]) == 0.f) e0 = 0.f;
-          if (__uint_as_float(x[c + 1]) == 0.f) e1 = 0.f;
+      for (int g = 0; g < 2; ++g) {
+        if (none >> g & 1u) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) y[g * 16 + c] = 0u;
+          continue;
         }
-        y[c >> 1] = pack_bf162(e0, e1);
+#pragma unroll
+        for (int c = g * 32; c < g * 32 + 32; c += 2) {
+          float e0, e1;
+          pair_to(pair_mul(pair_get(&x[c]), pair_add(pair_get(&y[c]), nd)), e0, e1);
+          if (part >> g & 1u) {           // whatever V and delta hold there
+            if (__uint_as_float(x[c]) == 0.f) e0 = 0.f;
+            if (__uint_as_float(x[c + 1]) == 0.f) e1 = 0.f;
+          }
+          y[c >> 1] = pack_bf162(e0, e1);
+        }
       }
       tmem_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&y[0]));
       tmem_st_wait();
       tc_fence_before();
-      sa_warp_arrive(ds_full, lane);
+      sa_warp_arrive(&ds_full[i & 1], lane);
     }
     if (ok && n > 0) {
       ok = sa_wait(dq_full, 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);

@@ -112,6 +112,9 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int j1 = any0 ? (any1 ? max(to[0], to[1]) : to[0]) : to[1];
   const int n = j1 - j0 + 1;               // 0 where no query sees a key
 
+  // the softmax warps hold a row of scores each: registers go from the four warps that move data to them (128 x 88 + 256 x 208 = 384 x 168)
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -178,7 +181,9 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         const uint64_t a = desc_advance(dq0, (uint32_t)(t * C::TILE)), k = desc_advance(dk0, (uint32_t)((i % C::NK) * C::TILE));
         const uint32_t d = tmem_base + (uint32_t)(C::TM_S + t * SA_T);
         tc_mma_bf16<false>(d, a, k, id_s);
-        for (int s = 1; s < ksteps; ++s) {
+#pragma unroll
+        for (int s = 1; s < DT / 16; ++s) {
+          if (s >= ksteps) break;         // unrolled: the one lane that issues bounds the tensor core otherwise
           const uint32_t off = (uint32_t)((s >> 2) * SA_PANEL + (s & 3) * 32);
           tc_mma_bf16<true>(d, desc_advance(a, off), desc_advance(k, off), id_s);
         }
@@ -269,7 +274,9 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       sa_warp_arrive(&v_ready[i % C::NV], lane);
     }
-  } else if (warp >= 4) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------------------------ softmax: thread = query row
     const int t = (warp - 4) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;
@@ -280,7 +287,8 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int lo = empty ? -1 : mine.x, hi = empty ? 0x7ffffff0 : mine.y;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t t_s = lane_base + (uint32_t)(C::TM_S + t * SA_T), t_o = lane_base + (uint32_t)(C::TM_O + t * DT);
-    const float slope = BIAS ? -p.slopes[h] * SA_LOG2E : 0.f;
+    const float slope = BIAS ? p.slopes[h] / p.scale : 0.f;
+    const int q_low = q - lane;            // the warp's first row
     float m = -INFINITY, l = 0.f;          // m: what the row's exponentials are taken against; -infinity until the row has seen a key
     bool ok = true;
     const int steps = to[t] - from[t] + 1;
@@ -293,28 +301,19 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(t_s + (uint32_t)(c * 32), *reinterpret_cast<uint32_t(*)[32]>(&x[c * 32]));
       tmem_ld_wait();
+      // a warp whose rows all see the whole tile takes no mask; masked scores do not choose the way tanh is taken
       const bool full = __all_sync(0xffffffffu, lo <= k0 && hi >= k0 + SA_T - 1);
-      const int a = lo - k0, w = hi - lo;
-      if (CAP && !full) {                 // what masked scores hold does not choose the way tanh is taken
+      const int first = lo - k0, width = hi - lo;
+      if (CAP && !full) {
 #pragma unroll
         for (int c = 0; c < 128; ++c)
-          if ((unsigned)(c - a) > (unsigned)w) x[c] = 0u;
+          if ((unsigned)(c - first) > (unsigned)width) x[c] = 0u;
       }
-      float f = sa_capped<128, CAP>(x, p, !empty);
-      if constexpr (BIAS) {
-        const pair32 ff = pair_of(f, f), ss = pair_of(slope, slope), two = pair_of(2.f, 2.f);
-        pair32 d = pair_of((float)(k0 - q), (float)(k0 - q + 1));       // whole numbers: exact
-#pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          pair_set(&x[c], pair_fma(ss, d & 0x7fffffff7fffffffull, pair_mul(pair_get(&x[c]), ff)));
-          d = pair_add(d, two);
-        }
-        f = 1.f;
-      }
+      sa_scores<CAP, BIAS>(x, p, !empty, slope, (float)(k0 - q), k0 + SA_T - 1 <= q_low ? -1 : k0 >= q_low + 31 ? 1 : 0);
       if (!full) {
 #pragma unroll
         for (int c = 0; c < 128; ++c)
-          if ((unsigned)(c - a) > (unsigned)w) x[c] = 0xff800000u;
+          if ((unsigned)(c - first) > (unsigned)width) x[c] = 0xff800000u;
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -322,6 +321,7 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], fmaxf(__uint_as_float(x[c + u]), __uint_as_float(x[c + 4 + u])));
       }
+      const float f = p.factor;
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
       const bool need = top > m + SAF_GAP;
       if (i == 0) {
@@ -350,9 +350,7 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int u = 0; u < 16; u += 2) pair_to(pair_fma(pair_get(&x[c + u]), ff, neg), e[u], e[u + 1]);
 #pragma unroll
-        for (int u = 0; u < 12; ++u) e[u] = sa_exp2(e[u]);
-        sa_exp2_pair(e[12], e[13]);
-        sa_exp2_pair(e[14], e[15]);
+        for (int u = 0; u < 16; ++u) e[u] = sa_exp2(e[u]);
 #pragma unroll
         for (int u = 0; u < 16; u += 4) {
           sum0 = pair_add(sum0, pair_of(e[u], e[u + 1]));

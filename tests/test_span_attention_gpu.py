@@ -266,3 +266,16 @@ def test_visible_is_what_the_plain_masks_say():
     flags = torch.zeros(1, S, dtype=torch.bool, device="cuda")
     flags[0, :9] = True
     assert torch.equal(visible(K.attention_spans(zero, flags), S)[0].cpu(), (at[None] <= at[:, None]) | (at[None] < 9))
+
+
+@pytest.mark.parametrize("D,KH", [(128, 16), (64, 4)])
+def test_many_passes_give_the_same_bits(D, KH):
+    """Warps of a block run apart by as much as the barriers let them: many blocks, many passes."""
+    B, S, H = 4, 1536, 16
+    _, q, k, v, dout = make(B, S, H, KH, D, seed=31)
+    spans = mask("documents", B, S, 6)
+    sizes = dict(B=B, S=S, H=H, KH=KH, D=D, scale=1.0 / math.sqrt(D), cap=50.0)
+    first = run(q, k, v, dout, spans, **sizes)
+    for _ in range(30):
+        again = run(q, k, v, dout, spans, **sizes)
+        assert all(torch.equal(first[n], again[n]) for n in first)
