@@ -176,6 +176,14 @@ struct SaBias {
 template <int N>
 __device__ __forceinline__ uint32_t (&sa_group(uint32_t (&x)[N], int g))[32] { return *reinterpret_cast<uint32_t(*)[32]>(&x[g * 32]); }
 
+// 16 columns of a warp's 32 lanes into tensor memory
+__device__ __forceinline__ void sa_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+               "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+               "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+
 __device__ __forceinline__ void sa_warp_arrive(uint64_t *bar, int lane) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);

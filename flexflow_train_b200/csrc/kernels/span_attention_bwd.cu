@@ -11,15 +11,16 @@
 //                          transposed (lanes = keys), so that P^T and dS^T, written back to tensor memory as bf16, are the A operands of
 //                          dV += P^T dO and dK += dS^T Q where they lie.
 //   span_attn_dq_kernel    CTA = 128 queries of one head, over the key tiles that they see; lanes = queries, dS is the A operand of dQ += dS K.
-// Roles in both (384 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 clears rows that nothing sees, warps 4-11 the element-wise
-// part (thread = one row and half of the columns); in the first kernel warp 3 brings each query tile's lse, delta and spans.
+// Roles in both (640 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 clears rows that nothing sees, warps 4-19 the element-wise
+// part (thread = one row and 32 of the columns); in the first kernel warp 3 brings each query tile's lse, delta and spans.
 //
 // Every wait is bounded (tcgen05.cuh).
 #include "span_attention.cuh"
 
 namespace {
 
-constexpr int SAB_THREADS = 384;
+constexpr int SAB_THREADS = 640;
+constexpr int SAB_WARPS = 16;           // element-wise warps: 32 columns of a tile each
 
 // y[c], y[c + 1] (scores, see sa_scores) become e0, e1 times the cap's derivative 1 - (a y)^2
 __device__ __forceinline__ void sa_times_slope(uint32_t (&y)[32], int c, float e0, float e1, float a) {
@@ -116,16 +117,15 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint64_t *qd_ready = bars + 3;      // [2]
   uint64_t *qd_empty = bars + 5;      // [2]
   uint64_t *st_full = bars + 7;       // [2]
-  uint64_t *st_empty = bars + 9;      // [2] eight warps
+  uint64_t *st_empty = bars + 9;      // [2] SAB_WARPS
   uint64_t *s_full = bars + 11;
   uint64_t *dp_full = bars + 12;
-  uint64_t *p_full = bars + 13;       // eight warps
-  uint64_t *ds_full = bars + 14;      // eight warps
+  uint64_t *p_full = bars + 13;       // SAB_WARPS
+  uint64_t *ds_full = bars + 14;      // SAB_WARPS
   uint64_t *dkv_full = bars + 15;
   uint32_t *tmem_slot = (uint32_t *)(bars + 16);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
   int *walk = (int *)(tmem_slot + 2);                             // first and last query tile
-  volatile int *full_flag = (volatile int *)(tmem_slot + 4);      // [2] every query of the stage sees every key
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {
     pdl_entry();
@@ -141,8 +141,8 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    for (int s = 0; s < 2; ++s) { mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], 8); }
-    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_full, 8); mbar_init(ds_full, 8); mbar_init(dkv_full, 1);
+    for (int s = 0; s < 2; ++s) { mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], SAB_WARPS); }
+    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_full, SAB_WARPS); mbar_init(ds_full, SAB_WARPS); mbar_init(dkv_full, 1);
     *abort_flag = 0;
     walk[0] = 0x7fffffff;
     walk[1] = -1;
@@ -169,9 +169,9 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int i0 = walk[0], ni = walk[1] < 0 ? 0 : walk[1] - i0 + 1;
   const int n = ni * group;                                       // steps: (head, query tile)
 
-  // the element-wise warps hold half a row of a tile each: registers go from the warps that move data to them (128 x 104 + 256 x 200)
+  // registers go from the warps that move data to the element-wise ones (128 x 64 + 512 x 104 = 640 x 96)
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -216,14 +216,14 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       __syncwarp();
     };
-    // [keys x D] += A (bf16 in tensor memory: keys x queries, 64 queries in the first 32 columns of either half) B (queries x D)
+    // [keys x D] += A (bf16 in tensor memory: keys x queries, 32 queries in the first 16 of each 32 columns) B (queries x D)
     auto issue_g = [&](uint32_t d, uint32_t a, uint64_t bn, bool first) {
       if (leader) {
         if (first) tc_mma_ts_bf16<false>(d, a, bn, id_g);
         else tc_mma_ts_bf16<true>(d, a, bn, id_g);
 #pragma unroll
         for (int s = 1; s < SA_T / 16; ++s)
-          tc_mma_ts_bf16<true>(d, a + (uint32_t)((s >> 2) * 64 + (s & 3) * 8), desc_advance(bn, (uint32_t)(s * 2048)), id_g);
+          tc_mma_ts_bf16<true>(d, a + (uint32_t)((s >> 1) * 32 + (s & 1) * 8), desc_advance(bn, (uint32_t)(s * 2048)), id_g);
       }
       __syncwarp();
     };
@@ -298,7 +298,6 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       float *lse = (float *)(smem + C::OFF_LSE) + s * SA_T, *dlt = (float *)(smem + C::OFF_DELTA) + s * SA_T;
       int2 *sp = (int2 *)(smem + C::OFF_SPAN) + s * SA_T;
       const long long base = ((long long)b * p.H + kh * group + g) * p.S;
-      const int4 all = summary[i];
       float vl[4], vd[4];
       int2 vs[4];
 #pragma unroll
@@ -333,128 +332,111 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         t.w = __reduce_min_sync(0xffffffffu, sees ? vs[r].y : there ? -1 : 0x7fffffff);
         if (lane == 0) *(int4 *)(smem + C::OFF_GROUP + (s * 4 + r) * 16) = t;
       }
-      if (lane == 0) full_flag[s] = all.z <= k0 && all.w >= k1;
       sa_warp_arrive(&st_full[s], lane);
       if (++i == i0 + ni) { i = i0; ++g; }
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ------------------------------------------------------------------ P^T and dS^T: thread = key x 64 of the tile's queries
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const int r = quarter * 32 + lane, key = k0 + r;
-    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ------------------------------------------------------------------ P^T and dS^T: thread = key x 32 of the tile's queries
+    const int quarter = warp & 3, cols = (warp - 4) >> 2;
+    const int r = quarter * 32 + lane, key = k0 + r, kw = k0 + quarter * 32;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(cols * 32);
+    const pair32 ff = pair_of(p.factor, p.factor);
     bool ok = true;
     int g = 0, i = i0;
     for (int it = 0; it < n && ok; ++it) {
       const int s = it & 1;
       const uint32_t ph = (uint32_t)it & 1u;
-      const float *lse = (const float *)(smem + C::OFF_LSE) + s * SA_T + half * 64, *dlt = (const float *)(smem + C::OFF_DELTA) + s * SA_T + half * 64;
-      const int4 *sp = (const int4 *)(smem + C::OFF_SPAN) + (s * SA_T + half * 64) / 2;     // two spans each
+      const float *lse = (const float *)(smem + C::OFF_LSE) + s * SA_T + cols * 32, *dlt = (const float *)(smem + C::OFF_DELTA) + s * SA_T + cols * 32;
+      const int4 *sp = (const int4 *)(smem + C::OFF_SPAN) + (s * SA_T + cols * 32) / 2;       // two spans each
       ok = sa_wait(&st_full[s], (uint32_t)(it >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE) &&
            sa_wait(s_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       tc_fence_after();
-      // how this warp's 32 keys are seen by each 32 of the tile's queries
-      uint32_t none = 0, part = 0;
-      if (full_flag[s] == 0) {
-        const int a = k0 + quarter * 32;
+      // how this warp's 32 keys are seen by its 32 queries
+      const int4 seen = *(const int4 *)(smem + C::OFF_GROUP + (s * 4 + cols) * 16);
+      const bool none = seen.x > kw + 31 || seen.y < kw, masked = seen.z > kw || seen.w < kw + 31;
+      uint32_t y[32], pk[16];
+      if (none) {
 #pragma unroll
-        for (int gq = 0; gq < 2; ++gq) {
-          const int4 t = *(const int4 *)(smem + C::OFF_GROUP + (s * 4 + half * 2 + gq) * 16);
-          if (t.x > a + 31 || t.y < a) none |= 1u << gq;
-          else if (t.z > a || t.w < a + 31) part |= 1u << gq;
-        }
-      }
-      uint32_t x[64];
-      tmem_ld32(lane_base + C::TM_S, sa_group(x, 0));
-      tmem_ld32(lane_base + C::TM_S + 32u, sa_group(x, 1));
-      tmem_ld_wait();
-      uint32_t pk[32];
-      float slope = 0.f;
-      if constexpr (BIAS) slope = p.slopes[kh * group + g];
-      const pair32 ff = pair_of(p.factor, p.factor);
-#pragma unroll
-      for (int gq = 0; gq < 2; ++gq) {
-        uint32_t(&y)[32] = sa_group(x, gq);
-        if (none >> gq & 1u) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) y[c] = 0u;
-#pragma unroll
-          for (int c = 0; c < 16; ++c) pk[gq * 16 + c] = 0u;
-          continue;
-        }
-        const bool masked = part >> gq & 1u;
-        const int qg = i * SA_T + half * 64 + gq * 32, kw = k0 + quarter * 32;
+        for (int c = 0; c < 16; ++c) pk[c] = 0u;
+      } else {
+        tmem_ld32(lane_base + C::TM_S, y);
+        tmem_ld_wait();
         if (CAP && masked) {              // masked scores do not choose the way tanh is taken
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const int4 t = sp[gq * 16 + c / 2];
+            const int4 t = sp[c / 2];
             if (key < t.x || key > t.y) y[c] = 0u;
             if (key < t.z || key > t.w) y[c + 1] = 0u;
           }
         }
         sa_scores<CAP, false>(y, p, true, 0.f, 0.f, 0);
-        SaBias bias(slope, (float)(qg - key), qg >= kw + 31 ? 1 : qg + 31 <= kw ? -1 : 0);
+        const int qg = i * SA_T + cols * 32;
+        SaBias bias(BIAS ? p.slopes[kh * group + g] : 0.f, (float)(qg - key), qg >= kw + 31 ? 1 : qg + 31 <= kw ? -1 : 0);
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 w = *reinterpret_cast<const float4 *>(lse + gq * 32 + c);
-          float e[4];
-          pair32 w0 = pair_of(-w.x, -w.y), w1 = pair_of(-w.z, -w.w);
-          if constexpr (BIAS) { w0 = bias.next(w0); w1 = bias.next(w1); }
-          pair_to(pair_fma(pair_get(&y[c]), ff, w0), e[0], e[1]);
-          pair_to(pair_fma(pair_get(&y[c + 2]), ff, w1), e[2], e[3]);
+        for (int c = 0; c < 32; c += 16) {
+          float e[16];
+#pragma unroll
+          for (int u = 0; u < 16; u += 4) {
+            const float4 w = *reinterpret_cast<const float4 *>(lse + c + u);
+            pair32 w0 = pair_of(-w.x, -w.y), w1 = pair_of(-w.z, -w.w);
+            if constexpr (BIAS) { w0 = bias.next(w0); w1 = bias.next(w1); }
+            pair_to(pair_fma(pair_get(&y[c + u]), ff, w0), e[u], e[u + 1]);
+            pair_to(pair_fma(pair_get(&y[c + u + 2]), ff, w1), e[u + 2], e[u + 3]);
+          }
           if (masked) {
-            const int4 a = sp[gq * 16 + c / 2], z = sp[gq * 16 + c / 2 + 1];
-            if (key < a.x || key > a.y) e[0] = -INFINITY;
-            if (key < a.z || key > a.w) e[1] = -INFINITY;
-            if (key < z.x || key > z.y) e[2] = -INFINITY;
-            if (key < z.z || key > z.w) e[3] = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 16; u += 2) {
+              const int4 t = sp[(c + u) / 2];
+              if (key < t.x || key > t.y) e[u] = -INFINITY;
+              if (key < t.z || key > t.w) e[u + 1] = -INFINITY;
+            }
           }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) e[u] = sa_exp2(e[u]);
-          pk[gq * 16 + (c >> 1)] = pack_bf162(e[0], e[1]);
-          pk[gq * 16 + (c >> 1) + 1] = pack_bf162(e[2], e[3]);
-          // what dS needs of P: times the cap's derivative
-          if constexpr (CAP) {
-            sa_times_slope(y, c, e[0], e[1], p.to_z);
-            sa_times_slope(y, c + 2, e[2], e[3], p.to_z);
-          } else {
+          for (int u = 0; u < 16; ++u) e[u] = sa_exp2(e[u]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) y[c + u] = __float_as_uint(e[u]);
+          for (int u = 0; u < 16; u += 2) pk[(c + u) >> 1] = pack_bf162(e[u], e[u + 1]);
+          // what dS needs of P: times the cap's derivative
+#pragma unroll
+          for (int u = 0; u < 16; u += 2) {
+            if constexpr (CAP) {
+              sa_times_slope(y, c + u, e[u], e[u + 1], p.to_z);
+            } else {
+              y[c + u] = __float_as_uint(e[u]);
+              y[c + u + 1] = __float_as_uint(e[u + 1]);
+            }
           }
         }
       }
-      tmem_st32(lane_base + C::TM_S, pk);
+      sa_tmem_st16(lane_base + C::TM_S, pk);
       tmem_st_wait();
       tc_fence_before();
       sa_warp_arrive(p_full, lane);
       ok = sa_wait(dp_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       tc_fence_after();
-#pragma unroll
-      for (int gq = 0; gq < 2; ++gq) {
-        if (none >> gq & 1u) continue;    // zeros already
-        const uint32_t(&e)[32] = sa_group(x, gq);
-        uint32_t y[32];
-        tmem_ld32(lane_base + C::TM_DP + (uint32_t)(gq * 32), y);
+      if (!none) {
+        uint32_t z[32];
+        tmem_ld32(lane_base + C::TM_DP, z);
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          const float4 w = *reinterpret_cast<const float4 *>(dlt + gq * 32 + c);
+          const float4 w = *reinterpret_cast<const float4 *>(dlt + c);
           float v[4];
-          pair_to(pair_mul(pair_get(&e[c]), pair_add(pair_get(&y[c]), pair_of(-w.x, -w.y))), v[0], v[1]);
-          pair_to(pair_mul(pair_get(&e[c + 2]), pair_add(pair_get(&y[c + 2]), pair_of(-w.z, -w.w))), v[2], v[3]);
-          if (part >> gq & 1u) {
+          pair_to(pair_mul(pair_get(&y[c]), pair_add(pair_get(&z[c]), pair_of(-w.x, -w.y))), v[0], v[1]);
+          pair_to(pair_mul(pair_get(&y[c + 2]), pair_add(pair_get(&z[c + 2]), pair_of(-w.z, -w.w))), v[2], v[3]);
+          if (masked) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-              if (__uint_as_float(e[c + u]) == 0.f) v[u] = 0.f;                 // whatever dO and delta hold there
+              if (__uint_as_float(y[c + u]) == 0.f) v[u] = 0.f;                 // whatever dO and delta hold there
           }
-          pk[gq * 16 + (c >> 1)] = pack_bf162(v[0], v[1]);
-          pk[gq * 16 + (c >> 1) + 1] = pack_bf162(v[2], v[3]);
+          pk[c >> 1] = pack_bf162(v[0], v[1]);
+          pk[(c >> 1) + 1] = pack_bf162(v[2], v[3]);
         }
       }
-      tmem_st32(lane_base + C::TM_DP, pk);
+      sa_tmem_st16(lane_base + C::TM_DP, pk);
       tmem_st_wait();
       tc_fence_before();
       sa_warp_arrive(ds_full, lane);
@@ -466,33 +448,32 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tc_fence_after();
     }
     if (ok) {
+      // eight warps store dK, eight dV; a thread half of its key's columns
       constexpr int DH = DT / 2;
+      const int w = cols & 1, half = cols >> 1;
       const long long row = (long long)b * p.S + key;
       const uint32_t t_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
+      const float f = w == 0 ? p.scale : 1.f;
+      bf16 *orow = (w == 0 ? p.dK + row * p.lddk : p.dV + row * p.lddv) + (long long)kh * p.D + half * DH;
 #pragma unroll 1
-      for (int w = 0; w < 2; ++w) {
-        const float f = w == 0 ? p.scale : 1.f;
-        bf16 *orow = (w == 0 ? p.dK + row * p.lddk : p.dV + row * p.lddv) + (long long)kh * p.D + half * DH;
-#pragma unroll 1
-        for (int c = 0; c < DH / 32; ++c) {
-          uint32_t o[32];
-          if (n > 0) {
-            tmem_ld32(t_base + (uint32_t)((w == 0 ? C::TM_DK : C::TM_DV) + half * DH + c * 32), o);
-            tmem_ld_wait();
-          } else {
+      for (int c = 0; c < DH / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(t_base + (uint32_t)((w == 0 ? C::TM_DK : C::TM_DV) + half * DH + c * 32), o);
+          tmem_ld_wait();
+        } else {
 #pragma unroll
-            for (int u = 0; u < 32; ++u) o[u] = 0u;
-          }
-          if (key < p.S) {
+          for (int u = 0; u < 32; ++u) o[u] = 0u;
+        }
+        if (key < p.S) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (half * DH + c * 32 + 8 * u < p.D)
-                *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) =
-                    make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * f, __uint_as_float(o[8 * u + 1]) * f),
-                               pack_bf162(__uint_as_float(o[8 * u + 2]) * f, __uint_as_float(o[8 * u + 3]) * f),
-                               pack_bf162(__uint_as_float(o[8 * u + 4]) * f, __uint_as_float(o[8 * u + 5]) * f),
-                               pack_bf162(__uint_as_float(o[8 * u + 6]) * f, __uint_as_float(o[8 * u + 7]) * f));
-          }
+          for (int u = 0; u < 4; ++u)
+            if (half * DH + c * 32 + 8 * u < p.D)
+              *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) =
+                  make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * f, __uint_as_float(o[8 * u + 1]) * f),
+                             pack_bf162(__uint_as_float(o[8 * u + 2]) * f, __uint_as_float(o[8 * u + 3]) * f),
+                             pack_bf162(__uint_as_float(o[8 * u + 4]) * f, __uint_as_float(o[8 * u + 5]) * f),
+                             pack_bf162(__uint_as_float(o[8 * u + 6]) * f, __uint_as_float(o[8 * u + 7]) * f));
         }
       }
       tc_fence_before();
@@ -544,10 +525,10 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t *v_empty = bars + 12;      // [NV]
   uint64_t *s_full = bars + 14;       // [2]
   uint64_t *dp_full = bars + 16;
-  uint64_t *dp_free = bars + 17;      // eight warps
+  uint64_t *dp_free = bars + 17;      // SAB_WARPS
   // two, for the warps may be a tile apart (dP of the next one is there as soon as all have read this one's): an arrival for the next tile
   // must not count for this one
-  uint64_t *ds_full = bars + 18;      // [2] eight warps
+  uint64_t *ds_full = bars + 18;      // [2] SAB_WARPS
   uint64_t *dq_full = bars + 20;
   uint32_t *tmem_slot = (uint32_t *)(bars + 21);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
@@ -568,8 +549,8 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_ready[s], 1); mbar_init(&k_empty[s], 1); }
     for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
     mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
-    mbar_init(&ds_full[0], 8); mbar_init(&ds_full[1], 8);
-    mbar_init(dp_full, 1); mbar_init(dp_free, 8); mbar_init(dq_full, 1);
+    mbar_init(&ds_full[0], SAB_WARPS); mbar_init(&ds_full[1], SAB_WARPS);
+    mbar_init(dp_full, 1); mbar_init(dp_free, SAB_WARPS); mbar_init(dq_full, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -596,9 +577,9 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   const int j0 = last < 0 ? 0 : first / SA_T;
   const int n = last < 0 ? 0 : last / SA_T - j0 + 1;
 
-  // the element-wise warps hold half a row of a tile each: registers go from the warps that move data to them (128 x 104 + 256 x 200)
+  // registers go from the warps that move data to the element-wise ones (128 x 64 + 512 x 104 = 640 x 96)
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -706,7 +687,7 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         else tc_mma_ts_bf16<true>(d, a, bn, id_g);
 #pragma unroll
         for (int s = 1; s < SA_T / 16; ++s)
-          tc_mma_ts_bf16<true>(d, a + (uint32_t)((s >> 2) * 64 + (s & 3) * 8), desc_advance(bn, (uint32_t)(s * 2048)), id_g);
+          tc_mma_ts_bf16<true>(d, a + (uint32_t)((s >> 1) * 32 + (s & 1) * 8), desc_advance(bn, (uint32_t)(s * 2048)), id_g);
         tc_commit(&k_empty[i % C::NK]);
         if (i + 1 == n) tc_commit(dq_full);
       }
@@ -735,90 +716,84 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ------------------------------------------------------------------ dS: thread = query x 64 of the tile's keys
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const int r = quarter * 32 + lane, q = q0 + r;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ------------------------------------------------------------------ dS: thread = query x 32 of the tile's keys
+    const int quarter = warp & 3, cols = (warp - 4) >> 2;
+    const int r = quarter * 32 + lane, q = q0 + r, q_low = q - lane;
     const int2 mine = span[r];
     const bool empty = mine.x > mine.y;
     const int lo = empty ? -1 : mine.x, hi = empty ? 0x7ffffff0 : mine.y;      // see the forward kernel
-    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(cols * 32);
     const float slope = BIAS ? p.slopes[h] : 0.f;
-    const int q_low = q - lane;
     const long long stat = ((long long)b * p.H + h) * p.S + q;
     const float neg_lse = empty ? -INFINITY : -p.lse[stat], neg_delta = empty ? 0.f : -p.delta[stat];
     const pair32 nl = pair_of(neg_lse, neg_lse), nd = pair_of(neg_delta, neg_delta), ff = pair_of(p.factor, p.factor);
     bool ok = true;
     for (int i = 0; i < n && ok; ++i) {
       const uint32_t ph = (uint32_t)i & 1u;
-      const int k0 = (j0 + i) * SA_T + half * 64;
+      const int kg = (j0 + i) * SA_T + cols * 32;
       const uint32_t t_s = lane_base + (uint32_t)(C::TM_S + (i & 1) * SA_T);
+      const bool masked = !__all_sync(0xffffffffu, lo <= kg && hi >= kg + 31);
+      const bool none = masked && !__any_sync(0xffffffffu, lo <= kg + 31 && hi >= kg);
       ok = sa_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       tc_fence_after();
-      uint32_t x[64];
-      tmem_ld32(t_s, sa_group(x, 0));
-      tmem_ld32(t_s + 32u, sa_group(x, 1));
-      tmem_ld_wait();
-      uint32_t none, part;
-      sa_kinds<2>(lo, hi, k0, none, part);
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (none >> g & 1u) continue;
-        const int kg = k0 + g * 32;
-        uint32_t(&y)[32] = sa_group(x, g);
-        if (CAP && (part >> g & 1u)) sa_mask(y, lo - kg, hi - kg, 0u);
+      uint32_t y[32], pk[16];
+      if (!none) {
+        tmem_ld32(t_s, y);
+        tmem_ld_wait();
+        if (CAP && masked) sa_mask(y, lo - kg, hi - kg, 0u);       // masked scores do not choose the way tanh is taken
         sa_scores<CAP, false>(y, p, !empty, 0.f, 0.f, 0);
         SaBias bias(slope, (float)(kg - q), kg + 31 <= q_low ? -1 : kg >= q_low + 31 ? 1 : 0);
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          float e[4];
-          pair_to(pair_fma(pair_get(&y[c]), ff, BIAS ? bias.next(nl) : nl), e[0], e[1]);
-          pair_to(pair_fma(pair_get(&y[c + 2]), ff, BIAS ? bias.next(nl) : nl), e[2], e[3]);
-          if (part >> g & 1u) {
+        for (int c = 0; c < 32; c += 16) {
+          float e[16];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+          for (int u = 0; u < 16; u += 2) pair_to(pair_fma(pair_get(&y[c + u]), ff, BIAS ? bias.next(nl) : nl), e[u], e[u + 1]);
+          if (masked) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
               if (c + u < lo - kg || c + u > hi - kg) e[u] = -INFINITY;
           }
 #pragma unroll
-          for (int u = 0; u < 4; ++u) e[u] = sa_exp2(e[u]);
-          if constexpr (CAP) {
-            sa_times_slope(y, c, e[0], e[1], p.to_z);
-            sa_times_slope(y, c + 2, e[2], e[3], p.to_z);
-          } else {
+          for (int u = 0; u < 16; ++u) e[u] = sa_exp2(e[u]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) y[c + u] = __float_as_uint(e[u]);
+          for (int u = 0; u < 16; u += 2) {
+            if constexpr (CAP) {
+              sa_times_slope(y, c + u, e[u], e[u + 1], p.to_z);
+            } else {
+              y[c + u] = __float_as_uint(e[u]);
+              y[c + u + 1] = __float_as_uint(e[u + 1]);
+            }
           }
         }
       }
       ok = sa_wait(dp_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       tc_fence_after();
-      uint32_t y[64];
-      tmem_ld32(lane_base + C::TM_DP, *reinterpret_cast<uint32_t(*)[32]>(&y[0]));
-      tmem_ld32(lane_base + C::TM_DP + 32u, *reinterpret_cast<uint32_t(*)[32]>(&y[32]));
-      tmem_ld_wait();
+      uint32_t z[32];
+      if (!none) {
+        tmem_ld32(lane_base + C::TM_DP, z);
+        tmem_ld_wait();
+      }
       tc_fence_before();
       sa_warp_arrive(dp_free, lane);
+      if (none) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        if (none >> g & 1u) {
+        for (int c = 0; c < 16; ++c) pk[c] = 0u;
+      } else {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) y[g * 16 + c] = 0u;
-          continue;
-        }
-#pragma unroll
-        for (int c = g * 32; c < g * 32 + 32; c += 2) {
+        for (int c = 0; c < 32; c += 2) {
           float e0, e1;
-          pair_to(pair_mul(pair_get(&x[c]), pair_add(pair_get(&y[c]), nd)), e0, e1);
-          if (part >> g & 1u) {           // whatever V and delta hold there
-            if (__uint_as_float(x[c]) == 0.f) e0 = 0.f;
-            if (__uint_as_float(x[c + 1]) == 0.f) e1 = 0.f;
+          pair_to(pair_mul(pair_get(&y[c]), pair_add(pair_get(&z[c]), nd)), e0, e1);
+          if (masked) {                   // whatever V and delta hold there
+            if (__uint_as_float(y[c]) == 0.f) e0 = 0.f;
+            if (__uint_as_float(y[c + 1]) == 0.f) e1 = 0.f;
           }
-          y[c >> 1] = pack_bf162(e0, e1);
+          pk[c >> 1] = pack_bf162(e0, e1);
         }
       }
-      tmem_st32(t_s, *reinterpret_cast<uint32_t(*)[32]>(&y[0]));
+      sa_tmem_st16(t_s, pk);
       tmem_st_wait();
       tc_fence_before();
       sa_warp_arrive(&ds_full[i & 1], lane);
@@ -828,27 +803,24 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       tc_fence_after();
     }
     if (ok) {
-      constexpr int DH = DT / 2;
-      const uint32_t t_q = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(C::TM_DQ + half * DH);
-      bf16 *orow = p.dQ + ((long long)b * p.S + q) * p.lddq + (long long)h * p.D + half * DH;
-#pragma unroll 1
-      for (int c = 0; c < DH / 32; ++c) {
+      if (cols * 32 < DT) {               // a thread 32 of its query's columns
         uint32_t o[32];
         if (n > 0) {
-          tmem_ld32(t_q + (uint32_t)(c * 32), o);
+          tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(C::TM_DQ + cols * 32), o);
           tmem_ld_wait();
         }
+        bf16 *orow = p.dQ + ((long long)b * p.S + q) * p.lddq + (long long)h * p.D + cols * 32;
         if (q < p.S) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            if (half * DH + c * 32 + 8 * u < p.D) {
+            if (cols * 32 + 8 * u < p.D) {
               uint4 v = make_uint4(0, 0, 0, 0);
               if (!empty)
                 v = make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * p.scale, __uint_as_float(o[8 * u + 1]) * p.scale),
                                pack_bf162(__uint_as_float(o[8 * u + 2]) * p.scale, __uint_as_float(o[8 * u + 3]) * p.scale),
                                pack_bf162(__uint_as_float(o[8 * u + 4]) * p.scale, __uint_as_float(o[8 * u + 5]) * p.scale),
                                pack_bf162(__uint_as_float(o[8 * u + 6]) * p.scale, __uint_as_float(o[8 * u + 7]) * p.scale));
-              *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) = v;
+              *reinterpret_cast<uint4 *>(orow + 8 * u) = v;
             }
         }
       }
