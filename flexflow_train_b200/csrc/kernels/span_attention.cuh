@@ -43,13 +43,9 @@ struct SpanArgs {
   float to_z, from_z;              // with a cap: scale / cap and cap / scale
   float lim2, lim4;                // |raw score| up to which tanh is a polynomial of degree 2 or 4 in its square; negative: nowhere
   float t2[3], t4[5];              // the polynomials' coefficients, for raw scores
-  bf16 *O;
-  long long ldo;
   float *lse;
   const float *delta;
   const int4 *summary;
-  bf16 *dQ, *dK, *dV;
-  long long lddq, lddk, lddv;
   int tiles;                       // forward: 128-query tiles of a CTA, 1 or 2
   int *err;
 };
@@ -219,26 +215,41 @@ __device__ __forceinline__ void sa_mask(uint32_t (&x)[32], int a, int z, uint32_
     if (i < a || i > z) x[i] = v;
 }
 
-// Clears the rows of a tile (panels of 64 columns, 128 bytes a row) whose bit in `keep` (four words, 32 rows each) is not set.  One warp.
-__device__ __forceinline__ void sa_clear_rows(uint8_t *tile, int panels, const uint32_t (&keep)[4], int lane) {
-  const int per_row = panels * 8;                        // 16-byte pieces
-  const int at_once = 32 / per_row;                      // rows a warp clears at once
+// Clears the rows of a tile (panels of 64 columns, 128 bytes a row) whose bit in `keep` (four words, 32 rows each) is not set.  One warp, a
+// lane per row; lanes begin at different pieces of their rows, so that four and not 32 of them share a bank.
+template <int PANELS>
+__device__ __forceinline__ void sa_clear_rows(uint8_t *tile, const uint32_t (&keep)[4], int lane) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    uint32_t drop = ~keep[w];
-    while (drop) {
-      // the rows of the `at_once` lowest bits
-      int mine = -1;
-      for (int i = 0; i < at_once && drop; ++i) {
-        const int r = __ffs(drop) - 1;
-        drop &= drop - 1;
-        if (lane / per_row == i) mine = w * 32 + r;
-      }
-      if (mine >= 0) {
-        const int c = lane % per_row;
-        *reinterpret_cast<uint4 *>(tile + (c >> 3) * SA_PANEL + mine * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-      }
+  for (int w = 0; w < 4; ++w)
+    if (!(keep[w] >> lane & 1u)) {
+#pragma unroll
+      for (int c = 0; c < PANELS * 8; ++c)
+        *reinterpret_cast<uint4 *>(tile + (c >> 3) * SA_PANEL + (w * 32 + lane) * 128 + ((c + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
     }
+}
+
+// 32 columns of a row (from column `col` on, a multiple of 32) into a tile in shared memory as TMA reads it: 16-byte piece XOR (row % 8)
+__device__ __forceinline__ void sa_tile_row(uint8_t *tile, int row, int col, const uint32_t (&o)[32], float f) {
+  uint8_t *base = tile + (col >> 6) * SA_PANEL + row * 128;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    *reinterpret_cast<uint4 *>(base + ((((col & 63) >> 3) + u) ^ (row & 7)) * 16) =
+        make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * f, __uint_as_float(o[8 * u + 1]) * f),
+                   pack_bf162(__uint_as_float(o[8 * u + 2]) * f, __uint_as_float(o[8 * u + 3]) * f),
+                   pack_bf162(__uint_as_float(o[8 * u + 4]) * f, __uint_as_float(o[8 * u + 5]) * f),
+                   pack_bf162(__uint_as_float(o[8 * u + 6]) * f, __uint_as_float(o[8 * u + 7]) * f));
+}
+// The tile that `threads` threads (named barrier `id`) have written goes out by TMA, which leaves out what lies behind the sequence or the
+// head's columns; thread `first` issues and waits until it is written.
+template <int PANELS>
+__device__ __forceinline__ void sa_tile_out(uint8_t *tile, const CUtensorMap *map, int row, int head, int b, int id, int threads, bool first) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+  if (first) {
+#pragma unroll
+    for (int c = 0; c < PANELS; ++c) tma_store_4d(smem_u32(tile + c * SA_PANEL), map, c * 64, row, head, b);
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 }
 
@@ -293,7 +304,7 @@ inline void sa_args(const FfkSpanAttnDesc *d, SpanArgs &a, int *err) {
       a.lim4 = 0.625f / z;
     }
   }
-  a.O = (bf16 *)d->O; a.ldo = d->ldo; a.lse = d->lse;
+  a.lse = d->lse;
   a.err = err;
 }
 

@@ -37,11 +37,13 @@ __global__ void __launch_bounds__(256) span_attn_prep_kernel(const bf16 *dO, lon
   pdl_entry();
   const int lane = threadIdx.x & 31;
   if ((int)blockIdx.x < delta_blocks) {
-    const long long at = ((long long)blockIdx.x * 256 + threadIdx.x) / L, total = (long long)p.B * p.S * p.H;
+    // (row, head) pairs are counted in 32 bits (checked at the launch): 64-bit divisions had bounded this kernel
+    const unsigned at = blockIdx.x * (256 / L) + threadIdx.x / L, total = (unsigned)p.B * p.S * p.H;
     const int c = (threadIdx.x % L) * 8;
     const bool here = at < total;
-    const int h = (int)(at % p.H);
-    const long long row = at / p.H;
+    const unsigned row32 = at / (unsigned)p.H;
+    const int h = (int)(at - row32 * p.H);
+    const long long row = row32;
     float s = 0.f;
     if (here && c < p.D) {
       const uint4 u = *reinterpret_cast<const uint4 *>(dO + row * lddo + (long long)h * p.D + c);
@@ -56,8 +58,8 @@ __global__ void __launch_bounds__(256) span_attn_prep_kernel(const bf16 *dO, lon
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (here && c == 0) {
-      const long long b = row / p.S, q = row - b * p.S;
-      delta[(b * p.H + h) * p.S + q] = s;
+      const unsigned b = row32 / (unsigned)p.S, q = row32 - b * p.S;
+      delta[((long long)b * p.H + h) * p.S + q] = s;
     }
     return;
   }
@@ -107,7 +109,7 @@ struct DkvCfg {
 template <int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(SAB_THREADS, 1)
 span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                     const __grid_constant__ CUtensorMap tmDO, const SpanArgs p) {
+                     const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV, const SpanArgs p) {
   using C = DkvCfg<DT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -282,8 +284,8 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ok = sa_wait(&qd_full[s], (uint32_t)(it >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
-        sa_clear_rows(smem + C::OFF_Q + s * C::TILE, C::PANELS, keep, lane);
-        sa_clear_rows(smem + C::OFF_DO + s * C::TILE, C::PANELS, keep, lane);
+        sa_clear_rows<C::PANELS>(smem + C::OFF_Q + s * C::TILE, keep, lane);
+        sa_clear_rows<C::PANELS>(smem + C::OFF_DO + s * C::TILE, keep, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       sa_warp_arrive(&qd_ready[s], lane);
@@ -448,34 +450,23 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tc_fence_after();
     }
     if (ok) {
-      // eight warps store dK, eight dV; a thread half of its key's columns
+      // eight warps store dK, eight dV, through the places of Q and dO: the last products have read those
       constexpr int DH = DT / 2;
       const int w = cols & 1, half = cols >> 1;
-      const long long row = (long long)b * p.S + key;
-      const uint32_t t_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
-      const float f = w == 0 ? p.scale : 1.f;
-      bf16 *orow = (w == 0 ? p.dK + row * p.lddk : p.dV + row * p.lddv) + (long long)kh * p.D + half * DH;
+      uint8_t *tile = smem + (w == 0 ? C::OFF_Q : C::OFF_DO);
 #pragma unroll 1
       for (int c = 0; c < DH / 32; ++c) {
         uint32_t o[32];
         if (n > 0) {
-          tmem_ld32(t_base + (uint32_t)((w == 0 ? C::TM_DK : C::TM_DV) + half * DH + c * 32), o);
+          tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((w == 0 ? C::TM_DK : C::TM_DV) + half * DH + c * 32), o);
           tmem_ld_wait();
         } else {
 #pragma unroll
           for (int u = 0; u < 32; ++u) o[u] = 0u;
         }
-        if (key < p.S) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (half * DH + c * 32 + 8 * u < p.D)
-              *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) =
-                  make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * f, __uint_as_float(o[8 * u + 1]) * f),
-                             pack_bf162(__uint_as_float(o[8 * u + 2]) * f, __uint_as_float(o[8 * u + 3]) * f),
-                             pack_bf162(__uint_as_float(o[8 * u + 4]) * f, __uint_as_float(o[8 * u + 5]) * f),
-                             pack_bf162(__uint_as_float(o[8 * u + 6]) * f, __uint_as_float(o[8 * u + 7]) * f));
-        }
+        sa_tile_row(tile, r, half * DH + c * 32, o, w == 0 ? p.scale : 1.f);
       }
+      sa_tile_out<C::PANELS>(tile, w == 0 ? &tmDK : &tmDV, k0, kh, b, 1 + w, 256, warp == 4 + 4 * w && lane == 0);
       tc_fence_before();
     }
   }
@@ -510,7 +501,7 @@ struct DqCfg {
 template <int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(SAB_THREADS, 1)
 span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    const __grid_constant__ CUtensorMap tmDO, const SpanArgs p) {
+                    const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDQ, const SpanArgs p) {
   using C = DqCfg<DT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -709,7 +700,7 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       ok = sa_wait(&k_full[s], (uint32_t)(i / C::NK) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
-        sa_clear_rows(smem + C::OFF_K + s * C::TILE, C::PANELS, keep, lane);
+        sa_clear_rows<C::PANELS>(smem + C::OFF_K + s * C::TILE, keep, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       sa_warp_arrive(&k_ready[s], lane);
@@ -803,26 +794,18 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       tc_fence_after();
     }
     if (ok) {
-      if (cols * 32 < DT) {               // a thread 32 of its query's columns
+      if (cols * 32 < DT) {               // a thread 32 of its query's columns, through the place of Q
         uint32_t o[32];
         if (n > 0) {
           tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(C::TM_DQ + cols * 32), o);
           tmem_ld_wait();
         }
-        bf16 *orow = p.dQ + ((long long)b * p.S + q) * p.lddq + (long long)h * p.D + cols * 32;
-        if (q < p.S) {
+        if (empty) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (cols * 32 + 8 * u < p.D) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (!empty)
-                v = make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * p.scale, __uint_as_float(o[8 * u + 1]) * p.scale),
-                               pack_bf162(__uint_as_float(o[8 * u + 2]) * p.scale, __uint_as_float(o[8 * u + 3]) * p.scale),
-                               pack_bf162(__uint_as_float(o[8 * u + 4]) * p.scale, __uint_as_float(o[8 * u + 5]) * p.scale),
-                               pack_bf162(__uint_as_float(o[8 * u + 6]) * p.scale, __uint_as_float(o[8 * u + 7]) * p.scale));
-              *reinterpret_cast<uint4 *>(orow + 8 * u) = v;
-            }
+          for (int u = 0; u < 32; ++u) o[u] = 0u;
         }
+        sa_tile_row(smem + C::OFF_Q, r, cols * 32, o, p.scale);
+        sa_tile_out<C::PANELS>(smem + C::OFF_Q, &tmDQ, q0, h, b, 1, DT * 4, warp == 4 && lane == 0);
       }
       tc_fence_before();
     }
@@ -836,7 +819,7 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   }
 }
 
-struct SpanMaps { CUtensorMap q, k, v, dout; };
+struct SpanMaps { CUtensorMap q, k, v, dout, dq, dk, dv; };
 
 template <int DT, bool CAP, bool BIAS>
 int launch_bwd(const SpanMaps &m, const SpanArgs &a, cudaStream_t st) {
@@ -846,9 +829,10 @@ int launch_bwd(const SpanMaps &m, const SpanArgs &a, cudaStream_t st) {
   e = ffk_allow_smem(span_attn_dq_kernel<DT, CAP, BIAS>, DqCfg<DT>::SMEM, done_q);
   if (e != cudaSuccess) return (int)e;
   const long long tiles = (a.S + SA_T - 1) / SA_T;
-  int r = ffk_launch(span_attn_dkv_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.KH), SAB_THREADS, DkvCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, a);
+  int r = ffk_launch(span_attn_dkv_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.KH), SAB_THREADS, DkvCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, m.dk, m.dv,
+                     a);
   if (r) return r;
-  return ffk_launch(span_attn_dq_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.H), SAB_THREADS, DqCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, a);
+  return ffk_launch(span_attn_dq_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.H), SAB_THREADS, DqCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, m.dq, a);
 }
 
 long long delta_floats(long long B, long long H, long long S) { return (B * H * S + 3) / 4 * 4; }
@@ -869,20 +853,22 @@ FFK_API int ffk_span_attention_bwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
   const long long tiles = (d->S + SA_T - 1) / SA_T, rows = (long long)d->B * d->S * d->H;
   const int lanes = d->D <= 64 ? 8 : 16;
   const long long delta_blocks = (rows * lanes + 255) / 256, sum_blocks = (d->B * tiles + 7) / 8;
-  if (tiles * d->B * d->H > 0x7fffffffll || delta_blocks + sum_blocks > 0x7fffffffll) return -2;
+  if (tiles * d->B * d->H > 0x7fffffffll || rows > 0x7fffffffll || delta_blocks + sum_blocks > 0x7fffffffll) return -2;
   SpanMaps m;
   int r;
   if ((r = sa_head_map(&m.q, d->Q, d->D, d->S, d->ldq, d->H, d->B))) return r;
   if ((r = sa_head_map(&m.k, d->K, d->D, d->S, d->ldk, d->KH, d->B))) return r;
   if ((r = sa_head_map(&m.v, d->V, d->D, d->S, d->ldv, d->KH, d->B))) return r;
   if ((r = sa_head_map(&m.dout, d->dO, d->D, d->S, d->lddo, d->H, d->B))) return r;
+  if ((r = sa_head_map(&m.dq, d->dQ, d->D, d->S, d->lddq, d->H, d->B))) return r;
+  if ((r = sa_head_map(&m.dk, d->dK, d->D, d->S, d->lddk, d->KH, d->B))) return r;
+  if ((r = sa_head_map(&m.dv, d->dV, d->D, d->S, d->lddv, d->KH, d->B))) return r;
   SpanArgs a = {};
   sa_args(d, a, ffk_span_attention_err());
   float *delta = d->scratch;
   int4 *summary = reinterpret_cast<int4 *>(d->scratch + delta_floats(d->B, d->H, d->S));
   a.delta = delta;
   a.summary = summary;
-  a.dQ = (bf16 *)d->dQ; a.lddq = d->lddq; a.dK = (bf16 *)d->dK; a.lddk = d->lddk; a.dV = (bf16 *)d->dV; a.lddv = d->lddv;
   FfkTraffic traffic((long long)d->B * d->S * d->D * 4 * (d->H + d->KH));
   const unsigned blocks = (unsigned)(delta_blocks + sum_blocks);
   r = lanes == 8 ? ffk_launch(span_attn_prep_kernel<8>, blocks, 256, 0, st, (const bf16 *)d->dO, d->lddo, (const bf16 *)d->O, d->ldo, delta, summary,

@@ -39,7 +39,7 @@ struct SafCfg {
 template <int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(SAF_THREADS, 1)
 span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                     const SpanArgs p) {
+                     const __grid_constant__ CUtensorMap tmO, const SpanArgs p) {
   using C = SafCfg<DT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -269,7 +269,7 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ok = sa_wait(&v_full[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
-        sa_clear_rows(smem + C::OFF_V + (i % C::NV) * C::TILE, C::PANELS, keep, lane);
+        sa_clear_rows<C::PANELS>(smem + C::OFF_V + (i % C::NV) * C::TILE, keep, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       sa_warp_arrive(&v_ready[i % C::NV], lane);
@@ -377,29 +377,22 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const bool stored = t * SA_T + r < rows_cta && q < p.S;
       const float inv = empty || !(l != 0.f) ? 0.f : 1.f / l;
       if (stored && p.lse) p.lse[((long long)b * p.H + h) * p.S + q] = empty ? 0.f : m + __log2f(l);
-      bf16 *orow = p.O + ((long long)b * p.S + q) * p.ldo + (long long)h * p.D;
+      // O goes out through the query tile's place: the last product has read that
+      uint8_t *tile = smem + C::OFF_Q + t * C::TILE;
 #pragma unroll 1
       for (int c = 0; c < DT / 32; ++c) {
         uint32_t o[32];
         if (steps > 0) {
-          tmem_ld32(t_o + (uint32_t)(c * 32), o);      // warp-wide: rows past the end read too and store nothing
+          tmem_ld32(t_o + (uint32_t)(c * 32), o);
           tmem_ld_wait();
         }
-        if (stored) {
+        if (empty) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if (c * 32 + 8 * u < p.D) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (!empty)
-                v = make_uint4(pack_bf162(__uint_as_float(o[8 * u]) * inv, __uint_as_float(o[8 * u + 1]) * inv),
-                               pack_bf162(__uint_as_float(o[8 * u + 2]) * inv, __uint_as_float(o[8 * u + 3]) * inv),
-                               pack_bf162(__uint_as_float(o[8 * u + 4]) * inv, __uint_as_float(o[8 * u + 5]) * inv),
-                               pack_bf162(__uint_as_float(o[8 * u + 6]) * inv, __uint_as_float(o[8 * u + 7]) * inv));
-              *reinterpret_cast<uint4 *>(orow + c * 32 + 8 * u) = v;
-            }
-          }
+          for (int u = 0; u < 32; ++u) o[u] = 0u;
         }
+        sa_tile_row(tile, r, c * 32, o, inv);
       }
+      if (t * SA_T < rows_cta && q0 + t * SA_T < p.S) sa_tile_out<C::PANELS>(tile, &tmO, q0 + t * SA_T, h, b, 1 + t, 128, warp == 4 + 4 * t && lane == 0);
       tc_fence_before();
     }
   }
@@ -415,11 +408,11 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 __device__ int g_span_attn_err = 0;
 
 template <int DT, bool CAP, bool BIAS>
-int launch_fwd(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const SpanArgs &a, long long grid, cudaStream_t st) {
+int launch_fwd(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const CUtensorMap &to, const SpanArgs &a, long long grid, cudaStream_t st) {
   static unsigned long long done = 0;
   const cudaError_t e = ffk_allow_smem(span_attn_fwd_kernel<DT, CAP, BIAS>, SafCfg<DT>::SMEM, done);
   if (e != cudaSuccess) return (int)e;
-  return ffk_launch(span_attn_fwd_kernel<DT, CAP, BIAS>, (unsigned)grid, SAF_THREADS, SafCfg<DT>::SMEM, st, tq, tk, tv, a);
+  return ffk_launch(span_attn_fwd_kernel<DT, CAP, BIAS>, (unsigned)grid, SAF_THREADS, SafCfg<DT>::SMEM, st, tq, tk, tv, to, a);
 }
 
 }  // namespace
@@ -433,11 +426,12 @@ FFK_API int ffk_span_attention_fwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
   if (d->B <= 0 || d->H <= 0 || d->S <= 0) return 0;
   if (!sa_shape_ok(d)) return -2;
   if (!sa_aligned(d->Q, d->ldq) || !sa_aligned(d->K, d->ldk) || !sa_aligned(d->V, d->ldv) || !sa_aligned(d->O, d->ldo)) return -2;
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   int r;
   if ((r = sa_head_map(&tq, d->Q, d->D, d->S, d->ldq, d->H, d->B))) return r;
   if ((r = sa_head_map(&tk, d->K, d->D, d->S, d->ldk, d->KH, d->B))) return r;
   if ((r = sa_head_map(&tv, d->V, d->D, d->S, d->ldv, d->KH, d->B))) return r;
+  if ((r = sa_head_map(&to, d->O, d->D, d->S, d->ldo, d->H, d->B))) return r;
   SpanArgs a = {};
   sa_args(d, a, ffk_span_attention_err());
   // two query tiles per CTA share the K and V tiles and the tensor core; one where that would leave SMs without work
@@ -448,11 +442,11 @@ FFK_API int ffk_span_attention_fwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
   FfkTraffic traffic((long long)d->B * d->S * d->D * 2 * (2 * d->H + 2 * d->KH));
   const bool cap = d->cap > 0.f, bias = d->slopes != nullptr;
   if (d->D <= 64) {
-    if (cap) return bias ? launch_fwd<64, true, true>(tq, tk, tv, a, grid, st) : launch_fwd<64, true, false>(tq, tk, tv, a, grid, st);
-    return bias ? launch_fwd<64, false, true>(tq, tk, tv, a, grid, st) : launch_fwd<64, false, false>(tq, tk, tv, a, grid, st);
+    if (cap) return bias ? launch_fwd<64, true, true>(tq, tk, tv, to, a, grid, st) : launch_fwd<64, true, false>(tq, tk, tv, to, a, grid, st);
+    return bias ? launch_fwd<64, false, true>(tq, tk, tv, to, a, grid, st) : launch_fwd<64, false, false>(tq, tk, tv, to, a, grid, st);
   }
-  if (cap) return bias ? launch_fwd<128, true, true>(tq, tk, tv, a, grid, st) : launch_fwd<128, true, false>(tq, tk, tv, a, grid, st);
-  return bias ? launch_fwd<128, false, true>(tq, tk, tv, a, grid, st) : launch_fwd<128, false, false>(tq, tk, tv, a, grid, st);
+  if (cap) return bias ? launch_fwd<128, true, true>(tq, tk, tv, to, a, grid, st) : launch_fwd<128, true, false>(tq, tk, tv, to, a, grid, st);
+  return bias ? launch_fwd<128, false, true>(tq, tk, tv, to, a, grid, st) : launch_fwd<128, false, false>(tq, tk, tv, to, a, grid, st);
 }
 
 // Reads (and clears) the error word of the bounded waits of both directions.  Synchronises the device.
