@@ -396,25 +396,31 @@ def attention_spans(documents, prompt=None, *, causal=True, out=None):
     documents [B, S] int32: a document is a run of equal numbers in a row; a negative number is padding, which sees nothing (first 0,
     last -1).  A token sees its own document: up to itself if `causal`, to the end otherwise.  prompt [B, S] (bool or uint8, with
     `causal` only): the flagged tokens that a document begins with are seen by all of its tokens."""
-    if documents.dim() != 2 or documents.dtype != torch.int32:
+    shape = documents.shape
+    if len(shape) != 2 or documents.dtype is not torch.int32:
         raise KernelError("attention_spans: documents is an int32 [batch, sequence] tensor")
-    B, S = documents.shape
+    B, S = shape
     if prompt is not None:
-        if prompt.dtype not in (torch.bool, torch.uint8) or prompt.shape != documents.shape:
+        if prompt.dtype not in (torch.bool, torch.uint8) or prompt.shape != shape:
             raise KernelError("attention_spans: prompt holds one bool or uint8 flag per token")
         if not causal:
             raise KernelError("attention_spans: a prompt is seen by all of its document anyway unless the mask is causal")
     if out is None:
         out = torch.empty(B, S, 2, dtype=torch.int32, device=documents.device)
-    if out.dtype != torch.int32 or tuple(out.shape) != (B, S, 2):
+    if out.dtype is not torch.int32 or out.shape != (B, S, 2):
         raise KernelError("attention_spans: out is an int32 [batch, sequence, 2] tensor")
     if B > 2**31 - 1 or S > 2**31 - 4096:
         raise KernelError("attention_spans: sequence too long")
-    _apart("attention_spans", ("documents", documents), ("out", out))
-    _apart("attention_spans", ("prompt", prompt), ("out", out))
-    _cuda_contig(documents, prompt, out)
-    _same_device(documents, prompt, out)
-    _check(_nlib().ffk_attention_spans(documents.data_ptr(), _p(prompt), out.data_ptr(), B, S, int(bool(causal)), _stream()), "ffk_attention_spans")
+    if not (documents.is_contiguous() and out.is_contiguous() and (prompt is None or prompt.is_contiguous())):
+        raise KernelError("kernel called with a non-contiguous tensor")
+    n, pd, pp, po = B * S, documents.data_ptr(), _p(prompt), out.data_ptr()
+    _apart("attention_spans", "documents", pd, 4 * n, "out", po, 8 * n)
+    if pp is not None:
+        _apart("attention_spans", "prompt", pp, n, "out", po, 8 * n)
+    if po % 8:
+        raise KernelError("attention_spans: out must start on an 8-byte boundary")
+    stream = _launch_stream(documents, prompt, out)
+    _check(_nlib().ffk_attention_spans(pd, pp, po, B, S, 1 if causal else 0, stream), "ffk_attention_spans")
     return out
 
 
@@ -428,49 +434,50 @@ def span_attention_last_error() -> int:
     return _nlib().ffk_span_attention_last_error()
 
 
-def _span_operand(what, name, t, rows, heads, D):
-    """A [B*S, >= heads*D] bf16 matrix with unit column stride whose rows TMA can address -> (pointer, leading dimension)."""
-    if t is None or t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] < heads * D or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
-    ld = t.stride(0) if rows > 1 else max(t.stride(0), (heads * D + 7) // 8 * 8)
-    if ld < heads * D or ld % 8 or t.data_ptr() % 16:
-        raise KernelError(f"{what}: {name} must start on a 16-byte boundary, at a pitch of a multiple of 8 elements that holds its heads")
-    return t.data_ptr(), ld
-
-
-def _span_desc(what, spans, B, S, H, KH, D, scale, cap, slopes):
-    if min(B, S) < 0 or H < 1 or KH < 1 or H % KH:
+def _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes):
+    """Checks of what both directions share."""
+    if B < 0 or S < 0 or H < 1 or KH < 1 or H % KH:
         raise KernelError(f"{what}: every key head serves the same number of query heads (H {H}, KH {KH}, B {B}, S {S})")
-    if not span_attention_supported(D):
+    if D < 8 or D > 128 or D % 8:
         raise KernelError(f"{what}: head dim {D} (a multiple of 8 up to 128 expected)")
-    if not (0.0 < scale < float("inf") and 0.0 <= cap < float("inf")):
+    if not (0.0 < scale < _INF and 0.0 <= cap < _INF):
         raise KernelError(f"{what}: scale must be positive and cap not negative")
-    if spans is None or spans.dtype != torch.int32 or tuple(spans.shape) != (B, S, 2) or not spans.is_contiguous() or spans.data_ptr() % 8:
+    if spans is None or spans.dtype is not torch.int32 or spans.shape != (B, S, 2) or not spans.is_contiguous() or spans.data_ptr() % 8:
         raise KernelError(f"{what}: spans is a contiguous int32 [B, S, 2] tensor (attention_spans)")
-    if slopes is not None and (slopes.dtype != torch.float32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous()):
+    if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous()):
         raise KernelError(f"{what}: slopes holds one fp32 value per query head")
-    d = SpanAttnDesc()
-    d.B, d.H, d.KH, d.S, d.D, d.scale, d.cap = B, H, KH, S, D, float(scale), float(cap)
-    d.spans, d.slopes = spans.data_ptr(), _p(slopes)
-    return d
+    if lse is None or lse.dtype is not torch.float32 or lse.shape != (B, H, S) or not lse.is_contiguous():
+        raise KernelError(f"{what}: lse must be a contiguous fp32 [B, H, S] tensor")
 
 
-def _span_apart(what, d, outs, ins, rows, widths):
-    """Refuses outputs that share memory with an input or with one another.  Two matrices of one pitch may lie side by side (views into a
-    packed buffer); `widths`: columns in use."""
-    def place(name):
-        return getattr(d, name), getattr(d, "ld" + name.lower()) * 2, widths[name] * 2
+_INF = float("inf")
 
-    plain = {"Q": "q", "K": "k", "V": "v", "O": "out", "dO": "dout", "dQ": "dq", "dK": "dk", "dV": "dv"}
-    for i, a in enumerate(outs):
-        for b in outs[i + 1:] + ins:
-            (pa, la, wa), (pb, lb, wb) = place(a), place(b)
-            if pa + (rows - 1) * la + wa <= pb or pb + (rows - 1) * lb + wb <= pa:
-                continue
-            gap = (pb - pa) % la
-            if la == lb and gap >= wa and gap + wb <= la:
-                continue
-            raise KernelError(f"{what}: {plain[a]} and {plain[b]} share memory")
+
+def _span_place(what, name, t, rows, width):
+    """A [B*S, >= width] bf16 matrix with unit column stride whose rows TMA can address: (name, address, pitch, width in bytes, end)."""
+    if t is None or t.dtype is not torch.bfloat16 or t.dim() != 2:
+        raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
+    (n, columns), (ld, one) = t.shape, t.stride()
+    if n != rows or columns < width or (one != 1 and columns > 1):
+        raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
+    if rows <= 1:
+        ld = width                       # a single row has no pitch
+    p = t.data_ptr()
+    if ld < width or ld % 8 or p % 16:
+        raise KernelError(f"{what}: {name} must start on a 16-byte boundary, at a pitch of a multiple of 8 elements that holds its heads")
+    return name, p, 2 * ld, 2 * width, p + 2 * ((rows - 1) * ld + width)
+
+
+def _span_apart(what, a, others):
+    """Refuses a matrix that shares memory with another.  Two of one pitch may lie side by side (views into a packed buffer)."""
+    name, p, ld, width, end = a
+    for other, q, lq, wq, last in others:
+        if end <= q or last <= p:
+            continue
+        gap = (q - p) % ld
+        if ld == lq and gap >= width and gap + wq <= ld:
+            continue
+        raise KernelError(f"{what}: {name} and {other} share memory")
 
 
 def span_attention_fwd(q, k, v, out, lse, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None):
@@ -482,50 +489,46 @@ def span_attention_fwd(q, k, v, out, lse, spans, *, B, S, H, KH, D, scale, cap=0
     (`attention_spans`, or any: what lies outside the sequence is cut off).  A query whose span is empty gets zeros.  lse [B, H, S]
     fp32 receives the base-2 log-sum-exp of x (0 for an empty span), which `span_attention_bwd` needs.  What tokens hold that no query
     sees does not matter, NaN included."""
-    d = _span_desc("span_attention_fwd", spans, B, S, H, KH, D, scale, cap, slopes)
-    rows = B * S
-    for f, ldf, name, t, heads in (("Q", "ldq", "q", q, H), ("K", "ldk", "k", k, KH), ("V", "ldv", "v", v, KH), ("O", "ldo", "out", out, H)):
-        ptr, ld = _span_operand("span_attention_fwd", name, t, rows, heads, D)
-        setattr(d, f, ptr)
-        setattr(d, ldf, ld)
-    if lse is None or lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or not lse.is_contiguous():
-        raise KernelError("span_attention_fwd: lse must be a contiguous fp32 [B, H, S] tensor")
+    what = "span_attention_fwd"
+    _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
+    rows, wide, narrow = B * S, H * D, KH * D
+    Q, Kp, V = _span_place(what, "q", q, rows, wide), _span_place(what, "k", k, rows, narrow), _span_place(what, "v", v, rows, narrow)
+    O = _span_place(what, "out", out, rows, wide)
     if rows:
-        _span_apart("span_attention_fwd", d, ["O"], ["Q", "K", "V"], rows, {"Q": H * D, "K": KH * D, "V": KH * D, "O": H * D})
-    d.lse = lse.data_ptr()
-    _same_device(q, k, v, out, lse, spans, slopes)
-    _check(_nlib().ffk_span_attention_fwd(ctypes.byref(d), _stream()), "ffk_span_attention_fwd")
+        _span_apart(what, O, (Q, Kp, V))
+    stream = _launch_stream(q, k, v, out, lse, spans, slopes)
+    d = SpanAttnDesc(B, H, KH, S, D, scale, cap, spans.data_ptr(), _p(slopes), Q[1], Q[2] >> 1, Kp[1], Kp[2] >> 1, V[1], V[2] >> 1, O[1], O[2] >> 1,
+                     lse.data_ptr())
+    _check(_nlib().ffk_span_attention_fwd(ctypes.byref(d), stream), what)
     return out
 
 
 def span_attention_bwd_scratch_floats(B, H, S) -> int:
     """fp32 elements of scratch `span_attention_bwd` needs."""
-    return int(_nlib().ffk_span_attention_bwd_scratch_floats(B, H, S))
+    return _nlib().ffk_span_attention_bwd_scratch_floats(B, H, S)
 
 
 def span_attention_bwd(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None):
     """Gradients of `span_attention_fwd` with respect to q, k and v (same layouts; dk and dv are summed over the query heads that share a
     key head).  out and lse are the forward pass's.  Every sum is taken in a fixed order: the same inputs give the same bits.  scratch:
     span_attention_bwd_scratch_floats(B, H, S) fp32 elements on a 16-byte boundary.  The slopes have no gradient."""
-    d = _span_desc("span_attention_bwd", spans, B, S, H, KH, D, scale, cap, slopes)
-    rows = B * S
-    for f, ldf, name, t, heads in (("Q", "ldq", "q", q, H), ("K", "ldk", "k", k, KH), ("V", "ldv", "v", v, KH), ("O", "ldo", "out", out, H),
-                                   ("dO", "lddo", "dout", dout, H), ("dQ", "lddq", "dq", dq, H), ("dK", "lddk", "dk", dk, KH),
-                                   ("dV", "lddv", "dv", dv, KH)):
-        ptr, ld = _span_operand("span_attention_bwd", name, t, rows, heads, D)
-        setattr(d, f, ptr)
-        setattr(d, ldf, ld)
-    if lse is None or lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or not lse.is_contiguous():
-        raise KernelError("span_attention_bwd: lse must be a contiguous fp32 [B, H, S] tensor")
-    if scratch is None or scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.data_ptr() % 16 or \
+    what = "span_attention_bwd"
+    _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
+    rows, wide, narrow = B * S, H * D, KH * D
+    Q, Kp, V = _span_place(what, "q", q, rows, wide), _span_place(what, "k", k, rows, narrow), _span_place(what, "v", v, rows, narrow)
+    O, dO = _span_place(what, "out", out, rows, wide), _span_place(what, "dout", dout, rows, wide)
+    dQ, dK, dV = _span_place(what, "dq", dq, rows, wide), _span_place(what, "dk", dk, rows, narrow), _span_place(what, "dv", dv, rows, narrow)
+    if scratch is None or scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.data_ptr() % 16 or \
             scratch.numel() < span_attention_bwd_scratch_floats(B, H, S):
-        raise KernelError("span_attention_bwd: scratch must hold span_attention_bwd_scratch_floats(B, H, S) fp32 elements")
+        raise KernelError(f"{what}: scratch must hold span_attention_bwd_scratch_floats(B, H, S) fp32 elements")
     if rows:
-        wide = {n: (KH if n[-1] in "KV" else H) * D for n in ("Q", "K", "V", "O", "dO", "dQ", "dK", "dV")}
-        _span_apart("span_attention_bwd", d, ["dQ", "dK", "dV"], ["Q", "K", "V", "O", "dO"], rows, wide)
-    d.lse, d.scratch = lse.data_ptr(), scratch.data_ptr()
-    _same_device(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, slopes)
-    _check(_nlib().ffk_span_attention_bwd(ctypes.byref(d), _stream()), "ffk_span_attention_bwd")
+        _span_apart(what, dQ, (dK, dV, Q, Kp, V, O, dO))
+        _span_apart(what, dK, (dV, Q, Kp, V, O, dO))
+        _span_apart(what, dV, (Q, Kp, V, O, dO))
+    stream = _launch_stream(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, slopes)
+    d = SpanAttnDesc(B, H, KH, S, D, scale, cap, spans.data_ptr(), _p(slopes), Q[1], Q[2] >> 1, Kp[1], Kp[2] >> 1, V[1], V[2] >> 1, O[1], O[2] >> 1,
+                     lse.data_ptr(), dO[1], dO[2] >> 1, dQ[1], dQ[2] >> 1, dK[1], dK[2] >> 1, dV[1], dV[2] >> 1, scratch.data_ptr())
+    _check(_nlib().ffk_span_attention_bwd(ctypes.byref(d), stream), what)
 
 
 def _es(t):
@@ -747,16 +750,27 @@ def loss_fwd(kind: str, pred, target, loss_rows):
                               _dt(pred), ldt, _stream()), "ffk_loss_fwd")
 
 
-def _same_device(*ts):
-    """Tensors of a call live on one device, which is the current one: the kernel is launched on its current stream."""
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) > 1:
-        raise KernelError(f"operands on different devices: {sorted(map(str, devices))}")
-    for d in devices:
-        if d.type != "cuda":
-            raise KernelError("kernel called with a CPU tensor")
-        if d.index != torch.cuda.current_device():
-            raise KernelError(f"operands on {d}, but cuda:{torch.cuda.current_device()} is the current device")
+def _launch_stream(*ts) -> int:
+    """The stream a kernel on these tensors is launched on: the current one of the current device, where all of them have to live (None
+    is skipped)."""
+    device = -2
+    for t in ts:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d != device:
+            if d < 0:
+                raise KernelError("kernel called with a CPU tensor")
+            if device >= 0:
+                raise KernelError(f"operands on cuda:{device} and on cuda:{d}")
+            device = d
+    if device != torch.cuda.current_device():
+        raise KernelError(f"operands on cuda:{device}, but cuda:{torch.cuda.current_device()} is the current device")
+    return _raw_stream(device)
+
+
+# the stream's handle without a Stream object around it (3 us less a call), where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _new_ops_decl(l):
@@ -792,84 +806,112 @@ def _nlib():
     return l
 
 
-def _rms_check(what, a, gamma, same, rstd):
-    """Checks of the RMS norm's operands: `a` [rows, cols], gamma [cols], tensors of a's shape, rstd [rows]."""
-    if a.dim() != 2:
+def _rms_check(what, a, gamma, rstd, same):
+    """Checks of the RMS norm's operands: `a` [rows, cols], gamma [cols], rstd [rows], (name, tensor) pairs of a's shape.  Everything is
+    contiguous.  Returns rows, cols and the tensors' bytes."""
+    shape, dtype = a.shape, a.dtype
+    if len(shape) != 2:
         raise KernelError(f"{what}: rows are a 2-D [rows, cols] tensor")
-    rows, cols = a.shape
-    if a.dtype not in (torch.float32, torch.bfloat16):
-        raise KernelError(f"{what}: bf16 or fp32 rows expected, got {a.dtype}")
+    rows, cols = shape
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise KernelError(f"{what}: bf16 or fp32 rows expected, got {dtype}")
     if cols < 1 or rows > 2**31 - 1 or cols > 2**31 - 1:
         raise KernelError(f"{what}: rows of {cols} elements")
-    for t in same:
-        if t is not None and (t.shape != a.shape or t.dtype != a.dtype):
+    for _, t in same:
+        if t is not None and (t.dtype is not dtype or t.shape != shape):
             raise KernelError(f"{what}: tensors of the rows' shape and dtype expected")
-    if gamma is None or gamma.dtype != a.dtype or tuple(gamma.shape) != (cols,):
+    if gamma is None or gamma.dtype is not dtype or gamma.shape != (cols,):
         raise KernelError(f"{what}: gamma must hold one value of the rows' dtype per column")
-    if rstd is not None and (rstd.dtype != torch.float32 or rstd.numel() != rows):
+    if rstd is not None and (rstd.dtype is not torch.float32 or rstd.numel() != rows):
         raise KernelError(f"{what}: rstd must be fp32 with one value per row")
+    for t in (a, gamma, rstd):
+        if t is not None and not t.is_contiguous():
+            raise KernelError("kernel called with a non-contiguous tensor")
+    for _, t in same:
+        if t is not None and not t.is_contiguous():
+            raise KernelError("kernel called with a non-contiguous tensor")
+    return rows, cols, rows * cols * (2 if dtype is torch.bfloat16 else 4)
 
 
-def _apart(what, *named):
-    """Refuses outputs that share memory with one another or with an input they may not replace: (name, tensor) pairs."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), n) for n, t in named if t is not None and t.numel())
-    for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
-        if start < end:
-            raise KernelError(f"{what}: {a} and {b} share memory")
-
-
-def _same_or_apart(what, out_name, out, others):
-    """An output that is read and written element by element may be one of the inputs, but not a part of one."""
-    for name, t in others:
-        if out is None or t is None or (out.data_ptr() == t.data_ptr() and out.numel() == t.numel()):
-            continue
-        _apart(what, (out_name, out), (name, t))
+def _apart(what, a, pa, na, b, pb, nb):
+    """Refuses two pieces of memory (name, address, bytes) that share some."""
+    if pa < pb + nb and pb < pa + na and na and nb:
+        raise KernelError(f"{what}: {a} and {b} share memory")
 
 
 def rmsnorm_fwd(a, gamma, eps, residual=None, xsum=None, out=None, rstd=None):
     """out = h / sqrt(mean(h^2) + eps) * gamma over the rows of h = a + residual (h = a without a residual), h rounded to the rows'
-    dtype.  xsum receives h, rstd (fp32, one per row) the reciprocal root, which `rmsnorm_bwd` needs.  `out` and `xsum` may be `a` or
-    `residual` themselves."""
-    _rms_check("rmsnorm_fwd", a, gamma, (residual, xsum, out), rstd)
-    out = torch.empty_like(a) if out is None else out
+    dtype (bf16 or fp32).  xsum receives h, rstd (fp32, one per row) the reciprocal root, which `rmsnorm_bwd` needs.  `out` and `xsum`
+    may be `a` or `residual` themselves."""
+    rows, cols, size = _rms_check("rmsnorm_fwd", a, gamma, rstd, (("residual", residual), ("xsum", xsum), ("out", out)))
     if xsum is not None and residual is None:
         raise KernelError("rmsnorm_fwd: xsum is the sum with a residual")
-    ins = (("a", a), ("residual", residual))
-    _same_or_apart("rmsnorm_fwd", "out", out, ins)
-    _same_or_apart("rmsnorm_fwd", "xsum", xsum, ins)
-    _apart("rmsnorm_fwd", ("out", out), ("xsum", xsum), ("gamma", gamma), ("rstd", rstd))
-    _cuda_contig(a, residual, gamma, xsum, out, rstd)
-    _same_device(a, residual, gamma, xsum, out, rstd)
-    rows, cols = a.shape
-    _check(_nlib().ffk_rmsnorm_fwd(a.data_ptr(), _p(residual), gamma.data_ptr(), _p(xsum), out.data_ptr(), _p(rstd), rows, cols, eps, _dt(a),
-                                   _stream()), "ffk_rmsnorm_fwd")
+    if out is None:
+        out = torch.empty_like(a)
+    pa, pg, po = a.data_ptr(), gamma.data_ptr(), out.data_ptr()
+    pr, px, ps = _p(residual), _p(xsum), _p(rstd)
+    small = gamma.numel() * gamma.element_size()
+    for name, p in (("out", po), ("xsum", px)):
+        if p is None:
+            continue
+        if p != pa:
+            _apart("rmsnorm_fwd", name, p, size, "a", pa, size)
+        if pr is not None and p != pr:
+            _apart("rmsnorm_fwd", name, p, size, "residual", pr, size)
+        _apart("rmsnorm_fwd", name, p, size, "gamma", pg, small)
+        if ps is not None:
+            _apart("rmsnorm_fwd", name, p, size, "rstd", ps, 4 * rows)
+    if px is not None:
+        _apart("rmsnorm_fwd", "out", po, size, "xsum", px, size)
+    if ps is not None:
+        for name, p, n in (("a", pa, size), ("residual", pr, size), ("gamma", pg, small)):
+            if p is not None:
+                _apart("rmsnorm_fwd", "rstd", ps, 4 * rows, name, p, n)
+    stream = _launch_stream(a, residual, gamma, xsum, out, rstd)
+    _check(_nlib().ffk_rmsnorm_fwd(pa, pr, pg, px, po, ps, rows, cols, eps, _DT[a.dtype], stream), "ffk_rmsnorm_fwd")
     return out
 
 
 def rmsnorm_bwd_scratch(rows, cols) -> int:
     """fp32 elements of scratch `rmsnorm_bwd` needs for [rows, cols]."""
-    return int(_nlib().ffk_rmsnorm_bwd_scratch(rows, cols))
+    return _nlib().ffk_rmsnorm_bwd_scratch(rows, cols)
 
 
 def rmsnorm_bwd(dy, x, gamma, rstd, dx, dgamma, scratch, dsum=None, accumulate_params=False):
     """Gradients of `rmsnorm_fwd`: x is what was normalized (`xsum` where there was a residual).  dx = gradient of x, to which `dsum`,
     the gradient that reaches x past the norm, is added: it is the gradient of both addends.  dgamma (None: not computed) (+)= its column
-    sums, added in a fixed order.  dx may be dy or dsum themselves.  scratch: rmsnorm_bwd_scratch(rows, cols) fp32 elements."""
-    _rms_check("rmsnorm_bwd", dy, gamma, (x, dx, dsum), rstd)
-    rows, cols = dy.shape
+    sums, added in a fixed order.  dx may be dy, x or dsum themselves.  scratch: rmsnorm_bwd_scratch(rows, cols) fp32 elements."""
     if rstd is None or x is None or dx is None:
         raise KernelError("rmsnorm_bwd: x, rstd and dx are needed")
+    rows, cols, size = _rms_check("rmsnorm_bwd", dy, gamma, rstd, (("x", x), ("dx", dx), ("dsum", dsum)))
+    px, pd, pg, ps = dx.data_ptr(), _p(dgamma), gamma.data_ptr(), rstd.data_ptr()
+    small, pc, nc = gamma.numel() * gamma.element_size(), None, 0
     if dgamma is not None:
-        if dgamma.dtype != dy.dtype or tuple(dgamma.shape) != (cols,):
+        if dgamma.dtype is not dy.dtype or dgamma.shape != (cols,) or not dgamma.is_contiguous():
             raise KernelError("rmsnorm_bwd: dgamma must be like gamma")
-        if rows and (scratch is None or scratch.dtype != torch.float32 or scratch.numel() < rmsnorm_bwd_scratch(rows, cols)):
-            raise KernelError("rmsnorm_bwd: scratch smaller than rmsnorm_bwd_scratch(rows, cols)")
-    _same_or_apart("rmsnorm_bwd", "dx", dx, (("dy", dy), ("x", x), ("dsum", dsum)))
-    _apart("rmsnorm_bwd", ("dx", dx), ("gamma", gamma), ("rstd", rstd), ("dgamma", dgamma), ("scratch", scratch if dgamma is not None else None))
-    _cuda_contig(dy, x, gamma, rstd, dx, dsum, dgamma, scratch)
-    _same_device(dy, x, gamma, rstd, dx, dsum, dgamma, scratch)
-    _check(_nlib().ffk_rmsnorm_bwd(dy.data_ptr(), x.data_ptr(), gamma.data_ptr(), rstd.data_ptr(), _p(dsum), dx.data_ptr(), _p(dgamma),
-                                   _p(scratch) if dgamma is not None else None, rows, cols, _dt(dy), int(accumulate_params), _stream()),
+        if rows:
+            nc = 4 * rmsnorm_bwd_scratch(rows, cols)
+            if scratch is None or scratch.dtype is not torch.float32 or 4 * scratch.numel() < nc or not scratch.is_contiguous():
+                raise KernelError("rmsnorm_bwd: scratch smaller than rmsnorm_bwd_scratch(rows, cols)")
+            pc = scratch.data_ptr()
+    py, ph, pu = dy.data_ptr(), x.data_ptr(), _p(dsum)
+    ins = [("dy", py, size), ("x", ph, size), ("gamma", pg, small), ("rstd", ps, 4 * rows)]
+    if pu is not None:
+        ins.append(("dsum", pu, size))
+    for name, p, n in ins:
+        if p != px or n != size:
+            _apart("rmsnorm_bwd", "dx", px, size, name, p, n)
+        if pd is not None:
+            _apart("rmsnorm_bwd", "dgamma", pd, small, name, p, n)
+            if pc is not None:
+                _apart("rmsnorm_bwd", "scratch", pc, nc, name, p, n)
+    if pd is not None:
+        _apart("rmsnorm_bwd", "dx", px, size, "dgamma", pd, small)
+        if pc is not None:
+            _apart("rmsnorm_bwd", "dx", px, size, "scratch", pc, nc)
+            _apart("rmsnorm_bwd", "dgamma", pd, small, "scratch", pc, nc)
+    stream = _launch_stream(dy, x, gamma, rstd, dx, dsum, dgamma, scratch if pc is not None else None)
+    _check(_nlib().ffk_rmsnorm_bwd(py, ph, pg, ps, pu, px, pd, pc, rows, cols, _DT[dy.dtype], 1 if accumulate_params else 0, stream),
            "ffk_rmsnorm_bwd")
 
 
@@ -904,7 +946,7 @@ class GradientList:
         if any(start < end for (_, end), (start, _) in zip(held, held[1:])):
             raise KernelError("GradientList: gradients or outputs that share memory")
         _cuda_contig(*self.tensors, *self.out)
-        self.check_device()
+        _launch_stream(*self.tensors, *self.out)
         piece = _nlib().ffk_grad_piece_elements()
         tables = []
         for t, o in zip(self.tensors, self.out):
@@ -921,15 +963,12 @@ class GradientList:
         self._partial = torch.empty(_nlib().ffk_grad_partials(), dtype=torch.float64, device=device)
         self.norm = torch.zeros(1, dtype=torch.float32, device=device)
 
-    def check_device(self):
-        _same_device(*self.tensors, *self.out)
-
 
 def gradient_norm(grads: GradientList):
     """The 2-norm of all gradients of the list taken as one vector: an fp32 device tensor of one element, the list's own, which the next
     call on the list overwrites.  The sum does not depend on the order in which blocks run."""
-    grads.check_device()
-    _check(_nlib().ffk_grad_norm(grads._table.data_ptr(), grads.pieces, grads._partial.data_ptr(), grads.norm.data_ptr(), grads.bytes, _stream()),
+    stream = _launch_stream(grads.norm)
+    _check(_nlib().ffk_grad_norm(grads._table.data_ptr(), grads.pieces, grads._partial.data_ptr(), grads.norm.data_ptr(), grads.bytes, stream),
            "ffk_grad_norm")
     return grads.norm
 
@@ -941,9 +980,9 @@ def clip_gradients(grads: GradientList, max_norm: float):
     max_norm = float(max_norm)
     if not 0.0 <= max_norm < float("inf"):
         raise KernelError("clip_gradients: max_norm is a finite number that is not negative")
-    grads.check_device()
+    stream = _launch_stream(grads.norm)
     _check(_nlib().ffk_grad_clip(grads._table.data_ptr(), grads.pieces, grads._partial.data_ptr(), max_norm, grads.norm.data_ptr(), 2 * grads.bytes,
-                                 _stream()), "ffk_grad_clip")
+                                 stream), "ffk_grad_clip")
     return grads.norm
 
 

@@ -122,3 +122,24 @@ def test_gradient_list_refuses():
     refused("share memory", lambda: K.GradientList([a[:6], a[5:]]))
     refused("share memory", lambda: K.GradientList([a, torch.zeros(10)], out=[torch.zeros(10), a]))
     refused("non-contiguous|CPU", lambda: K.GradientList([torch.zeros(4, 4).t()]))
+
+
+# ---------------------------------------------------------------------------------------------- devices
+class _On:
+    """Stands in for a tensor on a device of a machine with several."""
+
+    def __init__(self, device):
+        self.device_index = device
+
+    def get_device(self):
+        return self.device_index
+
+
+def test_operands_on_another_device_than_the_current_one(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(K, "_raw_stream", lambda device: 1000 + device)
+    assert K._launch_stream(_On(1), None, _On(1)) == 1001
+    refused("current device", lambda: K._launch_stream(_On(0), _On(0)))
+    refused("cuda:1 and on cuda:0", lambda: K._launch_stream(_On(1), None, _On(0)))
+    refused("CPU tensor", lambda: K._launch_stream(_On(1), _On(-1)))
+    refused("CPU tensor", lambda: K._launch_stream(_On(-1), _On(1)))
