@@ -17,9 +17,12 @@
 
 namespace {
 
-constexpr int PIECE = 16384;            // elements of a piece
+constexpr int PIECE = 16384;            // elements of a piece at most
+constexpr int PIECE_LEAST = 1024;
 constexpr int NORM_BLOCKS = 148 * 8;    // partial sums at most
 constexpr int NORM_THREADS = 256;
+constexpr int NORM_UNROLL = 8;          // 16-byte loads of a thread under way
+constexpr long long NORM_KEEP = 80ll << 20;   // bytes of the gradients that stay in L2 (126 MB) between the passes
 
 struct GradPiece {
   const void *src;
@@ -88,19 +91,19 @@ __device__ __forceinline__ double squares(const float (&v)[N]) {
 }
 
 template <typename T>
-__device__ __forceinline__ double piece_squares(const T *p, int n) {
+__device__ __forceinline__ double piece_squares(const T *p, int n, bool stream) {
   constexpr int N = GradVec<T>::N;
   double sum = 0.0;
   if ((((uintptr_t)p) & 15) == 0) {
     const int whole = n / N;
     const uint4 *q = reinterpret_cast<const uint4 *>(p);
     int i = threadIdx.x;
-    for (; i + 3 * NORM_THREADS < whole; i += 4 * NORM_THREADS) {
-      uint4 u[4];
+    for (; i + (NORM_UNROLL - 1) * NORM_THREADS < whole; i += NORM_UNROLL * NORM_THREADS) {
+      uint4 u[NORM_UNROLL];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = q[i + k * NORM_THREADS];
+      for (int k = 0; k < NORM_UNROLL; ++k) u[k] = stream ? __ldcs(q + i + k * NORM_THREADS) : q[i + k * NORM_THREADS];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < NORM_UNROLL; ++k) {
         float v[N];
         GradVec<T>::unpack(u[k], v);
         sum += squares(v);
@@ -138,15 +141,19 @@ __device__ __forceinline__ double block_sum_wide(double v, double *red) {
   return t;
 }
 
-__global__ void __launch_bounds__(NORM_THREADS) grad_squares_kernel(const GradPiece *pieces, int count, double *__restrict__ partial) {
+__global__ void __launch_bounds__(NORM_THREADS) grad_squares_kernel(const GradPiece *pieces, int count, int keep, double *__restrict__ partial) {
   pdl_entry();
   __shared__ double red[NORM_THREADS / 32];
   double sum = 0.0;
+  // the last `keep` pieces are left in L2 for the clipping, which begins with them; the others stream past it
+  GradPiece next = {};
+  if ((int)blockIdx.x < count) next = pieces[blockIdx.x];
   for (int c = blockIdx.x; c < count; c += gridDim.x) {
-    const GradPiece g = pieces[c];
-    if (g.dt == 1) sum += piece_squares((const bf16 *)g.src, g.n);
-    else if (g.dt == 0) sum += piece_squares((const float *)g.src, g.n);
-    else sum += piece_squares((const __half *)g.src, g.n);
+    const GradPiece g = next;
+    if (c + (int)gridDim.x < count) next = pieces[c + gridDim.x];      // the next entry comes in under this piece's loads
+    if (g.dt == 1) sum += piece_squares((const bf16 *)g.src, g.n, c < count - keep);
+    else if (g.dt == 0) sum += piece_squares((const float *)g.src, g.n, c < count - keep);
+    else sum += piece_squares((const __half *)g.src, g.n, c < count - keep);
   }
   sum = block_sum_wide(sum, red);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -183,12 +190,12 @@ __device__ __forceinline__ void piece_scale(const T *src, T *dst, int n, bool ov
     const uint4 *q = reinterpret_cast<const uint4 *>(src);
     uint4 *o = reinterpret_cast<uint4 *>(dst);
     int i = threadIdx.x;
-    for (; i + 3 * NORM_THREADS < whole; i += 4 * NORM_THREADS) {
-      uint4 u[4];
+    for (; i + (NORM_UNROLL - 1) * NORM_THREADS < whole; i += NORM_UNROLL * NORM_THREADS) {
+      uint4 u[NORM_UNROLL];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = q[i + k * NORM_THREADS];
+      for (int k = 0; k < NORM_UNROLL; ++k) u[k] = q[i + k * NORM_THREADS];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[i + k * NORM_THREADS] = scaled<T>(u[k], over, f);
+      for (int k = 0; k < NORM_UNROLL; ++k) o[i + k * NORM_THREADS] = scaled<T>(u[k], over, f);
     }
     for (; i < whole; i += NORM_THREADS) o[i] = scaled<T>(q[i], over, f);
     const int rest = whole * N + (int)threadIdx.x;
@@ -209,12 +216,15 @@ __global__ void __launch_bounds__(NORM_THREADS) grad_clip_kernel(const GradPiece
                                                                  float *__restrict__ norm) {
   pdl_entry();
   __shared__ double red[NORM_THREADS / 32];
+  GradPiece next = {};
+  if (count - 1 - (int)blockIdx.x >= 0) next = pieces[count - 1 - (int)blockIdx.x];
   const double n = folded_norm(partial, blocks, red);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
   const bool over = n > (double)max_norm && n <= 1.7e308;
   const float f = over ? (float)((double)max_norm / n) : 1.f;
   for (int c = count - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-    const GradPiece g = pieces[c];
+    const GradPiece g = next;
+    if (c - (int)gridDim.x >= 0) next = pieces[c - gridDim.x];
     if (!over && g.src == g.dst) continue;
     if (g.dt == 1) piece_scale((const bf16 *)g.src, (bf16 *)g.dst, g.n, over, f);
     else if (g.dt == 0) piece_scale((const float *)g.src, (float *)g.dst, g.n, over, f);
@@ -226,14 +236,18 @@ int norm_blocks(int count) { return count < 1 ? 1 : count < NORM_BLOCKS ? count 
 
 }  // namespace
 
-FFK_API int ffk_grad_piece_elements() { return PIECE; }
+// elements of a piece of a list of `total`: two pieces a block, where that leaves them long enough to be worth their table entry
+FFK_API int ffk_grad_piece_elements(long long total) {
+  const long long n = (total / (2 * NORM_BLOCKS) + PIECE_LEAST - 1) / PIECE_LEAST * PIECE_LEAST;
+  return (int)(n < PIECE_LEAST ? PIECE_LEAST : n > PIECE ? PIECE : n);
+}
 FFK_API int ffk_grad_partials() { return NORM_BLOCKS; }
 
 // pieces: `count` GradPiece in device memory; partial: ffk_grad_partials() doubles of scratch; norm: one float
 FFK_API int ffk_grad_norm(const void *pieces, int count, double *partial, float *norm, long long bytes, cudaStream_t st) {
   const int blocks = norm_blocks(count);
   FfkTraffic traffic(bytes);
-  int e = ffk_launch(grad_squares_kernel, blocks, NORM_THREADS, 0, st, (const GradPiece *)pieces, count, partial);
+  int e = ffk_launch(grad_squares_kernel, blocks, NORM_THREADS, 0, st, (const GradPiece *)pieces, count, 0, partial);
   traffic.done();
   if (e) return e;
   return ffk_launch(grad_norm_kernel, 1, NORM_THREADS, 0, st, partial, blocks, norm);
@@ -241,8 +255,9 @@ FFK_API int ffk_grad_norm(const void *pieces, int count, double *partial, float 
 
 FFK_API int ffk_grad_clip(const void *pieces, int count, double *partial, float max_norm, float *norm, long long bytes, cudaStream_t st) {
   const int blocks = norm_blocks(count);
-  FfkTraffic traffic(bytes);
-  int e = ffk_launch(grad_squares_kernel, blocks, NORM_THREADS, 0, st, (const GradPiece *)pieces, count, partial);
+  FfkTraffic traffic(2 * bytes);
+  const int keep = bytes <= NORM_KEEP ? count : (int)((double)NORM_KEEP / (double)bytes * count);
+  int e = ffk_launch(grad_squares_kernel, blocks, NORM_THREADS, 0, st, (const GradPiece *)pieces, count, keep, partial);
   if (e) return e;
   return ffk_launch(grad_clip_kernel, blocks, NORM_THREADS, 0, st, (const GradPiece *)pieces, count, partial, blocks, max_norm, norm);
 }

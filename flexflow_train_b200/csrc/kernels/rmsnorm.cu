@@ -7,10 +7,11 @@
 // y, dh and dgamma are rounded once, when they are stored.
 //
 // What bounds it: HBM.  A row is read once into registers and written once: forward 4, backward 4 row's worth of bytes.  A row belongs to
-// one warp (WARPS 1, shuffles only) or to a block of eight (WARPS 8, one exchange through shared memory); a thread holds N pieces
-// of V elements (16 bytes, or one element where the width or an address does not allow that).  Backward's blocks stay for many rows: a
-// thread keeps the columns it owns of dgamma in registers and the block leaves one partial row, which the fold adds in a fixed order.
-// Rows too wide for registers take the kernels at the end, which read a row twice.
+// WARPS warps (one exchange through shared memory among them; none for one warp), as many as give a thread one piece of V elements (16
+// bytes, or one element where the width or an address does not allow that), up to 16 warps (8 of single elements); wider rows give N pieces.  More pieces and fewer
+// warps cost registers and with them the loads under way: 32768 x 1024 backward 60 us with one warp and four pieces.  Backward's blocks stay
+// for many rows: a thread keeps the columns it owns of dgamma in registers and the block leaves one partial row, which the fold adds in a
+// fixed order.  Rows too wide for registers take the kernels at the end, which read a row twice.
 #include "common.cuh"
 
 namespace {
@@ -63,32 +64,34 @@ template <> struct Piece<bf16, 8> {
   __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
 };
 
-// sum over the warps that share a row; `red`: two sets of WARPS floats that successive rows use in turn
+// Sum over the WARPS warps that share a row (group `group` of the block).  `red`: two sets of WARPS floats per group, which successive rows use
+// in turn, so that one barrier a row is enough.
 template <int WARPS>
-__device__ __forceinline__ float row_sum(float v, float *red, int parity) {
+__device__ __forceinline__ float row_sum(float v, float *red, int group, int parity) {
   v = warp_sum(v);
   if constexpr (WARPS > 1) {
-    float *r = red + parity * WARPS;
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
-    __syncthreads();
+    float *r = red + (group * 2 + parity) * WARPS;
+    if ((threadIdx.x & 31) == 0) r[(threadIdx.x >> 5) % WARPS] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(WARPS * 32) : "memory");
     v = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) v += r[w];
   }
   return v;
 }
+__host__ __device__ constexpr int rms_threads(int warps) { return warps > 8 ? warps * 32 : 256; }      // of a block at most: several rows where they are narrow
 
 // a, r, xsum and y are read and written element by element by the same thread: y or xsum may be a or r
 template <typename T, int V, int N, int WARPS>
-__global__ void __launch_bounds__(256) rms_fwd_kernel(const T *a, const T *b, const T *gamma, T *xsum, T *y, float *__restrict__ rstd, int rows,
+__global__ void __launch_bounds__(rms_threads(WARPS)) rms_fwd_kernel(const T *a, const T *b, const T *gamma, T *xsum, T *y, float *__restrict__ rstd, int rows,
                                                       int cols, float eps) {
   pdl_entry(xsum, y);
-  __shared__ float red[2 * (WARPS > 1 ? WARPS : 1)];
-  const int slot = WARPS > 1 ? threadIdx.x : threadIdx.x & 31;
-  const int per_block = WARPS > 1 ? 1 : (int)(blockDim.x >> 5);
+  __shared__ float red[2 * rms_threads(WARPS) / 32];
+  const int slot = threadIdx.x % (WARPS * 32), group = threadIdx.x / (WARPS * 32);
+  const int per_block = blockDim.x / (WARPS * 32);
   const float inv = 1.f / (float)cols;
   int parity = 0;
-  for (long long row = (long long)blockIdx.x * per_block + (WARPS > 1 ? 0 : threadIdx.x >> 5); row < rows; row += (long long)gridDim.x * per_block) {
+  for (long long row = (long long)blockIdx.x * per_block + group; row < rows; row += (long long)gridDim.x * per_block) {
     const long long base = row * cols;
     Piece<T, V> pa[N], pb[N];
 #pragma unroll
@@ -116,7 +119,7 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(const T *a, const T *b, co
 #pragma unroll
       for (int j = 0; j < V; ++j) ss = fmaf(u[j], u[j], ss);
     }
-    ss = row_sum<WARPS>(ss, red, parity);
+    ss = row_sum<WARPS>(ss, red, group, parity);
     parity ^= 1;
     const float rs = rsqrtf(ss * inv + eps);
     if (slot == 0 && rstd) rstd[row] = rs;
@@ -141,14 +144,13 @@ __global__ void __launch_bounds__(256) rms_fwd_kernel(const T *a, const T *b, co
 
 // dh may be dy or dsum.  `partial`: [gridDim.x][cols]
 template <typename T, int V, int N, int WARPS>
-__global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, const T *gamma, const float *rstd, const T *dsum, T *dh,
+__global__ void __launch_bounds__(rms_threads(WARPS)) rms_bwd_kernel(const T *dy, const T *h, const T *gamma, const float *rstd, const T *dsum, T *dh,
                                                       float *__restrict__ partial, int rows, int cols) {
   pdl_entry(dh);
-  __shared__ float red[2 * (WARPS > 1 ? WARPS : 1)];
-  extern __shared__ float part[];            // WARPS 1: the block's sum of dgamma, [cols]
-  const int warp = threadIdx.x >> 5;
-  const int slot = WARPS > 1 ? threadIdx.x : threadIdx.x & 31;
-  const int per_block = WARPS > 1 ? 1 : (int)(blockDim.x >> 5);
+  __shared__ float red[2 * rms_threads(WARPS) / 32];
+  extern __shared__ float part[];            // several rows a block: its sum of dgamma, [cols]
+  constexpr int GROUPS = rms_threads(WARPS) / (WARPS * 32);
+  const int slot = threadIdx.x % (WARPS * 32), group = threadIdx.x / (WARPS * 32);
   const float inv = 1.f / (float)cols;
   float acc[N][V];
   Piece<T, V> pg[N];
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, c
     for (int j = 0; j < V; ++j) acc[i][j] = 0.f;
   }
   int parity = 0;
-  for (long long row = (long long)blockIdx.x * per_block + (WARPS > 1 ? 0 : warp); row < rows; row += (long long)gridDim.x * per_block) {
+  for (long long row = (long long)blockIdx.x * GROUPS + group; row < rows; row += (long long)gridDim.x * GROUPS) {
     const long long base = row * cols;
     Piece<T, V> py[N], ph[N], ps[N];
 #pragma unroll
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, c
       if (c < cols) {
         py[i].load(dy + base + c);
         ph[i].load(h + base + c);
-        if (N * V < 64 && dsum) ps[i].load(dsum + base + c);
+        if (N * V < 32 && dsum) ps[i].load(dsum + base + c);
       }
     }
     const float rs = rstd[row];
@@ -191,7 +193,7 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, c
         acc[i][j] = fmaf(yx, rs, acc[i][j]);
       }
     }
-    dot = row_sum<WARPS>(dot, red, parity);
+    dot = row_sum<WARPS>(dot, red, group, parity);
     parity ^= 1;
     const float k = dot * inv * rs * rs;
 #pragma unroll
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, c
         py[i].get(y);
         ph[i].get(x);
         pg[i].get(g);
-        if (N * V >= 64 && dsum) ps[i].load(dsum + base + c);      // the widest rows: the other three fill the registers
+        if (N * V >= 32 && dsum) ps[i].load(dsum + base + c);      // the widest rows: the other three fill the registers
         ps[i].get(s);
 #pragma unroll
         for (int j = 0; j < V; ++j) y[j] = fmaf(rs, fmaf(y[j], g[j], -x[j] * k), s[j]);
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, c
   }
   if (!partial) return;
   float *out = partial + (long long)blockIdx.x * cols;
-  if constexpr (WARPS > 1) {
+  if constexpr (GROUPS == 1) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = (i * WARPS * 32 + slot) * V;
@@ -223,12 +225,12 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, c
       }
     }
   } else {
-    // the warps add up their columns one after the other
-    for (int w = 0; w < per_block; ++w) {
-      if (warp == w) {
+    // the groups add up their columns one after the other
+    for (int w = 0; w < GROUPS; ++w) {
+      if (group == w) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int c = (i * 32 + slot) * V;
+          const int c = (i * WARPS * 32 + slot) * V;
           if (c < cols) {
 #pragma unroll
             for (int j = 0; j < V; ++j) part[c + j] = w == 0 ? acc[i][j] : part[c + j] + acc[i][j];
@@ -241,23 +243,56 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const T *dy, const T *h, c
   }
 }
 
-// dgamma (+)= column sums of the `parts` partial rows, in their order: 32 columns a block, 32 threads a column
-template <typename T>
+// dgamma (+)= column sums of the `parts` partial rows, in their order: 32 columns a block, 128 threads of four columns (or one, STEP 1) down the
+// rows, so that the loads of a thousand partial rows are under way at once (a thread per column: 12 us for 888 x 2048)
+template <typename T, int STEP>
 __global__ void __launch_bounds__(1024) rms_fold_kernel(const float *partial, int parts, int cols, T *dgamma, int accumulate) {
   pdl_entry(dgamma);
-  __shared__ float sum[32][33];
-  const int c = blockIdx.x * 32 + threadIdx.x;
-  float s = 0.f;
-  if (c < cols)
-    for (int p = threadIdx.y; p < parts; p += 32) s += partial[(long long)p * cols + c];
-  sum[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < cols) {
-    s = 0.f;
+  constexpr int LANES = 32 / STEP, DOWN = 1024 / LANES;
+  __shared__ float sum[DOWN][33];
+  const int x = threadIdx.x % LANES, y = threadIdx.x / LANES;
+  const int c = blockIdx.x * 32 + x * STEP;
+  float s[STEP];
 #pragma unroll
-    for (int p = 0; p < 32; ++p) s += sum[p][threadIdx.x];
-    if (accumulate) s += rms_ld(dgamma + c);
-    rms_st(dgamma + c, s);
+  for (int j = 0; j < STEP; ++j) s[j] = 0.f;
+  if (c < cols) {
+    const float *from = partial + c;
+    int p = y;
+    for (; p + 7 * DOWN < parts; p += 8 * DOWN) {
+      float v[8][STEP];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float *q = from + (long long)(p + k * DOWN) * cols;
+        if constexpr (STEP == 4) {
+          const float4 u = *reinterpret_cast<const float4 *>(q);
+          v[k][0] = u.x; v[k][1] = u.y; v[k][2] = u.z; v[k][3] = u.w;
+        } else {
+          v[k][0] = *q;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < STEP; ++j) s[j] += v[k][j];
+    }
+#pragma unroll 4
+    for (; p < parts; p += DOWN)
+#pragma unroll
+      for (int j = 0; j < STEP; ++j) s[j] += from[(long long)p * cols + j];
+  }
+#pragma unroll
+  for (int j = 0; j < STEP; ++j) sum[y][x * STEP + j] = s[j];
+  __syncthreads();
+  // a warp per column, its lanes down the rows
+  const int col = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float t = 0.f;
+#pragma unroll
+  for (int k = 0; k < DOWN / 32; ++k) t += sum[k * 32 + lane][col];
+  t = warp_sum(t);
+  const int out = blockIdx.x * 32 + col;
+  if (lane == 0 && out < cols) {
+    if (accumulate) t += rms_ld(dgamma + out);
+    rms_st(dgamma + out, t);
   }
 }
 
@@ -309,30 +344,37 @@ __global__ void __launch_bounds__(512) rms_bwd_wide_kernel(const T *dy, const T 
   }
 }
 
-// How a row is spread: warps (1 or 8) and pieces per thread (1, 2, 4, 8); pieces 0: too wide for registers
+// How a row is spread: elements of a piece, warps, pieces of a thread (0: too wide for registers)
 struct RmsForm { int v, warps, n; };
-RmsForm rms_form(int rows, int cols, int es, bool whole) {
+RmsForm rms_form(int cols, int es, bool whole) {
   const int v = whole && cols % (16 / es) == 0 ? 16 / es : 1;
   const int pieces = (cols + v * 32 - 1) / (v * 32);       // of a warp
-  RmsForm f = {v, 1, 0};
-  if (pieces > 64) return f;
-  if (pieces > 4) { f.warps = 8; }
-  const int need = f.warps == 8 ? (pieces + 7) / 8 : pieces;
-  f.n = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
-  (void)rows;
+  const int most_warps = v == 1 ? 8 : 16, most = v == 1 ? 8 : 4;       // single elements: fewer threads with more of them
+  RmsForm f = {v, 1, 1};
+  while (f.warps < most_warps && f.warps < pieces) f.warps *= 2;
+  while (f.n < most && f.warps * f.n < pieces) f.n *= 2;
+  if (f.warps * f.n < pieces) f.n = 0;
   return f;
 }
 int rms_fwd_grid(const RmsForm &f, int rows, int &threads) {
   if (f.n == 0) { threads = 512; return rows < 148 * 4 ? rows : 148 * 4; }
-  if (f.warps == 8) { threads = 256; return rows < 148 * 8 ? rows : 148 * 8; }
-  threads = rows >= 148 * 8 ? 256 : 64;
-  const int per = threads / 32, want = (rows + per - 1) / per;
+  // few rows: one a block, so that they spread over the SMs
+  threads = rows >= 148 * 8 ? rms_threads(f.warps) : f.warps * 32;
+  const int per = threads / (f.warps * 32), want = (rows + per - 1) / per;
   return want < 148 * 8 ? want : 148 * 8;
 }
-int rms_bwd_grid(const RmsForm &f, int rows) {
-  if (f.n == 0) return rows < 148 * 2 ? rows : 148 * 2;
-  const int want = f.warps == 8 ? rows : (rows + 7) / 8, most = 148 * 4;
+// backward's blocks stay for their rows: as many as are resident at once, at most RMS_BWD_PER_SM per SM
+constexpr int RMS_BWD_PER_SM = 8;
+int rms_bwd_grid(const RmsForm &f, int rows, int per_sm) {
+  if (per_sm > RMS_BWD_PER_SM) per_sm = RMS_BWD_PER_SM;
+  const int groups = f.n == 0 ? 1 : rms_threads(f.warps) / (f.warps * 32);
+  const int want = (rows + groups - 1) / groups, most = 148 * (per_sm < 1 ? 1 : per_sm);
   return want < most ? want : most;
+}
+template <typename K>
+int rms_resident(K kernel, int threads, size_t smem) {
+  int n = 0;
+  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess ? n : 1;
 }
 bool rms_aligned(const void *p) { return (((uintptr_t)p) & 15) == 0; }
 
@@ -344,21 +386,23 @@ int rms_fwd_run(const void *a, const void *b, const void *gamma, void *xsum, voi
 }
 template <typename T, int V, int N, int WARPS>
 int rms_bwd_run(const void *dy, const void *h, const void *gamma, const float *rstd, const void *dsum, void *dh, float *partial, int rows, int cols,
-                int grid, cudaStream_t st) {
-  return ffk_launch(rms_bwd_kernel<T, V, N, WARPS>, grid, 256, WARPS == 1 ? (size_t)cols * 4 : 0, st, (const T *)dy, (const T *)h, (const T *)gamma,
+                int &grid, cudaStream_t st) {
+  constexpr int threads = rms_threads(WARPS);
+  constexpr bool several = threads > WARPS * 32;
+  static const int per_sm = rms_resident(rms_bwd_kernel<T, V, N, WARPS>, threads, several ? (size_t)V * N * WARPS * 128 : 0);
+  grid = rms_bwd_grid({V, WARPS, N}, rows, per_sm);
+  return ffk_launch(rms_bwd_kernel<T, V, N, WARPS>, grid, threads, several ? (size_t)cols * 4 : 0, st, (const T *)dy, (const T *)h, (const T *)gamma,
                     rstd, (const T *)dsum, (T *)dh, partial, rows, cols);
 }
-#define RMS_FORMS(RUN, T, V, ...)                                                                              \
-  if (f.warps == 1) switch (f.n) {                                                                            \
-      case 1: return RUN<T, V, 1, 1>(__VA_ARGS__);                                                            \
-      case 2: return RUN<T, V, 2, 1>(__VA_ARGS__);                                                            \
-      default: return RUN<T, V, 4, 1>(__VA_ARGS__);                                                           \
-    }                                                                                                         \
-  switch (f.n) {                                                                                              \
-    case 1: return RUN<T, V, 1, 8>(__VA_ARGS__);                                                              \
-    case 2: return RUN<T, V, 2, 8>(__VA_ARGS__);                                                              \
-    case 4: return RUN<T, V, 4, 8>(__VA_ARGS__);                                                              \
-    default: return RUN<T, V, 8, 8>(__VA_ARGS__);                                                             \
+#define RMS_FORMS(RUN, T, V, ...)                            \
+  switch (f.warps * f.n) {                                  \
+    case 1: return RUN<T, V, 1, 1>(__VA_ARGS__);            \
+    case 2: return RUN<T, V, 1, 2>(__VA_ARGS__);            \
+    case 4: return RUN<T, V, 1, 4>(__VA_ARGS__);            \
+    case 8: return RUN<T, V, 1, 8>(__VA_ARGS__);            \
+    case 16: return RUN<T, V, V == 1 ? 2 : 1, V == 1 ? 8 : 16>(__VA_ARGS__); \
+    case 32: return RUN<T, V, V == 1 ? 4 : 2, V == 1 ? 8 : 16>(__VA_ARGS__); \
+    default: return RUN<T, V, V == 1 ? 8 : 4, V == 1 ? 8 : 16>(__VA_ARGS__); \
   }
 
 template <typename T, int WHOLE>
@@ -371,7 +415,8 @@ int rms_fwd_typed(const RmsForm &f, const void *a, const void *b, const void *ga
 }
 template <typename T, int WHOLE>
 int rms_bwd_typed(const RmsForm &f, const void *dy, const void *h, const void *gamma, const float *rstd, const void *dsum, void *dh, float *partial,
-                  int rows, int cols, int grid, cudaStream_t st) {
+                  int rows, int cols, int &grid, cudaStream_t st) {
+  if (f.n == 0) grid = rms_bwd_grid(f, rows, 2);
   if (f.n == 0)
     return ffk_launch(rms_bwd_wide_kernel<T>, grid, 512, 0, st, (const T *)dy, (const T *)h, (const T *)gamma, rstd, (const T *)dsum, (T *)dh, partial,
                       rows, cols);
@@ -389,7 +434,7 @@ FFK_API int ffk_rmsnorm_fwd(const void *a, const void *b, const void *gamma, voi
   if (cols <= 0) return -2;
   const int es = dt == 1 ? 2 : 4;
   FfkTraffic traffic((long long)rows * cols * es * (b ? xsum ? 4 : 3 : 2));
-  const RmsForm f = rms_form(rows, cols, es, rms_aligned(a) && rms_aligned(b) && rms_aligned(gamma) && rms_aligned(xsum) && rms_aligned(y));
+  const RmsForm f = rms_form(cols, es, rms_aligned(a) && rms_aligned(b) && rms_aligned(gamma) && rms_aligned(xsum) && rms_aligned(y));
   int threads = 0;
   const int grid = rms_fwd_grid(f, rows, threads);
   return dt == 1 ? rms_fwd_typed<bf16, 8>(f, a, b, gamma, xsum, y, rstd, rows, cols, eps, grid, threads, st)
@@ -402,7 +447,7 @@ FFK_API long long ffk_rmsnorm_bwd_scratch(int rows, int cols) {
   long long most = 0;
   for (int es = 2; es <= 4; es += 2)
     for (int whole = 0; whole < 2; ++whole) {
-      const long long g = rms_bwd_grid(rms_form(rows, cols, es, whole), rows);
+      const long long g = rms_bwd_grid(rms_form(cols, es, whole), rows, RMS_BWD_PER_SM);
       most = g > most ? g : most;
     }
   return most * cols;
@@ -418,15 +463,18 @@ FFK_API int ffk_rmsnorm_bwd(const void *dy, const void *h, const void *gamma, co
   if (dgamma && rows > 0 && !partial) return -2;
   if (rows > 0) {
     FfkTraffic traffic((long long)rows * cols * es * (dsum ? 4 : 3));
-    const RmsForm f = rms_form(rows, cols, es, rms_aligned(dy) && rms_aligned(h) && rms_aligned(gamma) && rms_aligned(dsum) && rms_aligned(dh));
-    grid = rms_bwd_grid(f, rows);
+    const RmsForm f = rms_form(cols, es, rms_aligned(dy) && rms_aligned(h) && rms_aligned(gamma) && rms_aligned(dsum) && rms_aligned(dh));
     float *part = dgamma ? partial : nullptr;
     const int e = dt == 1 ? rms_bwd_typed<bf16, 8>(f, dy, h, gamma, rstd, dsum, dh, part, rows, cols, grid, st)
                           : rms_bwd_typed<float, 4>(f, dy, h, gamma, rstd, dsum, dh, part, rows, cols, grid, st);
     if (e) return e;
   }
   if (!dgamma) return 0;
-  const dim3 block(32, 32);
-  if (dt == 1) return ffk_launch(rms_fold_kernel<bf16>, (cols + 31) / 32, block, 0, st, partial, grid, cols, (bf16 *)dgamma, accumulate_params);
-  return ffk_launch(rms_fold_kernel<float>, (cols + 31) / 32, block, 0, st, partial, grid, cols, (float *)dgamma, accumulate_params);
+  const bool four = cols % 4 == 0 && rms_aligned(partial);
+  const unsigned blocks = (unsigned)(cols + 31) / 32;
+  if (dt == 1)
+    return four ? ffk_launch(rms_fold_kernel<bf16, 4>, blocks, 1024, 0, st, partial, grid, cols, (bf16 *)dgamma, accumulate_params)
+                : ffk_launch(rms_fold_kernel<bf16, 1>, blocks, 1024, 0, st, partial, grid, cols, (bf16 *)dgamma, accumulate_params);
+  return four ? ffk_launch(rms_fold_kernel<float, 4>, blocks, 1024, 0, st, partial, grid, cols, (float *)dgamma, accumulate_params)
+              : ffk_launch(rms_fold_kernel<float, 1>, blocks, 1024, 0, st, partial, grid, cols, (float *)dgamma, accumulate_params);
 }

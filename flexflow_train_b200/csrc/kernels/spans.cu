@@ -17,33 +17,47 @@ constexpr int SPAN_THREADS = 256;
 constexpr int SPAN_PER = 4;
 constexpr int SEG = SPAN_THREADS * SPAN_PER;
 
-// The largest i < `from` with test(i), or `none`: the block looks at blockDim.x places at a time, going down.  All threads get it.
+// The largest i < `from` with test(i), or `none`: the block looks at LOOK places at a time, going down; all threads get it.  Its loads do not
+// depend on one another, so a run of thousands of tokens costs a few latencies.
+constexpr int LOOK_PER = 8;
+constexpr int LOOK = SPAN_THREADS * LOOK_PER;
 template <typename F>
-__device__ __forceinline__ int block_find_down(int from, int none, int *slot, F test) {
-  for (int hi = from; hi > 0; hi -= SPAN_THREADS) {
-    const int i = hi - 1 - (int)threadIdx.x;
-    const bool hit = i >= 0 && test(i);
+__device__ __forceinline__ int block_find_down(int from, int none, int *slots, F test) {
+  for (int hi = from; hi > 0; hi -= LOOK) {
+    int best = -1;
+#pragma unroll
+    for (int k = 0; k < LOOK_PER; ++k) {
+      const int i = hi - 1 - k * SPAN_THREADS - (int)threadIdx.x;
+      best = max(best, test(max(i, 0)) ? i : -1);                  // no branch around the loads: they all start at once
+    }
+    best = __reduce_max_sync(0xffffffffu, best);
     __syncthreads();
-    if (threadIdx.x == 0) *slot = -1;
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = best;
     __syncthreads();
-    if (hit) atomicMax(slot, i);
-    __syncthreads();
-    if (*slot >= 0) return *slot;
+#pragma unroll
+    for (int w = 0; w < SPAN_THREADS / 32; ++w) best = max(best, slots[w]);
+    if (best >= 0) return best;
   }
   return none;
 }
 // The smallest i >= `from` (and < n) with test(i), or n.
 template <typename F>
-__device__ __forceinline__ int block_find_up(int from, int n, int *slot, F test) {
-  for (int lo = from; lo < n; lo += SPAN_THREADS) {
-    const int i = lo + (int)threadIdx.x;
-    const bool hit = i < n && test(i);
+__device__ __forceinline__ int block_find_up(int from, int n, int *slots, F test) {
+  for (int lo = from; lo < n; lo += LOOK) {
+    int best = n;
+#pragma unroll
+    for (int k = 0; k < LOOK_PER; ++k) {
+      const int i = lo + k * SPAN_THREADS + (int)threadIdx.x;
+      const bool hit = test(min(i, n - 1));
+      if (hit & (i < n)) best = min(best, i);
+    }
+    best = __reduce_min_sync(0xffffffffu, best);
     __syncthreads();
-    if (threadIdx.x == 0) *slot = n;
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = best;
     __syncthreads();
-    if (hit) atomicMin(slot, i);
-    __syncthreads();
-    if (*slot < n) return *slot;
+#pragma unroll
+    for (int w = 0; w < SPAN_THREADS / 32; ++w) best = min(best, slots[w]);
+    if (best < n) return best;
   }
   return n;
 }
@@ -53,7 +67,7 @@ __global__ void __launch_bounds__(SPAN_THREADS) attention_spans_kernel(const int
   pdl_entry();
   __shared__ int scan[SPAN_THREADS / 32];
   __shared__ int stops[SEG];
-  __shared__ int slot;
+  __shared__ int slot[SPAN_THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long row = blockIdx.x / segments;
   const int s0 = (int)(blockIdx.x % segments) * SEG;
@@ -61,7 +75,7 @@ __global__ void __launch_bounds__(SPAN_THREADS) attention_spans_kernel(const int
   const int *doc = documents + row * S;
   const unsigned char *flag = prompt ? prompt + row * S : nullptr;
   const bool flags = causal && flag;
-  auto opens = [&](int i) { return i == 0 || doc[i] != doc[i - 1]; };          // i begins a run
+  auto opens = [&](int i) { return (doc[i] != doc[max(i - 1, 0)]) | (i == 0); };   // i begins a run
   auto ends_prompt = [&](int i) { return flag[i] == 0; };
 
   // four consecutive tokens a thread
@@ -93,7 +107,7 @@ __global__ void __launch_bounds__(SPAN_THREADS) attention_spans_kernel(const int
   if (lane == 0) before = -1;
   __syncthreads();
   for (int w = 0; w < warp; ++w) before = max(before, scan[w]);
-  const int first = opens(s0) ? s0 : block_find_down(s0, 0, &slot, opens);      // start of the run that s0 belongs to
+  const int first = opens(s0) ? s0 : block_find_down(s0, 0, slot, opens);      // start of the run that s0 belongs to
   int low[SPAN_PER];
   int run = max(before, first);
 #pragma unroll
@@ -131,8 +145,8 @@ __global__ void __launch_bounds__(SPAN_THREADS) attention_spans_kernel(const int
     // the first such place behind the segment: the run of its last token may go on there
     int beyond;
     if (s1 >= S || opens(s1)) beyond = flags ? s1 : s1 - 1;
-    else if (flags) beyond = block_find_up(s1, S, &slot, [&](int i) { return opens(i) || ends_prompt(i); });
-    else beyond = block_find_up(s1, S, &slot, opens) - 1;
+    else if (flags) beyond = block_find_up(s1, S, slot, [&](int i) { return opens(i) | ends_prompt(i); });
+    else beyond = block_find_up(s1, S, slot, opens) - 1;
     run = min(after, beyond);
     int back[SPAN_PER];
 #pragma unroll
@@ -145,7 +159,7 @@ __global__ void __launch_bounds__(SPAN_THREADS) attention_spans_kernel(const int
 #pragma unroll
       for (int j = 0; j < SPAN_PER; ++j) stops[tid * SPAN_PER + j] = back[j];
       int came = first;
-      if (first < s0) came = block_find_up(first, s1, &slot, [&](int i) { return (i > first && opens(i)) || ends_prompt(i); });
+      if (first < s0) came = block_find_up(first, s1, slot, [&](int i) { return (opens(i) & (i > first)) | ends_prompt(i); });
       if (first < s0 && came == s1) came = beyond;       // flagged throughout: as far as it goes behind the segment
       __syncthreads();
 #pragma unroll
@@ -171,7 +185,7 @@ FFK_API int ffk_attention_spans(const int *documents, const unsigned char *promp
   if (B <= 0 || S <= 0) return 0;
   if (((uintptr_t)spans) & 7) return -2;
   const long long segments = ((long long)S + SEG - 1) / SEG, grid = segments * B;
-  if (grid > 0x7fffffffll || (long long)S > 0x7fffffffll - SEG) return -2;
+  if (grid > 0x7fffffffll || (long long)S > 0x7fffffffll - LOOK - SEG) return -2;
   FfkTraffic traffic((long long)B * S * 12);
   return ffk_launch(attention_spans_kernel, (unsigned)grid, SPAN_THREADS, 0, st, documents, prompt, (int2 *)spans, S, (int)segments, causal);
 }

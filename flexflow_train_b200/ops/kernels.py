@@ -784,7 +784,7 @@ def _new_ops_decl(l):
         "ffk_span_attention_bwd": ([ctypes.POINTER(SpanAttnDesc), S], c_int),
         "ffk_span_attention_bwd_scratch_floats": ([I, I, I], c_longlong),
         "ffk_span_attention_last_error": ([], c_int),
-        "ffk_grad_piece_elements": ([], c_int),
+        "ffk_grad_piece_elements": ([L], c_int),
         "ffk_grad_partials": ([], c_int),
         "ffk_grad_norm": ([P, I, P, P, L, S], c_int),
         "ffk_grad_clip": ([P, I, P, F, P, L, S], c_int),
@@ -947,7 +947,7 @@ class GradientList:
             raise KernelError("GradientList: gradients or outputs that share memory")
         _cuda_contig(*self.tensors, *self.out)
         _launch_stream(*self.tensors, *self.out)
-        piece = _nlib().ffk_grad_piece_elements()
+        piece = _nlib().ffk_grad_piece_elements(sum(t.numel() for t in self.tensors))
         tables = []
         for t, o in zip(self.tensors, self.out):
             es, n = t.element_size(), t.numel()
@@ -981,7 +981,7 @@ def clip_gradients(grads: GradientList, max_norm: float):
     if not 0.0 <= max_norm < float("inf"):
         raise KernelError("clip_gradients: max_norm is a finite number that is not negative")
     stream = _launch_stream(grads.norm)
-    _check(_nlib().ffk_grad_clip(grads._table.data_ptr(), grads.pieces, grads._partial.data_ptr(), max_norm, grads.norm.data_ptr(), 2 * grads.bytes,
+    _check(_nlib().ffk_grad_clip(grads._table.data_ptr(), grads.pieces, grads._partial.data_ptr(), max_norm, grads.norm.data_ptr(), grads.bytes,
                                  stream), "ffk_grad_clip")
     return grads.norm
 
