@@ -16,12 +16,21 @@ template <typename G> __device__ __forceinline__ float ldg(const G *p, long long
 template <> __device__ __forceinline__ float ldg<float>(const float *p, long long i) { return p[i]; }
 template <> __device__ __forceinline__ float ldg<bf16>(const bf16 *p, long long i) { return bf2f(p[i]); }
 
+// Factor on the gradients that keeps their norm at most max_norm (gradient_norm's result, read on the device): 1 where there is no
+// norm, where it is small enough, and where it is not finite.
+__device__ __forceinline__ float clip_factor(const float *norm, float max_norm) {
+  if (!norm) return 1.f;
+  const float n = *norm;
+  return n > max_norm && n <= 3.402823466e38f ? max_norm / n : 1.f;
+}
+
 template <typename G>
 __global__ void adam_kernel(float *__restrict__ w, float *__restrict__ m, float *__restrict__ v,
                             const G *g, bf16 *__restrict__ shadow, long long n, float alpha_t,
                             float beta1, float beta2, float eps, float wd, float gscale,
-                            const float *alpha_ptr) {
+                            const float *alpha_ptr, const float *norm, float max_norm) {
   pdl_entry(w, m, v);
+  gscale *= clip_factor(norm, max_norm);
   // alpha_ptr (optional): bias-corrected step size kept in device memory so that a captured CUDA graph
   // sees the value of the current step.
   if (alpha_ptr) alpha_t = *alpha_ptr;
@@ -87,8 +96,9 @@ __device__ __forceinline__ float sgd_step(float wk, float gk, float *mom, float 
 template <typename G>
 __global__ void __launch_bounds__(256) sgd_kernel(float *__restrict__ w, float *__restrict__ mom, const G *g,
                                                   bf16 *__restrict__ shadow, long long n, float lr, float momentum, int nesterov, float wd,
-                                                  float gscale) {
+                                                  float gscale, const float *norm, float max_norm) {
   pdl_entry(w, mom);
+  gscale *= clip_factor(norm, max_norm);
   // groups of four where the arenas' addresses allow it (a slice may start anywhere)
   const bool vec = (((uintptr_t)w | (uintptr_t)(momentum > 0.f ? mom : w)) & 15) == 0 && ((uintptr_t)g & (4 * sizeof(G) - 1)) == 0 &&
                    ((uintptr_t)shadow & 7) == 0;
@@ -281,29 +291,40 @@ __global__ void embedding_sgd_kernel(const I *idx, const O *dout, float *__restr
 
 }  // namespace
 
-// grad_dt: 0 = fp32, 1 = bf16.  shadow may be null.
-FFK_API int ffk_adam_update(float *w, float *m, float *v, const void *g, void *shadow, long long n, float alpha_t,
-                            float beta1, float beta2, float eps, float wd, float gscale, const float *alpha_ptr,
-                            int grad_dt, cudaStream_t st) {
+// grad_dt: 0 = fp32, 1 = bf16.  shadow may be null.  norm (may be null): the gradients' norm in device memory, clipped to max_norm.
+FFK_API int ffk_adam_update_clipped(float *w, float *m, float *v, const void *g, void *shadow, long long n, float alpha_t, float beta1, float beta2,
+                                    float eps, float wd, float gscale, const float *alpha_ptr, const float *norm, float max_norm, int grad_dt,
+                                    cudaStream_t st) {
   if (n <= 0) return 0;
   FfkTraffic traffic(n * 28);
   int grid = ffk_blocks(n / 4 + 1, 256, 148 * 8);
   if (grad_dt == 1)
-    ffk_launch(adam_kernel<bf16>, grid, 256, 0, st, w, m, v, (const bf16 *)g, (bf16 *)shadow, n, alpha_t, beta1, beta2, eps, wd, gscale, alpha_ptr);
+    ffk_launch(adam_kernel<bf16>, grid, 256, 0, st, w, m, v, (const bf16 *)g, (bf16 *)shadow, n, alpha_t, beta1, beta2, eps, wd, gscale, alpha_ptr,
+               norm, max_norm);
   else
-    ffk_launch(adam_kernel<float>, grid, 256, 0, st, w, m, v, (const float *)g, (bf16 *)shadow, n, alpha_t, beta1, beta2, eps, wd, gscale, alpha_ptr);
+    ffk_launch(adam_kernel<float>, grid, 256, 0, st, w, m, v, (const float *)g, (bf16 *)shadow, n, alpha_t, beta1, beta2, eps, wd, gscale, alpha_ptr,
+               norm, max_norm);
   return (int)cudaGetLastError();
 }
-FFK_API int ffk_sgd_update(float *w, float *mom, const void *g, void *shadow, long long n, float lr, float momentum,
-                           int nesterov, float wd, float gscale, int grad_dt, cudaStream_t st) {
+FFK_API int ffk_adam_update(float *w, float *m, float *v, const void *g, void *shadow, long long n, float alpha_t,
+                            float beta1, float beta2, float eps, float wd, float gscale, const float *alpha_ptr,
+                            int grad_dt, cudaStream_t st) {
+  return ffk_adam_update_clipped(w, m, v, g, shadow, n, alpha_t, beta1, beta2, eps, wd, gscale, alpha_ptr, nullptr, 0.f, grad_dt, st);
+}
+FFK_API int ffk_sgd_update_clipped(float *w, float *mom, const void *g, void *shadow, long long n, float lr, float momentum, int nesterov, float wd,
+                                   float gscale, const float *norm, float max_norm, int grad_dt, cudaStream_t st) {
   if (n <= 0) return 0;
   FfkTraffic traffic(n * 20);
   int grid = ffk_blocks(n / 4 + 1, 256, 148 * 8);
   if (grad_dt == 1)
-    ffk_launch(sgd_kernel<bf16>, grid, 256, 0, st, w, mom, (const bf16 *)g, (bf16 *)shadow, n, lr, momentum, nesterov, wd, gscale);
+    ffk_launch(sgd_kernel<bf16>, grid, 256, 0, st, w, mom, (const bf16 *)g, (bf16 *)shadow, n, lr, momentum, nesterov, wd, gscale, norm, max_norm);
   else
-    ffk_launch(sgd_kernel<float>, grid, 256, 0, st, w, mom, (const float *)g, (bf16 *)shadow, n, lr, momentum, nesterov, wd, gscale);
+    ffk_launch(sgd_kernel<float>, grid, 256, 0, st, w, mom, (const float *)g, (bf16 *)shadow, n, lr, momentum, nesterov, wd, gscale, norm, max_norm);
   return (int)cudaGetLastError();
+}
+FFK_API int ffk_sgd_update(float *w, float *mom, const void *g, void *shadow, long long n, float lr, float momentum,
+                           int nesterov, float wd, float gscale, int grad_dt, cudaStream_t st) {
+  return ffk_sgd_update_clipped(w, mom, g, shadow, n, lr, momentum, nesterov, wd, gscale, nullptr, 0.f, grad_dt, st);
 }
 
 template <typename W, typename I, typename O>

@@ -127,16 +127,22 @@ def _init(i):
 
 
 class SGDOptimizer:
-    def __init__(self, ffmodel=None, lr=0.01, momentum=0.0, nesterov=False, weight_decay=0.0):
-        self.config = OptimizerConfig(kind="sgd", lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay)
+    """max_grad_norm: the gradients' norm over all parameters is clipped to it before the step (0: not clipped)."""
+
+    def __init__(self, ffmodel=None, lr=0.01, momentum=0.0, nesterov=False, weight_decay=0.0, max_grad_norm=0.0):
+        self.config = OptimizerConfig(kind="sgd", lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      max_grad_norm=max_grad_norm)
 
     def set_learning_rate(self, learning_rate):
         self.config.lr = learning_rate
 
 
 class AdamOptimizer:
-    def __init__(self, ffmodel=None, alpha=0.001, beta1=0.9, beta2=0.999, weight_decay=0.0, epsilon=1e-8):
-        self.config = OptimizerConfig(kind="adam", lr=alpha, beta1=beta1, beta2=beta2, weight_decay=weight_decay, epsilon=epsilon)
+    """max_grad_norm as in `SGDOptimizer`."""
+
+    def __init__(self, ffmodel=None, alpha=0.001, beta1=0.9, beta2=0.999, weight_decay=0.0, epsilon=1e-8, max_grad_norm=0.0):
+        self.config = OptimizerConfig(kind="adam", lr=alpha, beta1=beta1, beta2=beta2, weight_decay=weight_decay, epsilon=epsilon,
+                                      max_grad_norm=max_grad_norm)
 
     def set_learning_rate(self, learning_rate):
         self.config.lr = learning_rate

@@ -784,6 +784,8 @@ def _new_ops_decl(l):
         "ffk_span_attention_bwd": ([ctypes.POINTER(SpanAttnDesc), S], c_int),
         "ffk_span_attention_bwd_scratch_floats": ([I, I, I], c_longlong),
         "ffk_span_attention_last_error": ([], c_int),
+        "ffk_adam_update_clipped": ([P, P, P, P, P, L, F, F, F, F, F, F, P, P, F, I, S], c_int),
+        "ffk_sgd_update_clipped": ([P, P, P, P, L, F, F, I, F, F, P, F, I, S], c_int),
         "ffk_grad_piece_elements": ([L], c_int),
         "ffk_grad_partials": ([], c_int),
         "ffk_grad_norm": ([P, I, P, P, L, S], c_int),
@@ -987,16 +989,36 @@ def clip_gradients(grads: GradientList, max_norm: float):
 
 
 # --------------------------------------------------------------------------- optimizers / embedding
-def adam_update(w, m, v, g, shadow, alpha_t, beta1, beta2, eps, weight_decay=0.0, grad_scale=1.0, alpha_tensor=None):
-    """One Adam step over an arena; alpha_tensor (1-element fp32 device tensor) overrides alpha_t when given."""
+def adam_update(w, m, v, g, shadow, alpha_t, beta1, beta2, eps, weight_decay=0.0, grad_scale=1.0, alpha_tensor=None, grad_norm=None,
+                max_grad_norm=0.0):
+    """One Adam step over an arena; alpha_tensor (1-element fp32 device tensor) overrides alpha_t when given.  grad_norm (1-element fp32
+    device tensor, see `gradient_norm`): the gradients are clipped to max_grad_norm as they are read."""
     _cuda_contig(w, m, v, g, shadow, alpha_tensor)
+    if grad_norm is not None:
+        _clip_check(grad_norm, max_grad_norm)
+        _check(_nlib().ffk_adam_update_clipped(w.data_ptr(), m.data_ptr(), v.data_ptr(), g.data_ptr(), _p(shadow), w.numel(), alpha_t, beta1, beta2,
+                                               eps, weight_decay, grad_scale, _p(alpha_tensor), grad_norm.data_ptr(), max_grad_norm, _dt(g),
+                                               _stream()), "ffk_adam_update_clipped")
+        return
     _check(lib().ffk_adam_update(w.data_ptr(), m.data_ptr(), v.data_ptr(), g.data_ptr(), _p(shadow), w.numel(),
                                  alpha_t, beta1, beta2, eps, weight_decay, grad_scale, _p(alpha_tensor), _dt(g),
                                  _stream()), "ffk_adam_update")
 
 
-def sgd_update(w, mom, g, shadow, lr, momentum=0.0, nesterov=False, weight_decay=0.0, grad_scale=1.0):
+def _clip_check(grad_norm, max_grad_norm):
+    if grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or not 0.0 <= max_grad_norm < float("inf"):
+        raise KernelError("grad_norm is a 1-element fp32 tensor, max_grad_norm a finite number that is not negative")
+    _cuda_contig(grad_norm)
+
+
+def sgd_update(w, mom, g, shadow, lr, momentum=0.0, nesterov=False, weight_decay=0.0, grad_scale=1.0, grad_norm=None, max_grad_norm=0.0):
+    """One SGD step over an arena; grad_norm / max_grad_norm as in `adam_update`."""
     _cuda_contig(w, mom, g, shadow)
+    if grad_norm is not None:
+        _clip_check(grad_norm, max_grad_norm)
+        _check(_nlib().ffk_sgd_update_clipped(w.data_ptr(), _p(mom), g.data_ptr(), _p(shadow), w.numel(), lr, momentum, int(nesterov), weight_decay,
+                                              grad_scale, grad_norm.data_ptr(), max_grad_norm, _dt(g), _stream()), "ffk_sgd_update_clipped")
+        return
     _check(lib().ffk_sgd_update(w.data_ptr(), _p(mom), g.data_ptr(), _p(shadow), w.numel(), lr, momentum,
                                 int(nesterov), weight_decay, grad_scale, _dt(g), _stream()), "ffk_sgd_update")
 

@@ -372,6 +372,9 @@ class FuseOut:
 class DistExecutable(Executable):
     def __init__(self, pcg, cfg: Optional[ExecConfig], ctx: DistContext, bucket_mb: int = 128, overlap: bool = True,
                  fuse_collectives: bool = True, fuse_optimizer: bool = True, shard_inputs: bool = False):
+        if cfg is not None and cfg.optimizer.max_grad_norm > 0:
+            # the buckets' kernels apply the optimizer while backward still runs: the norm over all of them is not known then
+            raise NotImplementedError("max_grad_norm: gradients are clipped on one device only")
         self.ctx = ctx
         self.shard_inputs = shard_inputs
         self.direct_inputs: Dict[str, "RepartitionOp"] = {}

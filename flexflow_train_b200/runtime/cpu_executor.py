@@ -10,6 +10,7 @@ Update rules (lib/kernels/src/cuda/optimizer_kernels.cu:11-31, 177-203):
   SGD:  g' = g + wd*w;  v = momentum*v + g';  g'' = nesterov ? g' + momentum*v : v;  w -= lr*g''
   Adam: g' = g + wd*w;  m = b1*m + (1-b1)*g';  v = b2*v + (1-b2)*g'^2;  w -= alpha_t * m / (sqrt(v) + eps)
         with alpha_t = lr * sqrt(1 - b2^t) / (1 - b1^t)
+With ``max_grad_norm`` the gradients g are first scaled by min(1, max_grad_norm / norm of all of them).
 """
 from __future__ import annotations
 
@@ -39,6 +40,9 @@ class CpuExecutable:
         self._m = {k: torch.zeros_like(p) for k, p in self.oracle.params.items()}
         self._v = {k: torch.zeros_like(p) for k, p in self.oracle.params.items()}
         self.launches_per_step = 0
+        self.grad_norm = None
+        if not 0.0 <= self.cfg.optimizer.max_grad_norm < math.inf:
+            raise ValueError(f"max_grad_norm {self.cfg.optimizer.max_grad_norm} is not a finite number >= 0")
 
     # ---- step pieces (the legacy API drives them one by one)
     def set_inputs(self, inputs: Dict[str, torch.Tensor], labels: Optional[torch.Tensor] = None):
@@ -68,10 +72,16 @@ class CpuExecutable:
         self.step_count += 1
         t = self.step_count
         with torch.no_grad():
+            scale = 1.0
+            if o.max_grad_norm > 0:
+                squares = [p.grad.double().square().sum() for p in self.oracle.params.values() if p.grad is not None]
+                self.grad_norm = torch.stack(squares).sum().sqrt().float().reshape(1) if squares else torch.zeros(1)
+                if o.max_grad_norm < float(self.grad_norm) < math.inf:
+                    scale = o.max_grad_norm / float(self.grad_norm)
             for k, p in self.oracle.params.items():
                 if p.grad is None:
                     continue
-                g = p.grad + o.weight_decay * p
+                g = scale * p.grad + o.weight_decay * p
                 if o.kind == "adam":
                     m, v = self._m[k], self._v[k]
                     m.mul_(o.beta1).add_(g, alpha=1 - o.beta1)

@@ -45,6 +45,9 @@ class OptimizerConfig:
     beta1: float = 0.9
     beta2: float = 0.999
     epsilon: float = 1e-8
+    # Gradients are scaled by min(1, max_grad_norm / their norm) before the step, the norm taken over all parameters; 0: not clipped.
+    # The norm of the last step is `Executable.grad_norm`.
+    max_grad_norm: float = 0.0
 
 
 @dataclass
@@ -1224,7 +1227,7 @@ class Executable:
         """Weights that are the table of exactly one Embedding and can take the sparse SGD update."""
         o = self.cfg.optimizer
         if not (self.cfg.training and self.cfg.sparse_embedding_update and o.kind == "sgd" and o.momentum == 0
-                and o.weight_decay == 0):
+                and o.weight_decay == 0 and o.max_grad_norm == 0):   # a row updated in backward is updated before the norm is known
             return []
         out = []
         for nid in self.order:
@@ -1267,6 +1270,12 @@ class Executable:
             self.opt_m = self.allocator.allocate([max(total, 1)], torch.float32).zero_() \
                 if (self.cfg.optimizer.kind == "adam" or self.cfg.optimizer.momentum > 0) else None
             self.opt_v = self.allocator.allocate([max(total, 1)], torch.float32).zero_() if self.cfg.optimizer.kind == "adam" else None
+        clip = self.cfg.optimizer.max_grad_norm
+        if not 0.0 <= clip < math.inf:
+            raise ValueError(f"max_grad_norm {clip} is not a finite number >= 0")
+        # the arena's padding between parameters holds zeros: the arena is the gradients' vector
+        self.grad_list = K.GradientList([self.grads]) if self.cfg.training and self.on_gpu and clip > 0 else None
+        self.grad_norm = self.grad_list.norm if self.grad_list is not None else None
         for i, nid in enumerate(self.param_nodes):
             o, n = offs[nid]
             shape = self.local_weight_shape(nid)
@@ -1666,12 +1675,13 @@ class Executable:
             return
         sl = slice(start, None)
         shadow = self.shadow[sl] if self.shadow is not None else None
+        norm = K.gradient_norm(self.grad_list) if self.grad_list is not None else None
         if o.kind == "adam":
             K.adam_update(self.master[sl], self.opt_m[sl], self.opt_v[sl], self.grads[sl], shadow, 0.0, o.beta1, o.beta2, o.epsilon,
-                          o.weight_decay, 1.0, alpha_tensor=self.alpha_tensor)
+                          o.weight_decay, 1.0, alpha_tensor=self.alpha_tensor, grad_norm=norm, max_grad_norm=o.max_grad_norm)
         else:
             K.sgd_update(self.master[sl], self.opt_m[sl] if self.opt_m is not None else None, self.grads[sl], shadow, o.lr, o.momentum,
-                         o.nesterov, o.weight_decay)
+                         o.nesterov, o.weight_decay, grad_norm=norm, max_grad_norm=o.max_grad_norm)
 
     def _step_scalars(self):
         """Per-step scalars that a captured graph reads from device memory: (step size, its tensor, dropout seed, its tensor)."""
