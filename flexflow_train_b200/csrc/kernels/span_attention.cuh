@@ -39,7 +39,7 @@ struct SpanArgs {
   int B, H, KH, S, D;
   const int2 *spans;
   const float *slopes;
-  float scale, factor;             // factor = scale * log2(e): a score in log-2 units is factor * y, see sa_scores
+  float scale, factor;             // factor = scale * log2(e): a score in log-2 units is factor * y, see sa_cap
   float to_z, from_z;              // with a cap: scale / cap and cap / scale
   float lim2, lim4;                // |raw score| up to which tanh is a polynomial of degree 2 or 4 in its square; negative: nowhere
   float t2[3], t4[5];              // the polynomials' coefficients, for raw scores
@@ -98,58 +98,63 @@ __device__ __forceinline__ float sa_tanh_any(float z) { return 1.f - __fdividef(
 //   y = s, with a cap tanh(a s) / a (a = scale / cap), with a bias less slope / scale * |distance|.
 // The special-function unit has its hands full with the exponentials (8 cycles a warp instruction), and the FMA pipe takes one element a
 // cycle whether packed or not, so tanh(a s) / a = s T((a s)^2) is a polynomial as short as the warp's largest |s| allows: degree 2 up to |a s| =
-// 1/4, degree 4 up to 5/8 (least squares on the relative error: 4e-7 and 1.1e-7), the exponential form beyond.  `count`: whether the row has a
-// say in that (one that sees nothing may hold anything).  d0: position of the first column less the row's, side: -1 / 1 where no column of
-// the warp lies right / left of its row, 0 otherwise.  All lanes of the warp.
-template <bool CAP, bool BIAS, int N>
-__device__ __forceinline__ void sa_scores(uint32_t (&x)[N], const SpanArgs &p, bool count, float slope, float d0, int side) {
-  if constexpr (CAP) {
-    float most[2] = {0.f, 0.f};
+// 1/4, degree 4 up to 5/8 (least squares on the relative error: 4e-7 and 1.1e-7), the exponential form beyond.
+//
+// sa_cap: false where a score of the warp is beyond the polynomials (x is unchanged: sa_cap_any).  `count`: whether the row has a say in
+// that (one that sees nothing may hold anything).  All lanes of the warp.
+template <int N>
+__device__ __forceinline__ bool sa_cap(uint32_t (&x)[N], const SpanArgs &p, bool count) {
+  float most[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    most[0] = fmaxf(most[0], fabsf(__uint_as_float(x[i])));
+    most[1] = fmaxf(most[1], fabsf(__uint_as_float(x[i + 1])));
+  }
+  const float top = fmaxf(most[0], most[1]);
+  if (__all_sync(0xffffffffu, !count || top <= p.lim2)) {
+    const pair32 c0 = pair_of(p.t2[0], p.t2[0]), c1 = pair_of(p.t2[1], p.t2[1]), c2 = pair_of(p.t2[2], p.t2[2]);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      most[0] = fmaxf(most[0], fabsf(__uint_as_float(x[i])));
-      most[1] = fmaxf(most[1], fabsf(__uint_as_float(x[i + 1])));
+      const pair32 s = pair_get(&x[i]), w = pair_mul(s, s);
+      pair_set(&x[i], pair_mul(s, pair_fma(pair_fma(w, c2, c1), w, c0)));
     }
-    const float top = fmaxf(most[0], most[1]);
-    if (__all_sync(0xffffffffu, !count || top <= p.lim2)) {
-      const pair32 c0 = pair_of(p.t2[0], p.t2[0]), c1 = pair_of(p.t2[1], p.t2[1]), c2 = pair_of(p.t2[2], p.t2[2]);
-#pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const pair32 s = pair_get(&x[i]), w = pair_mul(s, s);
-        pair_set(&x[i], pair_mul(s, pair_fma(pair_fma(w, c2, c1), w, c0)));
-      }
-    } else if (__all_sync(0xffffffffu, !count || top <= p.lim4)) {
-      const pair32 c0 = pair_of(p.t4[0], p.t4[0]), c1 = pair_of(p.t4[1], p.t4[1]), c2 = pair_of(p.t4[2], p.t4[2]), c3 = pair_of(p.t4[3], p.t4[3]),
-                   c4 = pair_of(p.t4[4], p.t4[4]);
-#pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const pair32 s = pair_get(&x[i]), w = pair_mul(s, s);
-        pair_set(&x[i], pair_mul(s, pair_fma(pair_fma(pair_fma(pair_fma(w, c4, c3), w, c2), w, c1), w, c0)));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = __float_as_uint(sa_tanh_any(__uint_as_float(x[i]) * p.to_z) * p.from_z);
-    }
+    return true;
   }
-  if constexpr (BIAS) {
-    // distances are whole numbers: exact
-    pair32 d = pair_of(d0, d0 + 1.f);
-    const pair32 two = pair_of(2.f, 2.f);
-    if (side != 0) {
-      const float k = side > 0 ? -slope : slope;
-      const pair32 kk = pair_of(k, k);
+  if (__all_sync(0xffffffffu, !count || top <= p.lim4)) {
+    const pair32 c0 = pair_of(p.t4[0], p.t4[0]), c1 = pair_of(p.t4[1], p.t4[1]), c2 = pair_of(p.t4[2], p.t4[2]), c3 = pair_of(p.t4[3], p.t4[3]),
+                 c4 = pair_of(p.t4[4], p.t4[4]);
 #pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        pair_set(&x[i], pair_fma(kk, d, pair_get(&x[i])));
-        d = pair_add(d, two);
-      }
-    } else {
-      const pair32 kk = pair_of(-slope, -slope);
+    for (int i = 0; i < N; i += 2) {
+      const pair32 s = pair_get(&x[i]), w = pair_mul(s, s);
+      pair_set(&x[i], pair_mul(s, pair_fma(pair_fma(pair_fma(pair_fma(w, c4, c3), w, c2), w, c1), w, c0)));
+    }
+    return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void sa_cap_any(uint32_t (&x)[32], const SpanArgs &p) {
 #pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        pair_set(&x[i], pair_fma(kk, d & 0x7fffffff7fffffffull, pair_get(&x[i])));
-        d = pair_add(d, two);
-      }
+  for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(sa_tanh_any(__uint_as_float(x[i]) * p.to_z) * p.from_z);
+}
+// The bias: d0 = position of the first column less the row's (distances are whole numbers: exact), side: -1 / 1 where no column of the warp
+// lies right / left of its row, 0 otherwise; slope: the head's, over the scale
+template <int N>
+__device__ __forceinline__ void sa_bias(uint32_t (&x)[N], float slope, float d0, int side) {
+  pair32 d = pair_of(d0, d0 + 1.f);
+  const pair32 two = pair_of(2.f, 2.f);
+  const float k = side < 0 ? slope : -slope;
+  const pair32 kk = pair_of(k, k);
+  if (side != 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      pair_set(&x[i], pair_fma(kk, d, pair_get(&x[i])));
+      d = pair_add(d, two);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      pair_set(&x[i], pair_fma(kk, d & 0x7fffffff7fffffffull, pair_get(&x[i])));
+      d = pair_add(d, two);
     }
   }
 }
@@ -171,6 +176,9 @@ struct SaBias {
 // 32 of a thread's registers
 template <int N>
 __device__ __forceinline__ uint32_t (&sa_group(uint32_t (&x)[N], int g))[32] { return *reinterpret_cast<uint32_t(*)[32]>(&x[g * 32]); }
+
+// the first load through a tensor map waits for the map itself: asked for ahead
+__device__ __forceinline__ void sa_prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)map) : "memory"); }
 
 // 16 columns of a warp's 32 lanes into tensor memory
 __device__ __forceinline__ void sa_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {

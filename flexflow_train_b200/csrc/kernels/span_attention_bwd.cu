@@ -22,7 +22,7 @@ namespace {
 constexpr int SAB_THREADS = 640;
 constexpr int SAB_WARPS = 16;           // element-wise warps: 32 columns of a tile each
 
-// y[c], y[c + 1] (scores, see sa_scores) become e0, e1 times the cap's derivative 1 - (a y)^2
+// y[c], y[c + 1] (scores, see sa_cap) become e0, e1 times the cap's derivative 1 - (a y)^2
 __device__ __forceinline__ void sa_times_slope(uint32_t (&y)[32], int c, float e0, float e1, float a) {
   const pair32 e = pair_of(e0, e1), z = pair_mul(pair_get(&y[c]), pair_of(a, a));
   pair_set(&y[c], pair_fma(pair_mul(z, pair_of(-e0, -e1)), z, e));
@@ -141,6 +141,9 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int k0 = kb * SA_T, k1 = min(k0 + SA_T, p.S) - 1;
   const int nqt = (p.S + SA_T - 1) / SA_T;
 
+  if (threadIdx.x == 64) {
+    sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmQ); sa_prefetch_map(&tmDO); sa_prefetch_map(&tmDK); sa_prefetch_map(&tmDV);
+  }
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
     for (int s = 0; s < 2; ++s) { mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], SAB_WARPS); }
@@ -374,7 +377,9 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (key < t.z || key > t.w) y[c + 1] = 0u;
           }
         }
-        sa_scores<CAP, false>(y, p, true, 0.f, 0.f, 0);
+        if constexpr (CAP) {
+          if (!sa_cap(y, p, true)) sa_cap_any(y, p);
+        }
         const int qg = i * SA_T + cols * 32;
         SaBias bias(BIAS ? p.slopes[kh * group + g] : 0.f, (float)(qg - key), qg >= kw + 31 ? 1 : qg + 31 <= kw ? -1 : 0);
 #pragma unroll
@@ -535,6 +540,9 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   const int h = bh % p.H, b = bh / p.H, kh = h / (p.H / p.KH);
   const int q0 = qb * SA_T;
 
+  if (threadIdx.x == 64) {
+    sa_prefetch_map(&tmQ); sa_prefetch_map(&tmDO); sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmDQ);
+  }
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_ready[s], 1); mbar_init(&k_empty[s], 1); }
@@ -734,7 +742,9 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         tmem_ld32(t_s, y);
         tmem_ld_wait();
         if (CAP && masked) sa_mask(y, lo - kg, hi - kg, 0u);       // masked scores do not choose the way tanh is taken
-        sa_scores<CAP, false>(y, p, !empty, 0.f, 0.f, 0);
+        if constexpr (CAP) {
+          if (!sa_cap(y, p, !empty)) sa_cap_any(y, p);
+        }
         SaBias bias(slope, (float)(kg - q), kg + 31 <= q_low ? -1 : kg >= q_low + 31 ? 1 : 0);
 #pragma unroll
         for (int c = 0; c < 32; c += 16) {

@@ -71,6 +71,7 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int h = bh % p.H, b = bh / p.H, kh = h / (p.H / p.KH);
   const int q0 = qb * rows_cta;
 
+  if (threadIdx.x == 64) { sa_prefetch_map(&tmQ); sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmO); }
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) { mbar_init(&q_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
     for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
@@ -309,7 +310,25 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         for (int c = 0; c < 128; ++c)
           if ((unsigned)(c - first) > (unsigned)width) x[c] = 0u;
       }
-      sa_scores<CAP, BIAS>(x, p, !empty, slope, (float)(k0 - q), k0 + SA_T - 1 <= q_low ? -1 : k0 >= q_low + 31 ? 1 : 0);
+      if constexpr (CAP) {
+        if (!sa_cap(x, p, !empty)) {
+          // scores near the cap, 32 columns at a time through tensor memory, where they still are: this path is rare and its code was as long
+          // as the rest of the step's
+#pragma unroll 1
+          for (int g = 0; g < 4; ++g) {
+            uint32_t y[32];
+            tmem_ld32(t_s + (uint32_t)(g * 32), y);
+            tmem_ld_wait();
+            sa_cap_any(y, p);
+            tmem_st32(t_s + (uint32_t)(g * 32), y);
+          }
+          tmem_st_wait();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + (uint32_t)(c * 32), sa_group(x, c));
+          tmem_ld_wait();
+        }
+      }
+      if constexpr (BIAS) sa_bias(x, slope, (float)(k0 - q), k0 + SA_T - 1 <= q_low ? -1 : k0 >= q_low + 31 ? 1 : 0);
       if (!full) {
 #pragma unroll
         for (int c = 0; c < 128; ++c)
