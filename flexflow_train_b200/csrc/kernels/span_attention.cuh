@@ -248,7 +248,7 @@ __device__ __forceinline__ void sa_tile_row(uint8_t *tile, int row, int col, con
                    pack_bf162(__uint_as_float(o[8 * u + 6]) * f, __uint_as_float(o[8 * u + 7]) * f));
 }
 // The tile that `threads` threads (named barrier `id`) have written goes out by TMA, which leaves out what lies behind the sequence or the
-// head's columns; thread `first` issues and waits until it is written.
+// head's columns; thread `first` issues and waits until the tile has been read.
 template <int PANELS>
 __device__ __forceinline__ void sa_tile_out(uint8_t *tile, const CUtensorMap *map, int row, int head, int b, int id, int threads, bool first) {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -257,7 +257,7 @@ __device__ __forceinline__ void sa_tile_out(uint8_t *tile, const CUtensorMap *ma
 #pragma unroll
     for (int c = 0; c < PANELS; ++c) tma_store_4d(smem_u32(tile + c * SA_PANEL), map, c * 64, row, head, b);
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the tile has been read; it is written by the kernel's end
   }
 }
 

@@ -127,7 +127,6 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint64_t *dkv_full = bars + 15;
   uint32_t *tmem_slot = (uint32_t *)(bars + 16);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
-  int *walk = (int *)(tmem_slot + 2);                             // first and last query tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {
     pdl_entry();
@@ -141,62 +140,69 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int k0 = kb * SA_T, k1 = min(k0 + SA_T, p.S) - 1;
   const int nqt = (p.S + SA_T - 1) / SA_T;
 
-  if (threadIdx.x == 64) {
-    sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmQ); sa_prefetch_map(&tmDO); sa_prefetch_map(&tmDK); sa_prefetch_map(&tmDV);
-  }
-  if (threadIdx.x == 0) {
-    mbar_init(kv_full, 1);
-    for (int s = 0; s < 2; ++s) { mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], SAB_WARPS); }
-    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_full, SAB_WARPS); mbar_init(ds_full, SAB_WARPS); mbar_init(dkv_full, 1);
-    *abort_flag = 0;
-    walk[0] = 0x7fffffff;
-    walk[1] = -1;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
+  // Set-up; the warp that sets up the barriers asks for K and V, and for the first query tile, before the others have met (see the forward)
+  if (warp == 0) {
+    if (lane == 0) {
+      sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmQ); sa_prefetch_map(&tmDO);
+      mbar_init(kv_full, 1);
+      for (int s = 0; s < 2; ++s) { mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], SAB_WARPS); }
+      mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_full, SAB_WARPS); mbar_init(ds_full, SAB_WARPS); mbar_init(dkv_full, 1);
+      *abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+  } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_entry();
-  __syncthreads();
-  const int4 *summary = p.summary + (long long)b * nqt;
-  for (int i = threadIdx.x; i < nqt; i += SAB_THREADS) {
-    const int4 s = summary[i];
-    if (s.x <= k1 && s.y >= k0) {
-      atomicMin(&walk[0], i);
-      atomicMax(&walk[1], i);
+  if (warp == 0 && lane == 0) {
+    mbar_expect_tx(kv_full, 2 * C::TILE);
+#pragma unroll
+    for (int c = 0; c < C::PANELS; ++c) {
+      tma_load_4d(smem_u32(smem + C::OFF_K + c * SA_PANEL), &tmK, kv_full, c * 64, k0, kh, b);
+      tma_load_4d(smem_u32(smem + C::OFF_V + c * SA_PANEL), &tmV, kv_full, c * 64, k0, kh, b);
     }
   }
+  __syncwarp();
+  // first and last query tile that see a key of the block: each warp finds them by itself
+  const int4 *summary = p.summary + (long long)b * nqt;
+  int i0 = 0x7fffffff, i1 = -1;
+  for (int i = lane; i < nqt; i += 32) {
+    const int4 s = summary[i];
+    if (s.x <= k1 && s.y >= k0) { i0 = min(i0, i); i1 = i; }
+  }
+  i0 = __reduce_min_sync(0xffffffffu, i0);
+  i1 = __reduce_max_sync(0xffffffffu, i1);
+  const int ni = i1 < 0 ? 0 : i1 - i0 + 1;
+  const int n = ni * group;                                       // steps: (head, query tile)
+  auto load_qd = [&](int it, int g, int i) {
+    const int s = it & 1;
+    mbar_expect_tx(&qd_full[s], 2 * C::TILE);
+#pragma unroll
+    for (int c = 0; c < C::PANELS; ++c) {
+      tma_load_4d(smem_u32(smem + C::OFF_Q + s * C::TILE + c * SA_PANEL), &tmQ, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
+      tma_load_4d(smem_u32(smem + C::OFF_DO + s * C::TILE + c * SA_PANEL), &tmDO, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
+    }
+  };
+  if (warp == 0 && lane == 0 && n > 0) load_qd(0, 0, i0);
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int i0 = walk[0], ni = walk[1] < 0 ? 0 : walk[1] - i0 + 1;
-  const int n = ni * group;                                       // steps: (head, query tile)
 
   // registers go from the warps that move data to the element-wise ones (128 x 64 + 512 x 104 = 640 x 96)
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0 && n > 0) {
-      mbar_expect_tx(kv_full, 2 * C::TILE);
-#pragma unroll
-      for (int c = 0; c < C::PANELS; ++c) {
-        tma_load_4d(smem_u32(smem + C::OFF_K + c * SA_PANEL), &tmK, kv_full, c * 64, k0, kh, b);
-        tma_load_4d(smem_u32(smem + C::OFF_V + c * SA_PANEL), &tmV, kv_full, c * 64, k0, kh, b);
-      }
+    if (lane == 0) {                      // the first step's tiles are under way
       int g = 0, i = i0;
-      for (int it = 0; it < n; ++it) {
-        const int s = it & 1;
-        if (!mbar_wait(&qd_empty[s], ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_PRODUCER)) break;
-        mbar_expect_tx(&qd_full[s], 2 * C::TILE);
-#pragma unroll
-        for (int c = 0; c < C::PANELS; ++c) {
-          tma_load_4d(smem_u32(smem + C::OFF_Q + s * C::TILE + c * SA_PANEL), &tmQ, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
-          tma_load_4d(smem_u32(smem + C::OFF_DO + s * C::TILE + c * SA_PANEL), &tmDO, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
-        }
+      for (int it = 1; it < n; ++it) {
         if (++i == i0 + ni) { i = i0; ++g; }
+        if (!mbar_wait(&qd_empty[it & 1], ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_PRODUCER)) break;
+        load_qd(it, g, i);
       }
     }
   } else if (warp == 1) {
@@ -236,7 +242,8 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       return mbar_wait_warp(&qd_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
              mbar_wait_warp(&qd_ready[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
     };
-    bool ok = n > 0 && mbar_wait_warp(kv_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && wait_qd(0);
+    // also where no query sees a key: a load under way does not outlive its CTA
+    bool ok = mbar_wait_warp(kv_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && n > 0 && wait_qd(0);
     if (ok) {
       tc_fence_after();
       issue_t(tmem_base + C::TM_S, dk, q_k0, s_full);
@@ -540,31 +547,39 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   const int h = bh % p.H, b = bh / p.H, kh = h / (p.H / p.KH);
   const int q0 = qb * SA_T;
 
-  if (threadIdx.x == 64) {
-    sa_prefetch_map(&tmQ); sa_prefetch_map(&tmDO); sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmDQ);
-  }
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_ready[s], 1); mbar_init(&k_empty[s], 1); }
-    for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
-    mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1);
-    mbar_init(&ds_full[0], SAB_WARPS); mbar_init(&ds_full[1], SAB_WARPS);
-    mbar_init(dp_full, 1); mbar_init(dp_free, SAB_WARPS); mbar_init(dq_full, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
+  if (warp == 0) {
+    if (lane == 0) {
+      sa_prefetch_map(&tmQ); sa_prefetch_map(&tmDO); sa_prefetch_map(&tmK); sa_prefetch_map(&tmV);
+      mbar_init(q_full, 1);
+      for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_ready[s], 1); mbar_init(&k_empty[s], 1); }
+      for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1); }
+      for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&ds_full[s], SAB_WARPS); }
+      mbar_init(dp_full, 1); mbar_init(dp_free, SAB_WARPS); mbar_init(dq_full, 1);
+      *abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+  } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_entry();
-  if (threadIdx.x < SA_T) {
-    const int q = q0 + (int)threadIdx.x;
+  if (warp == 0 && lane == 0) {           // before the others have met (see the forward kernel)
+    mbar_expect_tx(q_full, 2 * C::TILE);
+#pragma unroll
+    for (int c = 0; c < C::PANELS; ++c) {
+      tma_load_4d(smem_u32(smem + C::OFF_Q + c * SA_PANEL), &tmQ, q_full, c * 64, q0, h, b);
+      tma_load_4d(smem_u32(smem + C::OFF_DO + c * SA_PANEL), &tmDO, q_full, c * 64, q0, h, b);
+    }
+  }
+  __syncwarp();
+  if (warp >= 4 && warp < 8) {
+    const int r = (int)threadIdx.x - 128, q = q0 + r;
     const int2 s = q < p.S ? sa_span(p, b, q) : make_int2(1, 0);
-    span[threadIdx.x] = s;
+    span[r] = s;
     const bool sees = s.x <= s.y;
     const int lo = __reduce_min_sync(0xffffffffu, sees ? s.x : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, sees ? s.y : -1);
-    if (lane == 0) range[warp] = make_int2(lo, hi);
+    if (lane == 0) range[warp - 4] = make_int2(lo, hi);
   }
   tc_fence_before();
   __syncthreads();
@@ -582,12 +597,6 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
-      mbar_expect_tx(q_full, 2 * C::TILE);
-#pragma unroll
-      for (int c = 0; c < C::PANELS; ++c) {
-        tma_load_4d(smem_u32(smem + C::OFF_Q + c * SA_PANEL), &tmQ, q_full, c * 64, q0, h, b);
-        tma_load_4d(smem_u32(smem + C::OFF_DO + c * SA_PANEL), &tmDO, q_full, c * 64, q0, h, b);
-      }
       int ki = 0, vi = 0;
       uint64_t t0 = ffk_globaltimer();
       uint32_t spins = 0;
@@ -669,7 +678,8 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       __syncwarp();
       return true;
     };
-    bool ok = n > 0 && mbar_wait_warp(q_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && issue_s(0) && issue_dp(0);
+    // also where the queries see nothing: a load under way does not outlive its CTA
+    bool ok = mbar_wait_warp(q_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && n > 0 && issue_s(0) && issue_dp(0);
     for (int i = 0; i < n && ok; ++i) {
       const uint32_t ph = (uint32_t)i & 1u;
       if (i + 1 < n) {
@@ -799,8 +809,8 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       tc_fence_before();
       sa_warp_arrive(&ds_full[i & 1], lane);
     }
-    if (ok && n > 0) {
-      ok = sa_wait(dq_full, 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+    if (ok) {                             // without a step, Q has to be there before its place is written
+      ok = sa_wait(n > 0 ? dq_full : q_full, 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       tc_fence_after();
     }
     if (ok) {

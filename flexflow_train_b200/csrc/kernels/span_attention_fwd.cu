@@ -71,28 +71,44 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int h = bh % p.H, b = bh / p.H, kh = h / (p.H / p.KH);
   const int q0 = qb * rows_cta;
 
-  if (threadIdx.x == 64) { sa_prefetch_map(&tmQ); sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmO); }
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < 2; ++s) { mbar_init(&q_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
-    for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
-    for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_ready[s], 1); mbar_init(&v_empty[s], 1); }
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
+  // Set-up, as far as it does not touch global memory under the previous kernel's tail.  The warp that sets up the barriers asks for Q before
+  // the others have met: a CTA is a few tiles long, and its first products wait for these loads.
+  if (warp == 0) {
+    if (lane == 0) {
+      sa_prefetch_map(&tmQ); sa_prefetch_map(&tmK); sa_prefetch_map(&tmV);
+      for (int s = 0; s < 2; ++s) { mbar_init(&q_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+      for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
+      for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_ready[s], 1); mbar_init(&v_empty[s], 1); }
+      *abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+  } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_entry();  // the set-up above ran under the previous kernel's tail
+  pdl_entry();
+  const bool has0 = q0 < p.S, has1 = p.tiles == 2 && q0 + SA_T < p.S;       // query tiles with a row
+  if (warp == 0 && lane == 0) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (t == 0 ? has0 : has1) {
+        mbar_expect_tx(&q_full[t], C::TILE);
+#pragma unroll
+        for (int c = 0; c < C::PANELS; ++c)
+          tma_load_4d(smem_u32(smem + C::OFF_Q + t * C::TILE + c * SA_PANEL), &tmQ, &q_full[t], c * 64, q0 + t * SA_T, h, b);
+      }
+  }
+  __syncwarp();
   // spans of the CTA's queries, and what each 32 of them see together
-  if (threadIdx.x < 256) {
-    const int q = q0 + (int)threadIdx.x;
+  if (threadIdx.x >= 64 && threadIdx.x < 320) {
+    const int r = (int)threadIdx.x - 64, q = q0 + r;
     int2 s = make_int2(1, 0);
-    if ((int)threadIdx.x < rows_cta && q < p.S) s = sa_span(p, b, q);
-    span[threadIdx.x] = s;
+    if (r < rows_cta && q < p.S) s = sa_span(p, b, q);
+    span[r] = s;
     const bool sees = s.x <= s.y;
     const int lo = __reduce_min_sync(0xffffffffu, sees ? s.x : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, sees ? s.y : -1);
-    if (lane == 0) range[warp] = make_int2(lo, hi);
+    if (lane == 0) range[warp - 2] = make_int2(lo, hi);
   }
   tc_fence_before();
   __syncthreads();
@@ -119,14 +135,6 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (from[t] <= to[t]) {
-          mbar_expect_tx(&q_full[t], C::TILE);
-#pragma unroll
-          for (int c = 0; c < C::PANELS; ++c)
-            tma_load_4d(smem_u32(smem + C::OFF_Q + t * C::TILE + c * SA_PANEL), &tmQ, &q_full[t], c * 64, q0 + t * SA_T, h, b);
-        }
       // the K and the V ring advance independently; the wait for progress on either is bounded
       int ki = 0, vi = 0;
       uint64_t t0 = ffk_globaltimer();
@@ -193,8 +201,9 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       __syncwarp();
     };
     auto wait_k = [&](int i) -> bool { return mbar_wait_warp(&k_full[i % C::NK], (uint32_t)(i / C::NK) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA); };
-    if (any0) ok = mbar_wait_warp(&q_full[0], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
-    if (any1 && ok) ok = mbar_wait_warp(&q_full[1], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    // also where a tile's queries see nothing: a load under way does not outlive its CTA
+    if (has0) ok = mbar_wait_warp(&q_full[0], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    if (has1 && ok) ok = mbar_wait_warp(&q_full[1], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
     if (ok && n > 0) {
       ok = wait_k(0);
       if (ok) {
@@ -388,8 +397,8 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tc_fence_before();
       sa_warp_arrive(&p_full[t], lane);
     }
-    if (ok && steps > 0) {
-      ok = sa_wait(&o_full[t], 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+    if (t == 0 ? has0 : has1) {           // without a step, Q has to be there before its place is written
+      if (ok) ok = sa_wait(steps > 0 ? &o_full[t] : &q_full[t], 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       tc_fence_after();
     }
     if (ok) {
