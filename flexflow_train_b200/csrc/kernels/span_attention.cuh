@@ -29,6 +29,8 @@ struct FfkSpanAttnDesc {
   float *scratch;                  // backward: delta [B, H, S], then one summary of four ints per batch row and 128 queries
 };
 
+static_assert(sizeof(FfkSpanAttnDesc) == 192, "packed field by field by the Python side");
+
 namespace {
 
 constexpr float SA_LOG2E = 1.4426950408889634f;

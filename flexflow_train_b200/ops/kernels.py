@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_longlong, c_ulonglong, c_void_p
 from typing import Optional
 
@@ -76,16 +77,10 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
-class SpanAttnDesc(ctypes.Structure):
-    _fields_ = [
-        ("B", c_int), ("H", c_int), ("KH", c_int), ("S", c_int), ("D", c_int), ("scale", c_float), ("cap", c_float),
-        ("spans", c_void_p), ("slopes", c_void_p),
-        ("Q", c_void_p), ("ldq", c_longlong), ("K", c_void_p), ("ldk", c_longlong), ("V", c_void_p), ("ldv", c_longlong),
-        ("O", c_void_p), ("ldo", c_longlong), ("lse", c_void_p),
-        ("dO", c_void_p), ("lddo", c_longlong),
-        ("dQ", c_void_p), ("lddq", c_longlong), ("dK", c_void_p), ("lddk", c_longlong), ("dV", c_void_p), ("lddv", c_longlong),
-        ("scratch", c_void_p),
-    ]
+# One call of span attention as the C structure lies in memory: B, H, KH, S, D, scale, cap, the spans' and the slopes' addresses, (address,
+# pitch) of Q, K, V, O, lse's address, (address, pitch) of dO, dQ, dK, dV, the scratch's address (packed in a third of the time that
+# filling a ctypes structure takes)
+_SPAN_DESC = struct.Struct("=5i2f4x" + "Q" * 2 + "Qq" * 4 + "Q" + "Qq" * 4 + "Q")
 
 
 class ConvDesc(ctypes.Structure):
@@ -435,29 +430,33 @@ def span_attention_last_error() -> int:
 
 
 def _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes):
-    """Checks of what both directions share."""
+    """Checks of what both directions share; the addresses of spans, slopes and lse."""
     if B < 0 or S < 0 or H < 1 or KH < 1 or H % KH:
         raise KernelError(f"{what}: every key head serves the same number of query heads (H {H}, KH {KH}, B {B}, S {S})")
     if D < 8 or D > 128 or D % 8:
         raise KernelError(f"{what}: head dim {D} (a multiple of 8 up to 128 expected)")
     if not (0.0 < scale < _INF and 0.0 <= cap < _INF):
         raise KernelError(f"{what}: scale must be positive and cap not negative")
-    if spans is None or spans.dtype is not torch.int32 or spans.shape != (B, S, 2) or not spans.is_contiguous() or spans.data_ptr() % 8:
+    at = spans.data_ptr() if spans is not None else 1
+    if at % 8 or spans.dtype is not torch.int32 or spans.shape != (B, S, 2) or not spans.is_contiguous():
         raise KernelError(f"{what}: spans is a contiguous int32 [B, S, 2] tensor (attention_spans)")
     if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous()):
         raise KernelError(f"{what}: slopes holds one fp32 value per query head")
     if lse is None or lse.dtype is not torch.float32 or lse.shape != (B, H, S) or not lse.is_contiguous():
         raise KernelError(f"{what}: lse must be a contiguous fp32 [B, H, S] tensor")
+    return at, 0 if slopes is None else slopes.data_ptr(), lse.data_ptr()
 
 
 _INF = float("inf")
 
 
 def _span_place(what, name, t, rows, width):
-    """A [B*S, >= width] bf16 matrix with unit column stride whose rows TMA can address: (name, address, pitch, width in bytes, end)."""
+    """A [B*S, >= width] bf16 matrix with unit column stride whose rows TMA can address: (address, pitch, width, end, name), pitch and
+    width in elements."""
     if t is None or t.dtype is not torch.bfloat16 or t.dim() != 2:
         raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
-    (n, columns), (ld, one) = t.shape, t.stride()
+    n, columns = t.shape
+    ld, one = t.stride()
     if n != rows or columns < width or (one != 1 and columns > 1):
         raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
     if rows <= 1:
@@ -465,17 +464,17 @@ def _span_place(what, name, t, rows, width):
     p = t.data_ptr()
     if ld < width or ld % 8 or p % 16:
         raise KernelError(f"{what}: {name} must start on a 16-byte boundary, at a pitch of a multiple of 8 elements that holds its heads")
-    return name, p, 2 * ld, 2 * width, p + 2 * ((rows - 1) * ld + width)
+    return p, ld, width, p + 2 * ((rows - 1) * ld + width), name
 
 
 def _span_apart(what, a, others):
     """Refuses a matrix that shares memory with another.  Two of one pitch may lie side by side (views into a packed buffer)."""
-    name, p, ld, width, end = a
-    for other, q, lq, wq, last in others:
+    p, ld, width, end, name = a
+    for q, lq, wq, last, other in others:
         if end <= q or last <= p:
             continue
-        gap = (q - p) % ld
-        if ld == lq and gap >= width and gap + wq <= ld:
+        gap = (q - p) % (2 * ld)
+        if ld == lq and gap >= 2 * width and gap + 2 * wq <= 2 * ld:
             continue
         raise KernelError(f"{what}: {name} and {other} share memory")
 
@@ -490,16 +489,15 @@ def span_attention_fwd(q, k, v, out, lse, spans, *, B, S, H, KH, D, scale, cap=0
     fp32 receives the base-2 log-sum-exp of x (0 for an empty span), which `span_attention_bwd` needs.  What tokens hold that no query
     sees does not matter, NaN included."""
     what = "span_attention_fwd"
-    _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
+    at, slope, stat = _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
     rows, wide, narrow = B * S, H * D, KH * D
     Q, Kp, V = _span_place(what, "q", q, rows, wide), _span_place(what, "k", k, rows, narrow), _span_place(what, "v", v, rows, narrow)
     O = _span_place(what, "out", out, rows, wide)
     if rows:
         _span_apart(what, O, (Q, Kp, V))
     stream = _launch_stream(q, k, v, out, lse, spans, slopes)
-    d = SpanAttnDesc(B, H, KH, S, D, scale, cap, spans.data_ptr(), _p(slopes), Q[1], Q[2] >> 1, Kp[1], Kp[2] >> 1, V[1], V[2] >> 1, O[1], O[2] >> 1,
-                     lse.data_ptr())
-    _check(_nlib().ffk_span_attention_fwd(ctypes.byref(d), stream), what)
+    d = _SPAN_DESC.pack(B, H, KH, S, D, scale, cap, at, slope, Q[0], Q[1], Kp[0], Kp[1], V[0], V[1], O[0], O[1], stat, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _check(_nlib().ffk_span_attention_fwd(d, stream), what)
     return out
 
 
@@ -513,22 +511,22 @@ def span_attention_bwd(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, *, B
     key head).  out and lse are the forward pass's.  Every sum is taken in a fixed order: the same inputs give the same bits.  scratch:
     span_attention_bwd_scratch_floats(B, H, S) fp32 elements on a 16-byte boundary.  The slopes have no gradient."""
     what = "span_attention_bwd"
-    _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
+    at, slope, stat = _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
     rows, wide, narrow = B * S, H * D, KH * D
     Q, Kp, V = _span_place(what, "q", q, rows, wide), _span_place(what, "k", k, rows, narrow), _span_place(what, "v", v, rows, narrow)
     O, dO = _span_place(what, "out", out, rows, wide), _span_place(what, "dout", dout, rows, wide)
     dQ, dK, dV = _span_place(what, "dq", dq, rows, wide), _span_place(what, "dk", dk, rows, narrow), _span_place(what, "dv", dv, rows, narrow)
-    if scratch is None or scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.data_ptr() % 16 or \
-            scratch.numel() < span_attention_bwd_scratch_floats(B, H, S):
+    room = scratch.data_ptr() if scratch is not None else 1
+    if room % 16 or scratch.dtype is not torch.float32 or not scratch.is_contiguous() or scratch.numel() < span_attention_bwd_scratch_floats(B, H, S):
         raise KernelError(f"{what}: scratch must hold span_attention_bwd_scratch_floats(B, H, S) fp32 elements")
     if rows:
         _span_apart(what, dQ, (dK, dV, Q, Kp, V, O, dO))
         _span_apart(what, dK, (dV, Q, Kp, V, O, dO))
         _span_apart(what, dV, (Q, Kp, V, O, dO))
     stream = _launch_stream(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, slopes)
-    d = SpanAttnDesc(B, H, KH, S, D, scale, cap, spans.data_ptr(), _p(slopes), Q[1], Q[2] >> 1, Kp[1], Kp[2] >> 1, V[1], V[2] >> 1, O[1], O[2] >> 1,
-                     lse.data_ptr(), dO[1], dO[2] >> 1, dQ[1], dQ[2] >> 1, dK[1], dK[2] >> 1, dV[1], dV[2] >> 1, scratch.data_ptr())
-    _check(_nlib().ffk_span_attention_bwd(ctypes.byref(d), stream), what)
+    d = _SPAN_DESC.pack(B, H, KH, S, D, scale, cap, at, slope, Q[0], Q[1], Kp[0], Kp[1], V[0], V[1], O[0], O[1], stat,
+                        dO[0], dO[1], dQ[0], dQ[1], dK[0], dK[1], dV[0], dV[1], room)
+    _check(_nlib().ffk_span_attention_bwd(d, stream), what)
 
 
 def _es(t):
@@ -780,8 +778,8 @@ def _new_ops_decl(l):
         "ffk_rmsnorm_bwd": ([P, P, P, P, P, P, P, P, I, I, I, I, S], c_int),
         "ffk_rmsnorm_bwd_scratch": ([I, I], c_longlong),
         "ffk_attention_spans": ([P, P, P, I, I, I, S], c_int),
-        "ffk_span_attention_fwd": ([ctypes.POINTER(SpanAttnDesc), S], c_int),
-        "ffk_span_attention_bwd": ([ctypes.POINTER(SpanAttnDesc), S], c_int),
+        "ffk_span_attention_fwd": ([ctypes.c_char_p, S], c_int),
+        "ffk_span_attention_bwd": ([ctypes.c_char_p, S], c_int),
         "ffk_span_attention_bwd_scratch_floats": ([I, I, I], c_longlong),
         "ffk_span_attention_last_error": ([], c_int),
         "ffk_adam_update_clipped": ([P, P, P, P, P, L, F, F, F, F, F, F, P, P, F, I, S], c_int),
@@ -809,30 +807,35 @@ def _nlib():
 
 
 def _rms_check(what, a, gamma, rstd, same):
-    """Checks of the RMS norm's operands: `a` [rows, cols], gamma [cols], rstd [rows], (name, tensor) pairs of a's shape.  Everything is
-    contiguous.  Returns rows, cols and the tensors' bytes."""
+    """Checks of the RMS norm's operands: `a` [rows, cols], gamma [cols], rstd [rows], tensors of a's shape.  Everything is contiguous.
+    Returns rows, cols and the bytes of `a` and of gamma."""
     shape, dtype = a.shape, a.dtype
     if len(shape) != 2:
         raise KernelError(f"{what}: rows are a 2-D [rows, cols] tensor")
     rows, cols = shape
-    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+    if dtype is torch.bfloat16:
+        es = 2
+    elif dtype is torch.float32:
+        es = 4
+    else:
         raise KernelError(f"{what}: bf16 or fp32 rows expected, got {dtype}")
     if cols < 1 or rows > 2**31 - 1 or cols > 2**31 - 1:
         raise KernelError(f"{what}: rows of {cols} elements")
-    for _, t in same:
-        if t is not None and (t.dtype is not dtype or t.shape != shape):
-            raise KernelError(f"{what}: tensors of the rows' shape and dtype expected")
+    whole = a.is_contiguous()
+    for t in same:
+        if t is not None:
+            if t.dtype is not dtype or t.shape != shape:
+                raise KernelError(f"{what}: tensors of the rows' shape and dtype expected")
+            whole = whole and t.is_contiguous()
     if gamma is None or gamma.dtype is not dtype or gamma.shape != (cols,):
         raise KernelError(f"{what}: gamma must hold one value of the rows' dtype per column")
-    if rstd is not None and (rstd.dtype is not torch.float32 or rstd.numel() != rows):
-        raise KernelError(f"{what}: rstd must be fp32 with one value per row")
-    for t in (a, gamma, rstd):
-        if t is not None and not t.is_contiguous():
-            raise KernelError("kernel called with a non-contiguous tensor")
-    for _, t in same:
-        if t is not None and not t.is_contiguous():
-            raise KernelError("kernel called with a non-contiguous tensor")
-    return rows, cols, rows * cols * (2 if dtype is torch.bfloat16 else 4)
+    if rstd is not None:
+        if rstd.dtype is not torch.float32 or rstd.numel() != rows:
+            raise KernelError(f"{what}: rstd must be fp32 with one value per row")
+        whole = whole and rstd.is_contiguous()
+    if not (whole and gamma.is_contiguous()):
+        raise KernelError("kernel called with a non-contiguous tensor")
+    return rows, cols, rows * cols * es, cols * es
 
 
 def _apart(what, a, pa, na, b, pb, nb):
@@ -845,33 +848,42 @@ def rmsnorm_fwd(a, gamma, eps, residual=None, xsum=None, out=None, rstd=None):
     """out = h / sqrt(mean(h^2) + eps) * gamma over the rows of h = a + residual (h = a without a residual), h rounded to the rows'
     dtype (bf16 or fp32).  xsum receives h, rstd (fp32, one per row) the reciprocal root, which `rmsnorm_bwd` needs.  `out` and `xsum`
     may be `a` or `residual` themselves."""
-    rows, cols, size = _rms_check("rmsnorm_fwd", a, gamma, rstd, (("residual", residual), ("xsum", xsum), ("out", out)))
+    rows, cols, size, small = _rms_check("rmsnorm_fwd", a, gamma, rstd, (residual, xsum, out))
     if xsum is not None and residual is None:
         raise KernelError("rmsnorm_fwd: xsum is the sum with a residual")
     if out is None:
         out = torch.empty_like(a)
+    # (name, address, bytes); an output may be an input of its size, but no part of one
     pa, pg, po = a.data_ptr(), gamma.data_ptr(), out.data_ptr()
-    pr, px, ps = _p(residual), _p(xsum), _p(rstd)
-    small = gamma.numel() * gamma.element_size()
-    for name, p in (("out", po), ("xsum", px)):
-        if p is None:
-            continue
-        if p != pa:
-            _apart("rmsnorm_fwd", name, p, size, "a", pa, size)
-        if pr is not None and p != pr:
-            _apart("rmsnorm_fwd", name, p, size, "residual", pr, size)
-        _apart("rmsnorm_fwd", name, p, size, "gamma", pg, small)
-        if ps is not None:
-            _apart("rmsnorm_fwd", name, p, size, "rstd", ps, 4 * rows)
-    if px is not None:
-        _apart("rmsnorm_fwd", "out", po, size, "xsum", px, size)
-    if ps is not None:
-        for name, p, n in (("a", pa, size), ("residual", pr, size), ("gamma", pg, small)):
-            if p is not None:
-                _apart("rmsnorm_fwd", "rstd", ps, 4 * rows, name, p, n)
+    pr = px = ps = None
+    ins, outs = [("a", pa, size), ("gamma", pg, small)], [("out", po, size)]
+    if residual is not None:
+        pr = residual.data_ptr()
+        ins.append(("residual", pr, size))
+    if xsum is not None:
+        px = xsum.data_ptr()
+        outs.append(("xsum", px, size))
+    if rstd is not None:
+        ps = rstd.data_ptr()
+        outs.append(("rstd", ps, 4 * rows))
+    _rms_apart("rmsnorm_fwd", outs, ins)
     stream = _launch_stream(a, residual, gamma, xsum, out, rstd)
     _check(_nlib().ffk_rmsnorm_fwd(pa, pr, pg, px, po, ps, rows, cols, eps, _DT[a.dtype], stream), "ffk_rmsnorm_fwd")
     return out
+
+
+def _rms_apart(what, outs, ins):
+    """Refuses outputs that share memory with one another or with an input: lists of (name, address, bytes).  The first output, and a sum,
+    are written element by element where the inputs of their size have been read: they may be one of those, but no part of one."""
+    for i, (name, p, n) in enumerate(outs):
+        end = p + n
+        may = i == 0 or name == "xsum"
+        for other, q, m in ins:
+            if p < q + m and q < end and not (may and p == q and n == m and other != "gamma"):
+                _apart(what, name, p, n, other, q, m)
+        for other, q, m in outs[i + 1:]:
+            if p < q + m and q < end:
+                _apart(what, name, p, n, other, q, m)
 
 
 def rmsnorm_bwd_scratch(rows, cols) -> int:
@@ -885,33 +897,25 @@ def rmsnorm_bwd(dy, x, gamma, rstd, dx, dgamma, scratch, dsum=None, accumulate_p
     sums, added in a fixed order.  dx may be dy, x or dsum themselves.  scratch: rmsnorm_bwd_scratch(rows, cols) fp32 elements."""
     if rstd is None or x is None or dx is None:
         raise KernelError("rmsnorm_bwd: x, rstd and dx are needed")
-    rows, cols, size = _rms_check("rmsnorm_bwd", dy, gamma, rstd, (("x", x), ("dx", dx), ("dsum", dsum)))
-    px, pd, pg, ps = dx.data_ptr(), _p(dgamma), gamma.data_ptr(), rstd.data_ptr()
-    small, pc, nc = gamma.numel() * gamma.element_size(), None, 0
+    rows, cols, size, small = _rms_check("rmsnorm_bwd", dy, gamma, rstd, (x, dx, dsum))
+    py, ph, px, pg, ps = dy.data_ptr(), x.data_ptr(), dx.data_ptr(), gamma.data_ptr(), rstd.data_ptr()
+    pd = pc = pu = None
+    ins, outs = [("dy", py, size), ("x", ph, size), ("gamma", pg, small), ("rstd", ps, 4 * rows)], [("dx", px, size)]
+    if dsum is not None:
+        pu = dsum.data_ptr()
+        ins.append(("dsum", pu, size))
     if dgamma is not None:
         if dgamma.dtype is not dy.dtype or dgamma.shape != (cols,) or not dgamma.is_contiguous():
             raise KernelError("rmsnorm_bwd: dgamma must be like gamma")
+        pd = dgamma.data_ptr()
+        outs.append(("dgamma", pd, small))
         if rows:
-            nc = 4 * rmsnorm_bwd_scratch(rows, cols)
-            if scratch is None or scratch.dtype is not torch.float32 or 4 * scratch.numel() < nc or not scratch.is_contiguous():
+            room = rmsnorm_bwd_scratch(rows, cols)
+            if scratch is None or scratch.dtype is not torch.float32 or scratch.numel() < room or not scratch.is_contiguous():
                 raise KernelError("rmsnorm_bwd: scratch smaller than rmsnorm_bwd_scratch(rows, cols)")
             pc = scratch.data_ptr()
-    py, ph, pu = dy.data_ptr(), x.data_ptr(), _p(dsum)
-    ins = [("dy", py, size), ("x", ph, size), ("gamma", pg, small), ("rstd", ps, 4 * rows)]
-    if pu is not None:
-        ins.append(("dsum", pu, size))
-    for name, p, n in ins:
-        if p != px or n != size:
-            _apart("rmsnorm_bwd", "dx", px, size, name, p, n)
-        if pd is not None:
-            _apart("rmsnorm_bwd", "dgamma", pd, small, name, p, n)
-            if pc is not None:
-                _apart("rmsnorm_bwd", "scratch", pc, nc, name, p, n)
-    if pd is not None:
-        _apart("rmsnorm_bwd", "dx", px, size, "dgamma", pd, small)
-        if pc is not None:
-            _apart("rmsnorm_bwd", "dx", px, size, "scratch", pc, nc)
-            _apart("rmsnorm_bwd", "dgamma", pd, small, "scratch", pc, nc)
+            outs.append(("scratch", pc, 4 * room))
+    _rms_apart("rmsnorm_bwd", outs, ins)
     stream = _launch_stream(dy, x, gamma, rstd, dx, dsum, dgamma, scratch if pc is not None else None)
     _check(_nlib().ffk_rmsnorm_bwd(py, ph, pg, ps, pu, px, pd, pc, rows, cols, _DT[dy.dtype], 1 if accumulate_params else 0, stream),
            "ffk_rmsnorm_bwd")

@@ -107,6 +107,12 @@ def test_rmsnorm_refuses():
     refused("dgamma", lambda: K.rmsnorm_bwd(x, x.clone(), g, r, x.clone(), g.bfloat16(), big))
     refused("needed", lambda: K.rmsnorm_bwd(x, x.clone(), g, None, x.clone(), g.clone(), big))
     refused("share memory", lambda: K.rmsnorm_bwd(x, x.clone(), g, r, flat[:128].view(4, 32), flat[100:132], big))
+    refused("dgamma and gamma share", lambda: K.rmsnorm_bwd(x, x.clone(), g, r, x.clone(), g, big))
+    one = torch.zeros(1, 32)
+    refused("out and gamma share", lambda: K.rmsnorm_fwd(one, g, 1e-6, out=g.view(1, 32)))
+    exact = torch.zeros(K.rmsnorm_bwd_scratch(4, 32) // 32, 32)
+    refused("scratch and x share|shape", lambda: K.rmsnorm_bwd(x, exact[:4], g, r, x.clone(), g.clone(), exact.view(-1)))
+    refused("rstd and a share", lambda: K.rmsnorm_fwd(flat[:4].view(4, 1), torch.zeros(1), 1e-6, rstd=flat[:4]))
 
 
 # ---------------------------------------------------------------------------------------------- clipping
