@@ -34,6 +34,7 @@ static_assert(sizeof(FfkSpanAttnDesc) == 192, "packed field by field by the Pyth
 namespace {
 
 constexpr float SA_LOG2E = 1.4426950408889634f;
+constexpr float SA_MOST_CAP = 1073741824.f;   // cap / scale at most: beyond, the cap is no cap
 constexpr int SA_T = 128;          // rows of a tile of queries or keys
 constexpr int SA_PANEL = SA_T * 128;   // bytes of 64 columns of a tile
 
@@ -206,18 +207,6 @@ __device__ __forceinline__ int2 sa_span(const SpanArgs &p, int b, int q) {
   return s;
 }
 
-// How a warp's 32 rows see columns [c, c + 31], as spans [lo, hi] of each lane: bits of `none` and `part` by column group of 32.  All lanes.
-template <int GROUPS>
-__device__ __forceinline__ void sa_kinds(int lo, int hi, int c, uint32_t &none, uint32_t &part) {
-  none = part = 0;
-  if (__all_sync(0xffffffffu, lo <= c && hi >= c + GROUPS * 32 - 1)) return;
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    const int a = c + g * 32, z = a + 31;
-    if (!__any_sync(0xffffffffu, lo <= z && hi >= a)) none |= 1u << g;
-    else if (!__all_sync(0xffffffffu, lo <= a && hi >= z)) part |= 1u << g;
-  }
-}
 // columns before `a` and behind `z` (of 32) become `v`
 __device__ __forceinline__ void sa_mask(uint32_t (&x)[32], int a, int z, uint32_t v) {
 #pragma unroll
@@ -290,7 +279,8 @@ inline int sa_head_map(CUtensorMap *map, const void *ptr, int D, int S, long lon
 
 inline bool sa_aligned(const void *p, long long ld) { return (((uintptr_t)p) & 15) == 0 && (ld * 2) % 16 == 0; }
 inline bool sa_shape_ok(const FfkSpanAttnDesc *d) {
-  return d->KH > 0 && d->H % d->KH == 0 && d->D >= 8 && d->D <= 128 && d->D % 8 == 0 && d->scale > 0.f && d->cap >= 0.f && (((uintptr_t)d->spans) & 7) == 0;
+  return d->KH > 0 && d->H % d->KH == 0 && d->D >= 8 && d->D <= 128 && d->D % 8 == 0 && d->scale > 0.f && d->cap >= 0.f &&
+         d->cap <= d->scale * SA_MOST_CAP && d->S <= (1 << 30) && (((uintptr_t)d->spans) & 7) == 0;
 }
 inline void sa_args(const FfkSpanAttnDesc *d, SpanArgs &a, int *err) {
   a.B = d->B; a.H = d->H; a.KH = d->KH; a.S = d->S; a.D = d->D;
@@ -309,9 +299,11 @@ inline void sa_args(const FfkSpanAttnDesc *d, SpanArgs &a, int *err) {
       if (i < 3) a.t2[i] = t2[i] * f;
       a.t4[i] = t4[i] * f;
     }
-    if (z >= 1.f / 4096 && z <= 1024.f) {      // z^8 within the range of 32 bits
+    // z^4 and z^8 have to be within the range of 32 bits (z is at least 2^-30: sa_shape_ok); the exponential form, which is exact to 2e-7 of the
+    // cap, is then taken only where a score is a fair part of the cap, or the cap itself is next to nothing
+    if (z <= 1024.f) {
       a.lim2 = 0.25f / z;
-      a.lim4 = 0.625f / z;
+      if (z >= 1.f / 16384) a.lim4 = 0.625f / z;
     }
   }
   a.lse = d->lse;

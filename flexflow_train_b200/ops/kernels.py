@@ -435,8 +435,10 @@ def _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes):
         raise KernelError(f"{what}: every key head serves the same number of query heads (H {H}, KH {KH}, B {B}, S {S})")
     if D < 8 or D > 128 or D % 8:
         raise KernelError(f"{what}: head dim {D} (a multiple of 8 up to 128 expected)")
-    if not (0.0 < scale < _INF and 0.0 <= cap < _INF):
-        raise KernelError(f"{what}: scale must be positive and cap not negative")
+    if not (0.0 < scale < _INF and 0.0 <= cap <= scale * 2.0**30):
+        raise KernelError(f"{what}: scale must be positive, cap not negative (0: none) and at most 2^30 times scale")
+    if S > 2**30:
+        raise KernelError(f"{what}: sequences of up to 2^30 tokens")
     at = spans.data_ptr() if spans is not None else 1
     if at % 8 or spans.dtype is not torch.int32 or spans.shape != (B, S, 2) or not spans.is_contiguous():
         raise KernelError(f"{what}: spans is a contiguous int32 [B, S, 2] tensor (attention_spans)")
@@ -486,8 +488,10 @@ def span_attention_fwd(q, k, v, out, lse, spans, *, B, S, H, KH, D, scale, cap=0
     q / out [B*S, >= H*D] and k / v [B*S, >= KH*D] are bf16 matrices with head h in columns [h*D, (h+1)*D) (views into a packed QKV
     buffer are fine); query head h reads key head h // (H // KH).  spans [B, S, 2] int32: the first and last key that each query sees
     (`attention_spans`, or any: what lies outside the sequence is cut off).  A query whose span is empty gets zeros.  lse [B, H, S]
-    fp32 receives the base-2 log-sum-exp of x (0 for an empty span), which `span_attention_bwd` needs.  What tokens hold that no query
-    sees does not matter, NaN included."""
+    fp32 receives the base-2 log-sum-exp of x (0 for an empty span), which `span_attention_bwd` needs.
+
+    What tokens hold that no query sees does not matter, NaN and infinity included.  A NaN or infinity in a token that some query does see
+    may reach other queries of its neighbourhood (up to 256 tokens that are computed together)."""
     what = "span_attention_fwd"
     at, slope, stat = _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
     rows, wide, narrow = B * S, H * D, KH * D

@@ -5,6 +5,8 @@ The bounds count roundings, each off by at most half a step of bf16 relative to 
   dV  = sum P^T do: the same                                                              |ddV| <= U (|dV| + P^T|dO|)
   dS  = P c (dP - delta) is rounded; delta = do . O takes O as it was stored             |ddS| <= U |dS| + P c |do| . |dO|
   dQ  = scale dS K, rounded when stored                                                   |ddQ| <= U |dQ| + scale ddS |K|, dK alike
+  c   = 1 - t^2 with t = tanh in 32 bits, to 4e-7 of itself (the polynomials' error, twice the exponential form's, with their roundings): c is off
+        by up to 2 * 4e-7 + 2^-23 < TANH = 1e-6 of 1, which is all there is to it where t is next to 1: a term of p |do| . |v| without c
 SLACK (of the same sums) covers what is held in 32 bits: scores of up to 128 products and exponents (a few 1e-6 each), the exponential and
 tanh (3e-6), accumulation over up to some thousand terms (1e-4 in the worst case), and second-order terms (U^2 = 1.5e-5)."""
 import math
@@ -13,6 +15,7 @@ import torch
 
 U = 2.0 ** -8
 SLACK = 4.0e-4
+TANH = 1.0e-6
 
 
 def visible(spans, S):
@@ -50,8 +53,8 @@ def reference(q, k, v, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None, do
     dp = do @ v.transpose(-1, -2)
     delta = (do * out).sum(-1, keepdim=True)
     ds = p * c * (dp - delta)
-    whole = p * c * (do.abs() @ v.abs().transpose(-1, -2) + (do.abs() * out.abs()).sum(-1, keepdim=True))
-    e_ds = U * ds.abs() + p * c * (do.abs() * e_out).sum(-1, keepdim=True) + SLACK * whole
+    whole = p * (do.abs() @ v.abs().transpose(-1, -2) + (do.abs() * out.abs()).sum(-1, keepdim=True))
+    e_ds = U * ds.abs() + p * c * (do.abs() * e_out).sum(-1, keepdim=True) + (SLACK * c + (TANH if cap > 0 else 0.0)) * whole
     dq, dk, dv = scale * ds @ k, share(scale * ds.transpose(-1, -2) @ q), share(p.transpose(-1, -2) @ do)
     m_dv = share(p.transpose(-1, -2) @ do.abs())
     tiny = 1e-30

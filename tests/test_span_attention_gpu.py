@@ -279,3 +279,77 @@ def test_many_passes_give_the_same_bits(D, KH):
     for _ in range(30):
         again = run(q, k, v, dout, spans, **sizes)
         assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+@pytest.mark.parametrize("cap", [1e-3, 0.05, 300.0, 3000.0, 1e5, 1e8])
+def test_caps_far_from_the_scores(cap):
+    """Caps that every score is far beyond, and caps that no score comes near: the same operator."""
+    B, S, H, KH, D = 1, 200, 2, 2, 64
+    _, q, k, v, dout = make(B, S, H, KH, D, seed=41)
+    spans = mask("causal", B, S, 0)
+    sizes = dict(B=B, S=S, H=H, KH=KH, D=D, scale=1.0 / math.sqrt(D), cap=cap)
+    check(run(q, k, v, dout, spans, **sizes), reference(q, k, v, spans, dout=dout, **sizes))
+
+
+@pytest.mark.parametrize("slope", [0.0, -0.05, 4.0])
+def test_slopes_of_any_sign(slope):
+    B, S, H, KH, D = 1, 300, 2, 1, 64
+    _, q, k, v, dout = make(B, S, H, KH, D, seed=43)
+    spans = mask("full", B, S, 0)
+    sizes = dict(B=B, S=S, H=H, KH=KH, D=D, scale=1.0 / math.sqrt(D), slopes=torch.tensor([slope, 0.01], device="cuda"))
+    check(run(q, k, v, dout, spans, **sizes), reference(q, k, v, spans, dout=dout, **sizes))
+
+
+@pytest.mark.parametrize("B,S", [(0, 5), (3, 0)])
+def test_nothing_to_do(B, S):
+    H, KH, D = 2, 1, 64
+    _, q, k, v, dout = make(B, S, H, KH, D, seed=1)
+    assert K.attention_spans(torch.zeros(B, S, dtype=torch.int32, device="cuda")).shape == (B, S, 2)
+    spans = torch.zeros(B, S, 2, dtype=torch.int32, device="cuda")
+    assert run(q, k, v, dout, spans, B=B, S=S, H=H, KH=KH, D=D, scale=0.1)["dq"].shape == (0, H * D)
+
+
+FIRST_CALL = """
+import torch
+from flexflow_train_b200.ops import kernels as K
+B, S, H, KH, D = 1, 300, 2, 1, 64
+g = torch.Generator(device="cuda").manual_seed(0)
+new = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+q, k, v, dout = new(S, H * D), new(S, D), new(S, D), new(S, H * D)
+out, dq, dk, dv = (torch.empty_like(t) for t in (q, q, k, v))
+x, gamma, y, dx, dgamma = new(S, 128), new(128), new(S, 128), new(S, 128), new(128)
+lse, rstd = torch.empty(B, H, S, device="cuda"), torch.empty(S, device="cuda")
+doc = torch.zeros(B, S, dtype=torch.int32, device="cuda")
+spans = torch.empty(B, S, 2, dtype=torch.int32, device="cuda")
+scratch, room = torch.empty(K.span_attention_bwd_scratch_floats(B, H, S), device="cuda"), torch.empty(K.rmsnorm_bwd_scratch(S, 128), device="cuda")
+grads = K.GradientList([dq, dk, dv, dgamma])
+sizes = dict(B=B, S=S, H=H, KH=KH, D=D, scale=0.125, cap=20.0)
+
+def step():
+    K.attention_spans(doc, out=spans)
+    K.span_attention_fwd(q, k, v, out, lse, spans, **sizes)
+    K.span_attention_bwd(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, **sizes)
+    K.rmsnorm_fwd(x, gamma, 1e-6, out=y, rstd=rstd)
+    K.rmsnorm_bwd(y, x, gamma, rstd, dx, dgamma, room)
+    K.clip_gradients(grads, 1.0)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step()
+graph.replay()
+torch.cuda.synchronize()
+kept = [t.clone() for t in (out, lse, dq, dk, dv, y, dx, dgamma, grads.norm)]
+step()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(kept, (out, lse, dq, dk, dv, y, dx, dgamma, grads.norm)))
+print("same")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stdout + r.stderr

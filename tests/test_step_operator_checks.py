@@ -42,6 +42,7 @@ def test_attention_refuses(name):
     refused("scale", lambda: attention(name, scale=float("nan")))
     refused("cap", lambda: attention(name, cap=-1.0))
     refused("cap", lambda: attention(name, cap=float("inf")))
+    refused("cap", lambda: attention(name, cap=0.126 * 2.0**30))
     refused("slopes", lambda: attention(name, slopes=torch.zeros(H + 1)))
     refused("slopes", lambda: attention(name, slopes=torch.zeros(H, dtype=torch.float64)))
     refused("spans", lambda: attention(name, spans=torch.zeros(B, S, 2, dtype=torch.int64)))
