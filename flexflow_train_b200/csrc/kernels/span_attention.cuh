@@ -49,6 +49,9 @@ struct SpanArgs {
   float *lse;
   const float *delta;
   const int4 *summary;
+  bf16 *dQ, *dK, *dV;
+  long long lddq, lddk, lddv;
+  int wide;                        // results' rows lie on 32-byte boundaries
   int tiles;                       // forward: 128-query tiles of a CTA, 1 or 2
   int *err;
 };
@@ -227,6 +230,47 @@ __device__ __forceinline__ void sa_clear_rows(uint8_t *tile, const uint32_t (&ke
     }
 }
 
+// ---- Blocks of a grid taken over by the ones that run.  A CTA of these kernels fills an SM (tensor memory, shared memory), so that the set-up of
+// one (barriers, tensor memory, first loads: about 5000 cycles) and the read-out of its results run with the tensor core idle; a CTA here
+// is a few tiles long.  So a running CTA asks for the next block that has not been launched, gets its index (or learns that there is none) while
+// it works, and goes on with that block, its rings and barriers running through.
+__device__ __forceinline__ void sa_ask_next(uint64_t *answer, uint64_t *bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// the answer's block, or -1
+__device__ __forceinline__ int sa_next_block(const uint64_t *answer) {
+  uint32_t x, got;
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b128 c;\nld.shared.b128 c, [%2];\nclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, c;\n"
+      "selp.u32 %1, 1, 0, p;\nmov.u32 %0, 0;\n@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, c;\n}"
+      : "=r"(x), "=r"(got)
+      : "r"(smem_u32(answer))
+      : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // read before the next answer is written there
+  return got ? (int)x : -1;
+}
+
+// 32 columns of a row of results, `left` of which exist, as bf16 to global memory: whole sectors where addresses allow it (`wide`)
+__device__ __forceinline__ void sa_store_row(bf16 *out, const uint32_t (&o)[32], float f, int left, bool wide) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = pack_bf162(__uint_as_float(o[16 * u + 2 * j]) * f, __uint_as_float(o[16 * u + 2 * j + 1]) * f);
+    if (wide && 16 * u + 16 <= left) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 16 * u), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                   "r"(v[5]), "r"(v[6]), "r"(v[7])
+                   : "memory");
+    } else {
+      if (16 * u < left) *reinterpret_cast<uint4 *>(out + 16 * u) = make_uint4(v[0], v[1], v[2], v[3]);
+      if (16 * u + 8 < left) *reinterpret_cast<uint4 *>(out + 16 * u + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+    }
+  }
+}
+
 // 32 columns of a row (from column `col` on, a multiple of 32) into a tile in shared memory as TMA reads it: 16-byte piece XOR (row % 8)
 __device__ __forceinline__ void sa_tile_row(uint8_t *tile, int row, int col, const uint32_t (&o)[32], float f) {
   uint8_t *base = tile + (col >> 6) * SA_PANEL + row * 128;
@@ -277,6 +321,7 @@ inline int sa_head_map(CUtensorMap *map, const void *ptr, int D, int S, long lon
   return r == CUDA_SUCCESS ? 0 : 1000 + (int)r;
 }
 
+inline bool sa_wide(const void *p, long long ld, int D) { return (((uintptr_t)p) & 31) == 0 && ld % 16 == 0 && D % 16 == 0; }
 inline bool sa_aligned(const void *p, long long ld) { return (((uintptr_t)p) & 15) == 0 && (ld * 2) % 16 == 0; }
 inline bool sa_shape_ok(const FfkSpanAttnDesc *d) {
   return d->KH > 0 && d->H % d->KH == 0 && d->D >= 8 && d->D <= 128 && d->D % 8 == 0 && d->scale > 0.f && d->cap >= 0.f &&

@@ -99,33 +99,53 @@ struct DkvCfg {
   static constexpr int OFF_DELTA = OFF_LSE + NQ * 512;             // [NQ][128] float
   static constexpr int OFF_SPAN = OFF_DELTA + NQ * 512;            // [NQ][128] int2
   static constexpr int OFF_GROUP = OFF_SPAN + NQ * 1024;           // [NQ][4] int4: summary of each 32 queries
-  static constexpr int OFF_BAR = OFF_GROUP + NQ * 64;
+  static constexpr int OFF_INFO = OFF_GROUP + NQ * 64;             // [2] int4: block, first query tile, query tiles
+  static constexpr int OFF_ANSWER = OFF_INFO + 32;                 // 16 bytes
+  static constexpr int OFF_BAR = OFF_ANSWER + 16;
   static constexpr int SLACK = 1024;
   static constexpr int SMEM = OFF_BAR + 256 + SLACK;
   static constexpr int TM_S = 0, TM_DP = 128, TM_DK = 256, TM_DV = 256 + DT;
   static_assert(SMEM <= 232448, "tiles exceed the shared memory of a CTA");
 };
 
+// A block: 128 keys of one key head.  Block numbers: the first keys, which most queries see under a causal mask, first.
+struct DkvBlock {
+  int b, kh, k0, k1;
+  __device__ __forceinline__ DkvBlock(const SpanArgs &p, int block) {
+    const int heads = p.B * p.KH, kb = block / heads, bh = block - kb * heads;
+    b = bh / p.KH;
+    kh = bh - b * p.KH;
+    k0 = kb * SA_T;
+    k1 = min(k0 + SA_T, p.S) - 1;
+  }
+};
+
 template <int DT, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(SAB_THREADS, 1)
 span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                     const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV, const SpanArgs p) {
+                     const __grid_constant__ CUtensorMap tmDO, const SpanArgs p) {
   using C = DkvCfg<DT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  int4 *info = (int4 *)(smem + C::OFF_INFO);
+  uint64_t *answer = (uint64_t *)(smem + C::OFF_ANSWER);
   uint64_t *bars = (uint64_t *)(smem + C::OFF_BAR);
   uint64_t *kv_full = bars;
-  uint64_t *qd_full = bars + 1;       // [2]
-  uint64_t *qd_ready = bars + 3;      // [2]
-  uint64_t *qd_empty = bars + 5;      // [2]
-  uint64_t *st_full = bars + 7;       // [2]
-  uint64_t *st_empty = bars + 9;      // [2] SAB_WARPS
-  uint64_t *s_full = bars + 11;
-  uint64_t *dp_full = bars + 12;
-  uint64_t *p_full = bars + 13;       // SAB_WARPS
-  uint64_t *ds_full = bars + 14;      // SAB_WARPS
-  uint64_t *dkv_full = bars + 15;
-  uint32_t *tmem_slot = (uint32_t *)(bars + 16);
+  uint64_t *kv_empty = bars + 1;
+  uint64_t *qd_full = bars + 2;       // [2]
+  uint64_t *qd_ready = bars + 4;      // [2]
+  uint64_t *qd_empty = bars + 6;      // [2]
+  uint64_t *st_full = bars + 8;       // [2]
+  uint64_t *st_empty = bars + 10;     // [2] SAB_WARPS
+  uint64_t *s_full = bars + 12;
+  uint64_t *dp_full = bars + 13;
+  uint64_t *p_full = bars + 14;       // SAB_WARPS
+  uint64_t *ds_full = bars + 15;      // SAB_WARPS
+  uint64_t *dkv_full = bars + 16;
+  uint64_t *info_full = bars + 17;    // [2]
+  uint64_t *info_empty = bars + 19;   // [2] all warps but the first
+  uint64_t *answered = bars + 21;
+  uint32_t *tmem_slot = (uint32_t *)(bars + 22);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {
@@ -134,19 +154,19 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     return;
   }
   const int group = p.H / p.KH;
-  const int bh = blockIdx.x % (p.B * p.KH);
-  const int kb = blockIdx.x / (p.B * p.KH);                       // the first keys, which most queries see under a causal mask, first
-  const int kh = bh % p.KH, b = bh / p.KH;
-  const int k0 = kb * SA_T, k1 = min(k0 + SA_T, p.S) - 1;
   const int nqt = (p.S + SA_T - 1) / SA_T;
 
-  // Set-up; the warp that sets up the barriers asks for K and V, and for the first query tile, before the others have met (see the forward)
   if (warp == 0) {
     if (lane == 0) {
       sa_prefetch_map(&tmK); sa_prefetch_map(&tmV); sa_prefetch_map(&tmQ); sa_prefetch_map(&tmDO);
       mbar_init(kv_full, 1);
-      for (int s = 0; s < 2; ++s) { mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], SAB_WARPS); }
+      mbar_init(kv_empty, 1);
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(&qd_full[s], 1); mbar_init(&qd_ready[s], 1); mbar_init(&qd_empty[s], 1); mbar_init(&st_full[s], 1); mbar_init(&st_empty[s], SAB_WARPS);
+        mbar_init(&info_full[s], 1); mbar_init(&info_empty[s], SAB_THREADS / 32 - 1);
+      }
       mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_full, SAB_WARPS); mbar_init(ds_full, SAB_WARPS); mbar_init(dkv_full, 1);
+      mbar_init(answered, 1);
       *abort_flag = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -156,54 +176,88 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_entry();
-  if (warp == 0 && lane == 0) {
-    mbar_expect_tx(kv_full, 2 * C::TILE);
-#pragma unroll
-    for (int c = 0; c < C::PANELS; ++c) {
-      tma_load_4d(smem_u32(smem + C::OFF_K + c * SA_PANEL), &tmK, kv_full, c * 64, k0, kh, b);
-      tma_load_4d(smem_u32(smem + C::OFF_V + c * SA_PANEL), &tmV, kv_full, c * 64, k0, kh, b);
-    }
-  }
-  __syncwarp();
-  // first and last query tile that see a key of the block: each warp finds them by itself
-  const int4 *summary = p.summary + (long long)b * nqt;
-  int i0 = 0x7fffffff, i1 = -1;
-  for (int i = lane; i < nqt; i += 32) {
-    const int4 s = summary[i];
-    if (s.x <= k1 && s.y >= k0) { i0 = min(i0, i); i1 = i; }
-  }
-  i0 = __reduce_min_sync(0xffffffffu, i0);
-  i1 = __reduce_max_sync(0xffffffffu, i1);
-  const int ni = i1 < 0 ? 0 : i1 - i0 + 1;
-  const int n = ni * group;                                       // steps: (head, query tile)
-  auto load_qd = [&](int it, int g, int i) {
-    const int s = it & 1;
-    mbar_expect_tx(&qd_full[s], 2 * C::TILE);
-#pragma unroll
-    for (int c = 0; c < C::PANELS; ++c) {
-      tma_load_4d(smem_u32(smem + C::OFF_Q + s * C::TILE + c * SA_PANEL), &tmQ, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
-      tma_load_4d(smem_u32(smem + C::OFF_DO + s * C::TILE + c * SA_PANEL), &tmDO, &qd_full[s], c * 64, i * SA_T, kh * group + g, b);
-    }
-  };
-  if (warp == 0 && lane == 0 && n > 0) load_qd(0, 0, i0);
-  __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  // The next block's (number, first query tile, query tiles), for the warps that follow the first one: false at the end
+  int turn = 0;
+  auto next_block = [&](int4 &t) -> bool {
+    const int s = turn & 1;
+    if (!sa_wait(&info_full[s], (uint32_t)(turn >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE)) return false;
+    t = info[s];
+    sa_warp_arrive(&info_empty[s], lane);
+    ++turn;
+    return t.x >= 0;
+  };
+
   // registers go from the warps that move data to the element-wise ones (128 x 64 + 512 x 104 = 640 x 96)
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {                      // the first step's tiles are under way
-      int g = 0, i = i0;
-      for (int it = 1; it < n; ++it) {
-        if (++i == i0 + ni) { i = i0; ++g; }
-        if (!mbar_wait(&qd_empty[it & 1], ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_PRODUCER)) break;
-        load_qd(it, g, i);
+    // ------------------------------------------------------------------ TMA producer; finds the next block while this one is worked on
+    int block = blockIdx.x, steps = 0, blocks = 0;        // steps: of all blocks so far; blocks: those with steps
+    bool ok = true;
+    while (true) {
+      int i0 = 0x7fffffff, i1 = -1;
+      const int s = turn & 1;
+      if (block >= 0) {                   // first and last query tile that see a key of the block
+        const DkvBlock k(p, block);
+        const int4 *summary = p.summary + (long long)k.b * nqt;
+        for (int i = lane; i < nqt; i += 32) {
+          const int4 t = summary[i];
+          if (t.x <= k.k1 && t.y >= k.k0) { i0 = min(i0, i); i1 = i; }
+        }
+        i0 = __reduce_min_sync(0xffffffffu, i0);
+        i1 = __reduce_max_sync(0xffffffffu, i1);
       }
+      const int ni = i1 < 0 ? 0 : i1 - i0 + 1;
+      ok = sa_wait(&info_empty[s], ((uint32_t)(turn >> 1) & 1u) ^ 1u, abort_flag, p, FFK_ERR_TIMEOUT_PRODUCER);
+      if (!ok) break;
+      if (lane == 0) {
+        info[s] = make_int4(block, i0, ni, 0);
+        mbar_arrive(&info_full[s]);
+      }
+      if (block < 0) break;
+      if (lane == 0) {
+        const DkvBlock k(p, block);
+        if (ni > 0) {
+          ok = mbar_wait(kv_empty, ((uint32_t)blocks & 1u) ^ 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_PRODUCER);
+          if (ok) {
+            mbar_expect_tx(kv_full, 2 * C::TILE);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c) {
+              tma_load_4d(smem_u32(smem + C::OFF_K + c * SA_PANEL), &tmK, kv_full, c * 64, k.k0, k.kh, k.b);
+              tma_load_4d(smem_u32(smem + C::OFF_V + c * SA_PANEL), &tmV, kv_full, c * 64, k.k0, k.kh, k.b);
+            }
+          }
+        }
+        int at = steps;
+        for (int g = 0; g < group && ok; ++g)
+          for (int i = i0; i < i0 + ni; ++i, ++at) {
+            ok = mbar_wait(&qd_empty[at & 1], ((uint32_t)(at >> 1) & 1u) ^ 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_PRODUCER);
+            if (!ok) break;
+            uint64_t *full = &qd_full[at & 1];
+            const uint32_t off = (uint32_t)((at & 1) * C::TILE);
+            mbar_expect_tx(full, 2 * C::TILE);
+#pragma unroll
+            for (int c = 0; c < C::PANELS; ++c) {
+              tma_load_4d(smem_u32(smem + C::OFF_Q + off + c * SA_PANEL), &tmQ, full, c * 64, i * SA_T, k.kh * group + g, k.b);
+              tma_load_4d(smem_u32(smem + C::OFF_DO + off + c * SA_PANEL), &tmDO, full, c * 64, i * SA_T, k.kh * group + g, k.b);
+            }
+          }
+        // asked for when the block's last tiles are on their way, two steps before its end: early enough to hide, and late enough that a
+        // CTA with a long block does not hold another one back (prompts, heads of 64: 79 us when asked for at the block's start, 58 without)
+        sa_ask_next(answer, answered);
+      }
+      // the answer is waited for even when a wait ran out: a write under way does not outlive its CTA
+      ok = sa_wait(answered, (uint32_t)turn & 1u, abort_flag, p, FFK_ERR_TIMEOUT_PRODUCER) && __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      steps += ni * group;
+      blocks += ni > 0;
+      block = sa_next_block(answer);
+      ++turn;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer: the whole warp runs, one lane issues
@@ -238,247 +292,273 @@ span_attn_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       __syncwarp();
     };
-    auto wait_qd = [&](int it) -> bool {
-      return mbar_wait_warp(&qd_full[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
-             mbar_wait_warp(&qd_ready[it & 1], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    auto wait_qd = [&](int at) -> bool {
+      return mbar_wait_warp(&qd_full[at & 1], (uint32_t)(at >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
+             mbar_wait_warp(&qd_ready[at & 1], (uint32_t)(at >> 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
     };
-    // also where no query sees a key: a load under way does not outlive its CTA
-    bool ok = mbar_wait_warp(kv_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && n > 0 && wait_qd(0);
-    if (ok) {
-      tc_fence_after();
-      issue_t(tmem_base + C::TM_S, dk, q_k0, s_full);
-      issue_t(tmem_base + C::TM_DP, dv, o_k0, dp_full);
-    }
-    for (int it = 0; it < n && ok; ++it) {
-      const uint32_t ph = (uint32_t)it & 1u, off = (uint32_t)((it & 1) * C::TILE), next = (uint32_t)(((it + 1) & 1) * C::TILE);
-      ok = mbar_wait_warp(p_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    bool ok = true;
+    int at = 0, blocks = 0;               // at: steps so far
+    int4 t;
+    while (ok && next_block(t)) {
+      const int n = t.z * group;
+      if (n == 0) continue;
+      ok = mbar_wait_warp(kv_full, (uint32_t)blocks & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) && wait_qd(at);
       if (!ok) break;
       tc_fence_after();
-      issue_g(tmem_base + C::TM_DV, tmem_base + C::TM_S, desc_advance(o_n0, off), it == 0);
-      if (it + 1 < n) {                   // the next scores take the columns that P^T is read from: products run in issue order
-        ok = wait_qd(it + 1);
+      const uint32_t off0 = (uint32_t)((at & 1) * C::TILE);
+      issue_t(tmem_base + C::TM_S, dk, desc_advance(q_k0, off0), s_full);
+      issue_t(tmem_base + C::TM_DP, dv, desc_advance(o_k0, off0), dp_full);
+      if (n == 1 && leader) tc_commit(kv_empty);
+      for (int it = 0; it < n; ++it, ++at) {
+        const uint32_t ph = (uint32_t)at & 1u, off = (uint32_t)((at & 1) * C::TILE), next = (uint32_t)(((at + 1) & 1) * C::TILE);
+        // the block before has been read out by the warps that now bring their probabilities
+        ok = mbar_wait_warp(p_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
         if (!ok) break;
         tc_fence_after();
-        issue_t(tmem_base + C::TM_S, dk, desc_advance(q_k0, next), s_full);
+        issue_g(tmem_base + C::TM_DV, tmem_base + C::TM_S, desc_advance(o_n0, off), it == 0);
+        if (it + 1 < n) {                 // the next scores take the columns that P^T is read from: products run in issue order
+          ok = wait_qd(at + 1);
+          if (!ok) break;
+          tc_fence_after();
+          issue_t(tmem_base + C::TM_S, dk, desc_advance(q_k0, next), s_full);
+        }
+        ok = mbar_wait_warp(ds_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        issue_g(tmem_base + C::TM_DK, tmem_base + C::TM_DP, desc_advance(q_n0, off), it == 0);
+        if (leader) tc_commit(&qd_empty[at & 1]);
+        __syncwarp();
+        if (it + 1 < n) issue_t(tmem_base + C::TM_DP, dv, desc_advance(o_k0, next), dp_full);
+        if (it + 2 == n && leader) tc_commit(kv_empty);
       }
-      ok = mbar_wait_warp(ds_full, ph, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
       if (!ok) break;
-      tc_fence_after();
-      issue_g(tmem_base + C::TM_DK, tmem_base + C::TM_DP, desc_advance(q_n0, off), it == 0);
-      if (leader) tc_commit(&qd_empty[it & 1]);
+      if (leader) tc_commit(dkv_full);
       __syncwarp();
-      if (it + 1 < n) issue_t(tmem_base + C::TM_DP, dv, desc_advance(o_k0, next), dp_full);
+      ++blocks;
     }
-    if (ok && leader) tc_commit(dkv_full);
-    __syncwarp();
   } else if (warp == 2) {
     // ------------------------------------------------------------------ rows of Q and dO that see none of these keys
     bool ok = true;
-    int i = i0;
-    for (int it = 0; it < n && ok; ++it) {
-      const int s = it & 1;
-      const int4 all = summary[i];
-      uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-      if (all.z > k0 || all.w < k1) {
+    int at = 0;
+    int4 t;
+    while (ok && next_block(t)) {
+      const DkvBlock k(p, t.x);
+      const int4 *summary = p.summary + (long long)k.b * nqt;
+      for (int g = 0; g < group && ok; ++g)
+        for (int i = t.y; i < t.y + t.z; ++i, ++at) {
+          const int s = at & 1;
+          const int4 all = summary[i];
+          uint32_t keep[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+          if (all.z > k.k0 || all.w < k.k1) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int q = i * SA_T + w * 32 + lane;
-          bool sees = true;                                       // rows behind the sequence arrive as zeros
-          if (q < p.S) {
-            const int2 sp = sa_span(p, b, q);
-            sees = sp.x <= sp.y && sp.x <= k1 && sp.y >= k0;
+            for (int w = 0; w < 4; ++w) {
+              const int q = i * SA_T + w * 32 + lane;
+              bool sees = true;                                   // rows behind the sequence arrive as zeros
+              if (q < p.S) {
+                const int2 sp = sa_span(p, k.b, q);
+                sees = sp.x <= sp.y && sp.x <= k.k1 && sp.y >= k.k0;
+              }
+              keep[w] = __ballot_sync(0xffffffffu, sees);
+            }
           }
-          keep[w] = __ballot_sync(0xffffffffu, sees);
+          ok = sa_wait(&qd_full[s], (uint32_t)(at >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+          if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
+            sa_clear_rows<C::PANELS>(smem + C::OFF_Q + s * C::TILE, keep, lane);
+            sa_clear_rows<C::PANELS>(smem + C::OFF_DO + s * C::TILE, keep, lane);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          sa_warp_arrive(&qd_ready[s], lane);
         }
-      }
-      ok = sa_wait(&qd_full[s], (uint32_t)(it >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
-      if (!ok) break;
-      if ((keep[0] & keep[1] & keep[2] & keep[3]) != 0xffffffffu) {
-        sa_clear_rows<C::PANELS>(smem + C::OFF_Q + s * C::TILE, keep, lane);
-        sa_clear_rows<C::PANELS>(smem + C::OFF_DO + s * C::TILE, keep, lane);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      }
-      sa_warp_arrive(&qd_ready[s], lane);
-      if (++i == i0 + ni) i = i0;
     }
-  } else if (warp == 3) {
+  } else {
     // ------------------------------------------------------------------ statistics of each query tile
     bool ok = true;
-    int g = 0, i = i0;
-    for (int it = 0; it < n && ok; ++it) {
-      const int s = it & 1;
-      float *lse = (float *)(smem + C::OFF_LSE) + s * SA_T, *dlt = (float *)(smem + C::OFF_DELTA) + s * SA_T;
-      int2 *sp = (int2 *)(smem + C::OFF_SPAN) + s * SA_T;
-      const long long base = ((long long)b * p.H + kh * group + g) * p.S;
-      float vl[4], vd[4];
-      int2 vs[4];
+    int at = 0;
+    int4 t;
+    while (ok && next_block(t)) {
+      const DkvBlock k(p, t.x);
+      for (int g = 0; g < group && ok; ++g)
+        for (int i = t.y; i < t.y + t.z; ++i, ++at) {
+          const int s = at & 1;
+          float *lse = (float *)(smem + C::OFF_LSE) + s * SA_T, *dlt = (float *)(smem + C::OFF_DELTA) + s * SA_T;
+          int2 *sp = (int2 *)(smem + C::OFF_SPAN) + s * SA_T;
+          const long long base = ((long long)k.b * p.H + k.kh * group + g) * p.S;
+          float vl[4], vd[4];
+          int2 vs[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int q = i * SA_T + r * 32 + lane;
-        // a query that sees nothing, or does not exist: probabilities of 0
-        vl[r] = INFINITY; vd[r] = 0.f; vs[r] = make_int2(1, 0);
-        if (q < p.S) {
-          const int2 t = sa_span(p, b, q);
-          if (t.x <= t.y) {
-            vs[r] = t;
-            vl[r] = p.lse[base + q];
-            vd[r] = p.delta[base + q];
+          for (int r = 0; r < 4; ++r) {
+            const int q = i * SA_T + r * 32 + lane;
+            // a query that sees nothing, or does not exist: probabilities of 0
+            vl[r] = INFINITY; vd[r] = 0.f; vs[r] = make_int2(1, 0);
+            if (q < p.S) {
+              const int2 u = sa_span(p, k.b, q);
+              if (u.x <= u.y) {
+                vs[r] = u;
+                vl[r] = p.lse[base + q];
+                vd[r] = p.delta[base + q];
+              }
+            }
           }
+          ok = sa_wait(&st_empty[s], ((uint32_t)(at >> 1) & 1u) ^ 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            lse[r * 32 + lane] = vl[r];
+            dlt[r * 32 + lane] = vd[r];
+            sp[r * 32 + lane] = vs[r];
+            // rows behind the sequence count as seeing all: their probabilities are zeros
+            const bool there = i * SA_T + r * 32 + lane < p.S, sees = vs[r].x <= vs[r].y;
+            int4 u;
+            u.x = __reduce_min_sync(0xffffffffu, sees ? vs[r].x : 0x7fffffff);
+            u.y = __reduce_max_sync(0xffffffffu, sees ? vs[r].y : -1);
+            u.z = __reduce_max_sync(0xffffffffu, sees ? vs[r].x : there ? 0x7fffffff : -1);
+            u.w = __reduce_min_sync(0xffffffffu, sees ? vs[r].y : there ? -1 : 0x7fffffff);
+            if (lane == 0) *(int4 *)(smem + C::OFF_GROUP + (s * 4 + r) * 16) = u;
+          }
+          sa_warp_arrive(&st_full[s], lane);
         }
-      }
-      ok = sa_wait(&st_empty[s], ((uint32_t)(it >> 1) & 1u) ^ 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
-      if (!ok) break;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        lse[r * 32 + lane] = vl[r];
-        dlt[r * 32 + lane] = vd[r];
-        sp[r * 32 + lane] = vs[r];
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {       // rows behind the sequence count as seeing all: their probabilities are zeros
-        const bool there = i * SA_T + r * 32 + lane < p.S, sees = vs[r].x <= vs[r].y;
-        int4 t;
-        t.x = __reduce_min_sync(0xffffffffu, sees ? vs[r].x : 0x7fffffff);
-        t.y = __reduce_max_sync(0xffffffffu, sees ? vs[r].y : -1);
-        t.z = __reduce_max_sync(0xffffffffu, sees ? vs[r].x : there ? 0x7fffffff : -1);
-        t.w = __reduce_min_sync(0xffffffffu, sees ? vs[r].y : there ? -1 : 0x7fffffff);
-        if (lane == 0) *(int4 *)(smem + C::OFF_GROUP + (s * 4 + r) * 16) = t;
-      }
-      sa_warp_arrive(&st_full[s], lane);
-      if (++i == i0 + ni) { i = i0; ++g; }
     }
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ------------------------------------------------------------------ P^T and dS^T: thread = key x 32 of the tile's queries
     const int quarter = warp & 3, cols = (warp - 4) >> 2;
-    const int r = quarter * 32 + lane, key = k0 + r, kw = k0 + quarter * 32;
+    const int r = quarter * 32 + lane;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(cols * 32);
     const pair32 ff = pair_of(p.factor, p.factor);
     bool ok = true;
-    int g = 0, i = i0;
-    for (int it = 0; it < n && ok; ++it) {
-      const int s = it & 1;
-      const uint32_t ph = (uint32_t)it & 1u;
-      const float *lse = (const float *)(smem + C::OFF_LSE) + s * SA_T + cols * 32, *dlt = (const float *)(smem + C::OFF_DELTA) + s * SA_T + cols * 32;
-      const int4 *sp = (const int4 *)(smem + C::OFF_SPAN) + (s * SA_T + cols * 32) / 2;       // two spans each
-      ok = sa_wait(&st_full[s], (uint32_t)(it >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE) &&
-           sa_wait(s_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
-      if (!ok) break;
-      tc_fence_after();
-      // how this warp's 32 keys are seen by its 32 queries
-      const int4 seen = *(const int4 *)(smem + C::OFF_GROUP + (s * 4 + cols) * 16);
-      const bool none = seen.x > kw + 31 || seen.y < kw, masked = seen.z > kw || seen.w < kw + 31;
-      uint32_t y[32], pk[16];
-      if (none) {
+    int at = 0, blocks = 0;
+    int4 t;
+    while (ok && next_block(t)) {
+      const DkvBlock k(p, t.x);
+      const int key = k.k0 + r, kw = k.k0 + quarter * 32;
+      for (int g = 0; g < group && ok; ++g) {
+        const float slope = BIAS ? p.slopes[k.kh * group + g] : 0.f;
+        for (int i = t.y; i < t.y + t.z; ++i, ++at) {
+          const int s = at & 1;
+          const uint32_t ph = (uint32_t)at & 1u;
+          const float *lse = (const float *)(smem + C::OFF_LSE) + s * SA_T + cols * 32, *dlt = (const float *)(smem + C::OFF_DELTA) + s * SA_T + cols * 32;
+          const int4 *sp = (const int4 *)(smem + C::OFF_SPAN) + (s * SA_T + cols * 32) / 2;       // two spans each
+          ok = sa_wait(&st_full[s], (uint32_t)(at >> 1) & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE) &&
+               sa_wait(s_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+          tc_fence_after();
+          // how this warp's 32 keys are seen by its 32 queries
+          const int4 seen = *(const int4 *)(smem + C::OFF_GROUP + (s * 4 + cols) * 16);
+          const bool none = seen.x > kw + 31 || seen.y < kw, masked = seen.z > kw || seen.w < kw + 31;
+          uint32_t y[32], pk[16];
+          if (none) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) pk[c] = 0u;
-      } else {
-        tmem_ld32(lane_base + C::TM_S, y);
-        tmem_ld_wait();
-        if (CAP && masked) {              // masked scores do not choose the way tanh is taken
+            for (int c = 0; c < 16; ++c) pk[c] = 0u;
+          } else {
+            tmem_ld32(lane_base + C::TM_S, y);
+            tmem_ld_wait();
+            if (CAP && masked) {              // masked scores do not choose the way tanh is taken
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const int4 t = sp[c / 2];
-            if (key < t.x || key > t.y) y[c] = 0u;
-            if (key < t.z || key > t.w) y[c + 1] = 0u;
-          }
-        }
-        if constexpr (CAP) {
-          if (!sa_cap(y, p, true)) sa_cap_any(y, p);
-        }
-        const int qg = i * SA_T + cols * 32;
-        SaBias bias(BIAS ? p.slopes[kh * group + g] : 0.f, (float)(qg - key), qg >= kw + 31 ? 1 : qg + 31 <= kw ? -1 : 0);
-#pragma unroll
-        for (int c = 0; c < 32; c += 16) {
-          float e[16];
-#pragma unroll
-          for (int u = 0; u < 16; u += 4) {
-            const float4 w = *reinterpret_cast<const float4 *>(lse + c + u);
-            pair32 w0 = pair_of(-w.x, -w.y), w1 = pair_of(-w.z, -w.w);
-            if constexpr (BIAS) { w0 = bias.next(w0); w1 = bias.next(w1); }
-            pair_to(pair_fma(pair_get(&y[c + u]), ff, w0), e[u], e[u + 1]);
-            pair_to(pair_fma(pair_get(&y[c + u + 2]), ff, w1), e[u + 2], e[u + 3]);
-          }
-          if (masked) {
-#pragma unroll
-            for (int u = 0; u < 16; u += 2) {
-              const int4 t = sp[(c + u) / 2];
-              if (key < t.x || key > t.y) e[u] = -INFINITY;
-              if (key < t.z || key > t.w) e[u + 1] = -INFINITY;
+              for (int c = 0; c < 32; c += 2) {
+                const int4 t = sp[c / 2];
+                if (key < t.x || key > t.y) y[c] = 0u;
+                if (key < t.z || key > t.w) y[c + 1] = 0u;
+              }
             }
-          }
-#pragma unroll
-          for (int u = 0; u < 16; ++u) e[u] = sa_exp2(e[u]);
-#pragma unroll
-          for (int u = 0; u < 16; u += 2) pk[(c + u) >> 1] = pack_bf162(e[u], e[u + 1]);
-          // what dS needs of P: times the cap's derivative
-#pragma unroll
-          for (int u = 0; u < 16; u += 2) {
             if constexpr (CAP) {
-              sa_times_slope(y, c + u, e[u], e[u + 1], p.to_z);
-            } else {
-              y[c + u] = __float_as_uint(e[u]);
-              y[c + u + 1] = __float_as_uint(e[u + 1]);
+              if (!sa_cap(y, p, true)) sa_cap_any(y, p);
+            }
+            const int qg = i * SA_T + cols * 32;
+            SaBias bias(slope, (float)(qg - key), qg >= kw + 31 ? 1 : qg + 31 <= kw ? -1 : 0);
+#pragma unroll
+            for (int c = 0; c < 32; c += 16) {
+              float e[16];
+#pragma unroll
+              for (int u = 0; u < 16; u += 4) {
+                const float4 w = *reinterpret_cast<const float4 *>(lse + c + u);
+                pair32 w0 = pair_of(-w.x, -w.y), w1 = pair_of(-w.z, -w.w);
+                if constexpr (BIAS) { w0 = bias.next(w0); w1 = bias.next(w1); }
+                pair_to(pair_fma(pair_get(&y[c + u]), ff, w0), e[u], e[u + 1]);
+                pair_to(pair_fma(pair_get(&y[c + u + 2]), ff, w1), e[u + 2], e[u + 3]);
+              }
+              if (masked) {
+#pragma unroll
+                for (int u = 0; u < 16; u += 2) {
+                  const int4 t = sp[(c + u) / 2];
+                  if (key < t.x || key > t.y) e[u] = -INFINITY;
+                  if (key < t.z || key > t.w) e[u + 1] = -INFINITY;
+                }
+              }
+#pragma unroll
+              for (int u = 0; u < 16; ++u) e[u] = sa_exp2(e[u]);
+#pragma unroll
+              for (int u = 0; u < 16; u += 2) pk[(c + u) >> 1] = pack_bf162(e[u], e[u + 1]);
+              // what dS needs of P: times the cap's derivative
+#pragma unroll
+              for (int u = 0; u < 16; u += 2) {
+                if constexpr (CAP) {
+                  sa_times_slope(y, c + u, e[u], e[u + 1], p.to_z);
+                } else {
+                  y[c + u] = __float_as_uint(e[u]);
+                  y[c + u + 1] = __float_as_uint(e[u + 1]);
+                }
+              }
             }
           }
-        }
-      }
-      sa_tmem_st16(lane_base + C::TM_S, pk);
-      tmem_st_wait();
-      tc_fence_before();
-      sa_warp_arrive(p_full, lane);
-      ok = sa_wait(dp_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
-      if (!ok) break;
-      tc_fence_after();
-      if (!none) {
-        uint32_t z[32];
-        tmem_ld32(lane_base + C::TM_DP, z);
-        tmem_ld_wait();
+          sa_tmem_st16(lane_base + C::TM_S, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          sa_warp_arrive(p_full, lane);
+          ok = sa_wait(dp_full, ph, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+          if (!ok) break;
+          tc_fence_after();
+          if (!none) {
+            uint32_t z[32];
+            tmem_ld32(lane_base + C::TM_DP, z);
+            tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 w = *reinterpret_cast<const float4 *>(dlt + c);
-          float v[4];
-          pair_to(pair_mul(pair_get(&y[c]), pair_add(pair_get(&z[c]), pair_of(-w.x, -w.y))), v[0], v[1]);
-          pair_to(pair_mul(pair_get(&y[c + 2]), pair_add(pair_get(&z[c + 2]), pair_of(-w.z, -w.w))), v[2], v[3]);
-          if (masked) {
+            for (int c = 0; c < 32; c += 4) {
+              const float4 w = *reinterpret_cast<const float4 *>(dlt + c);
+              float v[4];
+              pair_to(pair_mul(pair_get(&y[c]), pair_add(pair_get(&z[c]), pair_of(-w.x, -w.y))), v[0], v[1]);
+              pair_to(pair_mul(pair_get(&y[c + 2]), pair_add(pair_get(&z[c + 2]), pair_of(-w.z, -w.w))), v[2], v[3]);
+              if (masked) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (__uint_as_float(y[c + u]) == 0.f) v[u] = 0.f;                 // whatever dO and delta hold there
+                for (int u = 0; u < 4; ++u)
+                  if (__uint_as_float(y[c + u]) == 0.f) v[u] = 0.f;                 // whatever dO and delta hold there
+              }
+              pk[c >> 1] = pack_bf162(v[0], v[1]);
+              pk[(c >> 1) + 1] = pack_bf162(v[2], v[3]);
+            }
           }
-          pk[c >> 1] = pack_bf162(v[0], v[1]);
-          pk[(c >> 1) + 1] = pack_bf162(v[2], v[3]);
+          sa_tmem_st16(lane_base + C::TM_DP, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          sa_warp_arrive(ds_full, lane);
+          if (lane == 0) mbar_arrive(&st_empty[s]);
         }
       }
-      sa_tmem_st16(lane_base + C::TM_DP, pk);
-      tmem_st_wait();
-      tc_fence_before();
-      sa_warp_arrive(ds_full, lane);
-      if (lane == 0) mbar_arrive(&st_empty[s]);
-      if (++i == i0 + ni) { i = i0; ++g; }
-    }
-    if (ok && n > 0) {
-      ok = sa_wait(dkv_full, 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
-      tc_fence_after();
-    }
-    if (ok) {
-      // eight warps store dK, eight dV, through the places of Q and dO: the last products have read those
+      if (!ok) break;
+      // eight warps store dK, eight dV, a thread half of its key's columns
+      if (t.z > 0) {
+        ok = sa_wait(dkv_full, (uint32_t)blocks & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+        if (!ok) break;
+        tc_fence_after();
+        ++blocks;
+      }
       constexpr int DH = DT / 2;
-      const int w = cols & 1, half = cols >> 1;
-      uint8_t *tile = smem + (w == 0 ? C::OFF_Q : C::OFF_DO);
+      const int w = cols & 1, col = (cols >> 1) * DH;
+      const long long row = (long long)k.b * p.S + key;
+      bf16 *out = (w == 0 ? p.dK + row * p.lddk : p.dV + row * p.lddv) + (long long)k.kh * p.D + col;
 #pragma unroll 1
-      for (int c = 0; c < DH / 32; ++c) {
+      for (int c = 0; c < DH; c += 32) {
         uint32_t o[32];
-        if (n > 0) {
-          tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((w == 0 ? C::TM_DK : C::TM_DV) + half * DH + c * 32), o);
+        if (t.z > 0) {
+          tmem_ld32(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)((w == 0 ? C::TM_DK : C::TM_DV) + col + c), o);
           tmem_ld_wait();
         } else {
 #pragma unroll
           for (int u = 0; u < 32; ++u) o[u] = 0u;
         }
-        sa_tile_row(tile, r, half * DH + c * 32, o, w == 0 ? p.scale : 1.f);
+        if (key < p.S) sa_store_row(out + c, o, w == 0 ? p.scale : 1.f, p.D - col - c, p.wide);
       }
-      sa_tile_out<C::PANELS>(tile, w == 0 ? &tmDK : &tmDV, k0, kh, b, 1 + w, 256, warp == 4 + 4 * w && lane == 0);
       tc_fence_before();
     }
   }
@@ -839,7 +919,7 @@ span_attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   }
 }
 
-struct SpanMaps { CUtensorMap q, k, v, dout, dq, dk, dv; };
+struct SpanMaps { CUtensorMap q, k, v, dout, dq; };
 
 template <int DT, bool CAP, bool BIAS>
 int launch_bwd(const SpanMaps &m, const SpanArgs &a, cudaStream_t st) {
@@ -849,8 +929,7 @@ int launch_bwd(const SpanMaps &m, const SpanArgs &a, cudaStream_t st) {
   e = ffk_allow_smem(span_attn_dq_kernel<DT, CAP, BIAS>, DqCfg<DT>::SMEM, done_q);
   if (e != cudaSuccess) return (int)e;
   const long long tiles = (a.S + SA_T - 1) / SA_T;
-  int r = ffk_launch(span_attn_dkv_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.KH), SAB_THREADS, DkvCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, m.dk, m.dv,
-                     a);
+  int r = ffk_launch(span_attn_dkv_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.KH), SAB_THREADS, DkvCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, a);
   if (r) return r;
   return ffk_launch(span_attn_dq_kernel<DT, CAP, BIAS>, (unsigned)(tiles * a.B * a.H), SAB_THREADS, DqCfg<DT>::SMEM, st, m.q, m.k, m.v, m.dout, m.dq, a);
 }
@@ -881,14 +960,14 @@ FFK_API int ffk_span_attention_bwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
   if ((r = sa_head_map(&m.v, d->V, d->D, d->S, d->ldv, d->KH, d->B))) return r;
   if ((r = sa_head_map(&m.dout, d->dO, d->D, d->S, d->lddo, d->H, d->B))) return r;
   if ((r = sa_head_map(&m.dq, d->dQ, d->D, d->S, d->lddq, d->H, d->B))) return r;
-  if ((r = sa_head_map(&m.dk, d->dK, d->D, d->S, d->lddk, d->KH, d->B))) return r;
-  if ((r = sa_head_map(&m.dv, d->dV, d->D, d->S, d->lddv, d->KH, d->B))) return r;
   SpanArgs a = {};
   sa_args(d, a, ffk_span_attention_err());
   float *delta = d->scratch;
   int4 *summary = reinterpret_cast<int4 *>(d->scratch + delta_floats(d->B, d->H, d->S));
   a.delta = delta;
   a.summary = summary;
+  a.dK = (bf16 *)d->dK; a.lddk = d->lddk; a.dV = (bf16 *)d->dV; a.lddv = d->lddv;
+  a.wide = sa_wide(d->dK, d->lddk, d->D) && sa_wide(d->dV, d->lddv, d->D);
   FfkTraffic traffic((long long)d->B * d->S * d->D * 4 * (d->H + d->KH));
   const unsigned blocks = (unsigned)(delta_blocks + sum_blocks);
   r = lanes == 8 ? ffk_launch(span_attn_prep_kernel<8>, blocks, 256, 0, st, (const bf16 *)d->dO, d->lddo, (const bf16 *)d->O, d->ldo, delta, summary,
