@@ -52,7 +52,6 @@ struct SpanArgs {
   bf16 *dQ, *dK, *dV;
   long long lddq, lddk, lddv;
   int wide;                        // results' rows lie on 32-byte boundaries
-  int tiles;                       // forward: 128-query tiles of a CTA, 1 or 2
   int *err;
 };
 

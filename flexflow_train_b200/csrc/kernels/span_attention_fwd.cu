@@ -1,43 +1,51 @@
 // span_attention_fwd.cu -- forward pass of attention over spans of keys (span_attention.cuh has the mathematics).
 //
-// A CTA (384 threads) takes one or two tiles of 128 queries of one (batch row, head) and walks over the key tiles from the first
-// to the last that any of its queries sees; scores and probabilities exist in tensor memory and registers only:
-//   warp 0      TMA producer: Q once, then the K and V tiles through rings
-//   warp 1      MMA issuer: S_t = Q_t K_j^T (two products ahead of nothing but the other tile's softmax), O_t += P_t V_j
+// A CTA (256 threads, two of them on an SM) takes 128 queries of one (batch row, head) and walks over the key tiles from the first to the
+// last that any of them sees; scores and probabilities exist in tensor memory and registers only:
+//   warp 0      TMA producer: Q once, then the K and V tiles
+//   warp 1      MMA issuer: S = Q K_j^T, O += P V_j
 //   warp 2      clears the rows of V_j that no query of the CTA sees (only where a tile holds such rows)
-//   warps 4-11  softmax, thread = query row: four warps per query tile.  P_t overwrites the first columns of S_t as bf16 and is the A operand of
-//               the second product from there.  The reference maximum of a row moves only when the true one has grown by 2^8, and then the
-//               thread rescales its row of O in tensor memory: the common step has no correction pass.
-// While one tile's softmax runs, the tensor core works on the other tile's products.
+//   warps 4-7   softmax, thread = query row.  P overwrites the first columns of S as bf16 and is the A operand of the second product from
+//               there.  The reference maximum of a row moves only when the true one has grown by 2^8, and then the thread rescales its row
+//               of O in tensor memory: the common step has no correction pass.
+// P is rounded to bf16, the type that the second product takes; its sum l is taken of the unrounded values in fp32, O is rounded once.
+//
+// What bounds it: per SM and pair of tiles (128 x 128 x 128 each) the tensor core takes 2048 cycles for both CTAs' products, the exponentials
+// 2048 of the special-function unit, and within a tile the one waits for the other; a cap adds about as much of the FMA pipe.  Two CTAs an SM
+// fill each other's waits, also where one sets up or writes its result, which a CTA of a few tiles spends a third of its time on, and balance
+// spans of uneven lengths by 128 queries.  They hold half of the tensor memory and, with heads of 128, one K and one V tile each: K_j+1 arrives
+// under the softmax of tile j, V_j+1 under that of j + 1.  Against one CTA with two query tiles and rings of two and three, K and V read
+// once for both (both on the same device in turn): 8192 causal, 16 heads of 128, cap: 339 -> 329 us (835 TFLOP/s), without a cap 244 -> 255
+// (1080); 8 x 2048 in documents of about 700, 16 heads of 128, cap: 189 -> 162; 8 x 1024 with prompts, heads of 64, bias: 49 -> 41; 4 x 1001
+// causal, bias: 41 -> 35.
 //
 // Every wait is bounded (tcgen05.cuh).
 #include "span_attention.cuh"
 
 namespace {
 
-constexpr int SAF_THREADS = 384;
+constexpr int SAF_THREADS = 256;
 constexpr float SAF_GAP = 8.f;          // log-2 units by which a row's maximum may exceed the reference in use
 
 template <int DT>                       // columns of a tile: 64 or 128
 struct SafCfg {
   static constexpr int PANELS = DT / 64;
   static constexpr int TILE = SA_T * DT * 2;
-  static constexpr int NK = 2, NV = DT == 128 ? 3 : 4;
+  static constexpr int NK = DT == 128 ? 1 : 2, NV = NK;
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_K = OFF_Q + 2 * TILE;
+  static constexpr int OFF_K = OFF_Q + TILE;
   static constexpr int OFF_V = OFF_K + NK * TILE;
-  static constexpr int OFF_SPAN = OFF_V + NV * TILE;              // [256] int2
-  static constexpr int OFF_RANGE = OFF_SPAN + 256 * 8;            // [8] int2: smallest first and largest last of 32 rows
-  static constexpr int OFF_BAR = OFF_RANGE + 64;
-  static constexpr int SMEM = OFF_BAR + 256 + 640;                // the base is aligned to 1024 (checked in the kernel)
-  static constexpr int SLACK = 640;
-  static_assert(SMEM <= 232448, "tiles exceed the shared memory of a CTA");
-  static constexpr int TM_S = 0;                                  // S_t at t * 128
-  static constexpr int TM_O = 256;                                // O_t at 256 + t * DT
+  static constexpr int OFF_SPAN = OFF_V + NV * TILE;              // [128] int2
+  static constexpr int OFF_RANGE = OFF_SPAN + SA_T * 8;           // [4] int2: smallest first and largest last of 32 rows
+  static constexpr int OFF_BAR = OFF_RANGE + 32;
+  static constexpr int SLACK = 1024;                              // the base is aligned to that (checked in the kernel)
+  static constexpr int SMEM = OFF_BAR + 128 + SLACK;
+  static_assert(SMEM <= 233472 / 2 - 1024, "two CTAs do not fit an SM");
+  static constexpr int TM_S = 0, TM_O = 128, TM_COLS = 256;       // columns of tensor memory: half of the SM's
 };
 
 template <int DT, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(SAF_THREADS, 1)
+__global__ void __launch_bounds__(SAF_THREADS, 2)
 span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const __grid_constant__ CUtensorMap tmO, const SpanArgs p) {
   using C = SafCfg<DT>;
@@ -46,16 +54,16 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   int2 *span = (int2 *)(smem + C::OFF_SPAN);
   int2 *range = (int2 *)(smem + C::OFF_RANGE);
   uint64_t *bars = (uint64_t *)(smem + C::OFF_BAR);
-  uint64_t *q_full = bars;            // [2]
-  uint64_t *k_full = bars + 2;        // [NK]
-  uint64_t *k_empty = bars + 4;       // [NK]
-  uint64_t *v_full = bars + 6;        // [NV]
+  uint64_t *q_full = bars;
+  uint64_t *s_full = bars + 1;
+  uint64_t *p_full = bars + 2;        // four warps
+  uint64_t *o_full = bars + 3;
+  uint64_t *k_full = bars + 4;        // [NK]
+  uint64_t *k_empty = bars + 6;       // [NK]
+  uint64_t *v_full = bars + 8;        // [NV]
   uint64_t *v_ready = bars + 10;      // [NV]
-  uint64_t *v_empty = bars + 14;      // [NV]
-  uint64_t *s_full = bars + 18;       // [2]
-  uint64_t *p_full = bars + 20;       // [2] four warps
-  uint64_t *o_full = bars + 22;       // [2]
-  uint32_t *tmem_slot = (uint32_t *)(bars + 24);
+  uint64_t *v_empty = bars + 12;      // [NV]
+  uint32_t *tmem_slot = (uint32_t *)(bars + 14);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if ((uintptr_t)(smem - smem_raw) > (uintptr_t)C::SLACK) {      // the launch did not leave room to align the tiles: refuse
@@ -64,19 +72,18 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     return;
   }
   // the query blocks of all heads in turn, the last ones (which see most keys under a causal mask) first
-  const int rows_cta = SA_T * p.tiles;
-  const int nqb = (p.S + rows_cta - 1) / rows_cta;
+  const int nqb = (p.S + SA_T - 1) / SA_T;
   const int bh = blockIdx.x % (p.B * p.H);
   const int qb = nqb - 1 - blockIdx.x / (p.B * p.H);
   const int h = bh % p.H, b = bh / p.H, kh = h / (p.H / p.KH);
-  const int q0 = qb * rows_cta;
+  const int q0 = qb * SA_T;
 
   // Set-up, as far as it does not touch global memory under the previous kernel's tail.  The warp that sets up the barriers asks for Q before
   // the others have met: a CTA is a few tiles long, and its first products wait for these loads.
   if (warp == 0) {
     if (lane == 0) {
       sa_prefetch_map(&tmQ); sa_prefetch_map(&tmK); sa_prefetch_map(&tmV);
-      for (int s = 0; s < 2; ++s) { mbar_init(&q_full[s], 1); mbar_init(&s_full[s], 1); mbar_init(&p_full[s], 4); mbar_init(&o_full[s], 1); }
+      mbar_init(q_full, 1); mbar_init(s_full, 1); mbar_init(p_full, 4); mbar_init(o_full, 1);
       for (int s = 0; s < C::NK; ++s) { mbar_init(&k_full[s], 1); mbar_init(&k_empty[s], 1); }
       for (int s = 0; s < C::NV; ++s) { mbar_init(&v_full[s], 1); mbar_init(&v_ready[s], 1); mbar_init(&v_empty[s], 1); }
       *abort_flag = 0;
@@ -84,54 +91,41 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
     __syncwarp();
   } else if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)C::TM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_entry();
-  const bool has0 = q0 < p.S, has1 = p.tiles == 2 && q0 + SA_T < p.S;       // query tiles with a row
   if (warp == 0 && lane == 0) {
+    mbar_expect_tx(q_full, C::TILE);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (t == 0 ? has0 : has1) {
-        mbar_expect_tx(&q_full[t], C::TILE);
-#pragma unroll
-        for (int c = 0; c < C::PANELS; ++c)
-          tma_load_4d(smem_u32(smem + C::OFF_Q + t * C::TILE + c * SA_PANEL), &tmQ, &q_full[t], c * 64, q0 + t * SA_T, h, b);
-      }
+    for (int c = 0; c < C::PANELS; ++c) tma_load_4d(smem_u32(smem + C::OFF_Q + c * SA_PANEL), &tmQ, q_full, c * 64, q0, h, b);
   }
   __syncwarp();
   // spans of the CTA's queries, and what each 32 of them see together
-  if (threadIdx.x >= 64 && threadIdx.x < 320) {
-    const int r = (int)threadIdx.x - 64, q = q0 + r;
+  if (warp >= 4) {
+    const int r = (int)threadIdx.x - 128, q = q0 + r;
     int2 s = make_int2(1, 0);
-    if (r < rows_cta && q < p.S) s = sa_span(p, b, q);
+    if (q < p.S) s = sa_span(p, b, q);
     span[r] = s;
     const bool sees = s.x <= s.y;
     const int lo = __reduce_min_sync(0xffffffffu, sees ? s.x : 0x7fffffff), hi = __reduce_max_sync(0xffffffffu, sees ? s.y : -1);
-    if (lane == 0) range[warp - 2] = make_int2(lo, hi);
+    if (lane == 0) range[warp - 4] = make_int2(lo, hi);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // key tiles of each query tile: from[t] .. to[t], none where from > to
-  int from[2], to[2];
+  // key tiles that any of the queries sees: j0 to j0 + n - 1
+  int j0 = 0x7fffffff, j1 = -1;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    int lo = 0x7fffffff, hi = -1;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) { lo = min(lo, range[t * 4 + w].x); hi = max(hi, range[t * 4 + w].y); }
-    from[t] = hi < 0 ? 1 : lo / SA_T;
-    to[t] = hi < 0 ? 0 : hi / SA_T;
-  }
-  const bool any0 = from[0] <= to[0], any1 = from[1] <= to[1];
-  const int j0 = any0 ? (any1 ? min(from[0], from[1]) : from[0]) : from[1];
-  const int j1 = any0 ? (any1 ? max(to[0], to[1]) : to[0]) : to[1];
-  const int n = j1 - j0 + 1;               // 0 where no query sees a key
+  for (int w = 0; w < 4; ++w) { j0 = min(j0, range[w].x); j1 = max(j1, range[w].y); }
+  const int n = j1 < 0 ? 0 : j1 / SA_T - j0 / SA_T + 1;
+  j0 = n > 0 ? j0 / SA_T : 0;
 
-  // the softmax warps hold a row of scores each: registers go from the four warps that move data to them (128 x 88 + 256 x 208 = 384 x 168)
+  // the softmax warps hold a row of scores each: registers go from the four warps that move data to them (128 x 72 + 128 x 184 = 256 x
+  // 128; splits from 48 / 208 to this one take the same time within 2 %)
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0 && n > 0) {
@@ -184,84 +178,52 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int ksteps = (p.D + 15) / 16;                                   // of Q K^T; the columns beyond D are zeros
     const uint32_t id_s = sa_idesc(128, SA_T, 0, 0), id_o = sa_idesc(128, ksteps * 16, 0, 1);
     bool ok = true;
-    // i: number of the key tile in the walk.  S_t overwrites the buffer that P_t(i - 1) was read from: products run in issue order
-    auto issue_s = [&](int t, int i) {
+    // S overwrites the columns that P was read from: products run in issue order
+    auto issue_s = [&](int i) {
       if (leader) {
-        const uint64_t a = desc_advance(dq0, (uint32_t)(t * C::TILE)), k = desc_advance(dk0, (uint32_t)((i % C::NK) * C::TILE));
-        const uint32_t d = tmem_base + (uint32_t)(C::TM_S + t * SA_T);
-        tc_mma_bf16<false>(d, a, k, id_s);
+        const uint64_t k = desc_advance(dk0, (uint32_t)((i % C::NK) * C::TILE));
+        const uint32_t d = tmem_base + (uint32_t)C::TM_S;
+        tc_mma_bf16<false>(d, dq0, k, id_s);
 #pragma unroll
         for (int s = 1; s < DT / 16; ++s) {
           if (s >= ksteps) break;         // unrolled: the one lane that issues bounds the tensor core otherwise
           const uint32_t off = (uint32_t)((s >> 2) * SA_PANEL + (s & 3) * 32);
-          tc_mma_bf16<true>(d, desc_advance(a, off), desc_advance(k, off), id_s);
+          tc_mma_bf16<true>(d, desc_advance(dq0, off), desc_advance(k, off), id_s);
         }
-        tc_commit(&s_full[t]);
+        tc_commit(s_full);
+        tc_commit(&k_empty[i % C::NK]);
       }
       __syncwarp();
     };
-    auto wait_k = [&](int i) -> bool { return mbar_wait_warp(&k_full[i % C::NK], (uint32_t)(i / C::NK) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA); };
-    // also where a tile's queries see nothing: a load under way does not outlive its CTA
-    if (has0) ok = mbar_wait_warp(&q_full[0], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
-    if (has1 && ok) ok = mbar_wait_warp(&q_full[1], 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
-    if (ok && n > 0) {
-      ok = wait_k(0);
-      if (ok) {
+    // also where the queries see nothing: a load under way does not outlive its CTA
+    ok = mbar_wait_warp(q_full, 0, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+    for (int i = 0; i <= n && ok; ++i) {
+      if (i > 0) {
+        const int at = (i - 1) % C::NV;
+        const uint32_t phase = (uint32_t)((i - 1) / C::NV) & 1u;
+        ok = mbar_wait_warp(&v_full[at], phase, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
+             mbar_wait_warp(&v_ready[at], phase, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
+             mbar_wait_warp(p_full, (uint32_t)(i - 1) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+        if (!ok) break;
         tc_fence_after();
+        if (leader) {
+          const uint64_t v = desc_advance(dv0, (uint32_t)(at * C::TILE));
+          const uint32_t d = tmem_base + (uint32_t)C::TM_O, a = tmem_base + (uint32_t)C::TM_S;
+          if (i == 1) tc_mma_ts_bf16<false>(d, a, v, id_o);
+          else tc_mma_ts_bf16<true>(d, a, v, id_o);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (from[t] == j0 && from[t] <= to[t]) issue_s(t, 0);
-        if (leader) tc_commit(&k_empty[0]);
-      }
-    }
-    uint32_t done[2] = {0, 0};              // products P V issued for each query tile
-    for (int i = 0; i < n && ok; ++i) {
-      const int j = j0 + i;
-      const bool more = i + 1 < n;
-      bool k_here = false, v_here = false;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (ok && j >= from[t] && j <= to[t]) {
-          if (!v_here) {
-            ok = mbar_wait_warp(&v_full[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA) &&
-                 mbar_wait_warp(&v_ready[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
-            v_here = true;
-          }
-          if (ok) ok = mbar_wait_warp(&p_full[t], done[t] & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
-          if (ok) {
-            tc_fence_after();
-            if (leader) {
-              const uint64_t v = desc_advance(dv0, (uint32_t)((i % C::NV) * C::TILE));
-              const uint32_t d = tmem_base + (uint32_t)(C::TM_O + t * DT), a = tmem_base + (uint32_t)(C::TM_S + t * SA_T);
-              if (done[t] == 0) tc_mma_ts_bf16<false>(d, a, v, id_o);
-              else tc_mma_ts_bf16<true>(d, a, v, id_o);
-#pragma unroll
-              for (int s = 1; s < SA_T / 16; ++s) tc_mma_ts_bf16<true>(d, a + (uint32_t)(s * 8), desc_advance(v, (uint32_t)(s * 2048)), id_o);
-              if (j == to[t]) tc_commit(&o_full[t]);
-            }
-            __syncwarp();
-            ++done[t];
-          }
+          for (int s = 1; s < SA_T / 16; ++s) tc_mma_ts_bf16<true>(d, a + (uint32_t)(s * 8), desc_advance(v, (uint32_t)(s * 2048)), id_o);
+          tc_commit(&v_empty[at]);
+          if (i == n) tc_commit(o_full);
         }
-        if (ok && more && j + 1 >= from[t] && j + 1 <= to[t]) {
-          if (!k_here) {
-            ok = wait_k(i + 1);
-            k_here = true;
-          }
-          if (ok) {
-            tc_fence_after();
-            issue_s(t, i + 1);
-          }
-        }
+        __syncwarp();
       }
-      // a key tile that neither query tile takes (between two documents) is waited for all the same: its stage is given back below
-      if (ok && !v_here) ok = mbar_wait_warp(&v_ready[i % C::NV], (uint32_t)(i / C::NV) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
-      if (ok && more && !k_here) ok = wait_k(i + 1);
-      if (ok && leader) {
-        tc_commit(&v_empty[i % C::NV]);
-        if (more) tc_commit(&k_empty[(i + 1) % C::NK]);
+      if (i < n) {
+        ok = mbar_wait_warp(&k_full[i % C::NK], (uint32_t)(i / C::NK) & 1u, abort_flag, p.err, FFK_ERR_TIMEOUT_MMA);
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(i);
       }
-      __syncwarp();
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ rows of V that nothing sees
@@ -270,7 +232,7 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const int k0 = (j0 + i) * SA_T;
       uint32_t keep[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < 4; ++r) {
         const int2 s = span[r * 32 + lane];
         if (s.x <= s.y) sa_add_bits(keep, s.x - k0, s.y - k0);
       }
@@ -286,25 +248,24 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ------------------------------------------------------------------ softmax: thread = query row
-    const int t = (warp - 4) >> 2, quarter = warp & 3;
+    const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int q = q0 + t * SA_T + r;
-    const int2 mine = span[t * SA_T + r];
+    const int q = q0 + r;
+    const int2 mine = span[r];
     const bool empty = mine.x > mine.y;
     // a row that sees nothing computes what it likes and stores zeros: it does not keep its warp from the unmasked path
     const int lo = empty ? -1 : mine.x, hi = empty ? 0x7ffffff0 : mine.y;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t t_s = lane_base + (uint32_t)(C::TM_S + t * SA_T), t_o = lane_base + (uint32_t)(C::TM_O + t * DT);
+    const uint32_t t_s = lane_base + (uint32_t)C::TM_S, t_o = lane_base + (uint32_t)C::TM_O;
     const float slope = BIAS ? p.slopes[h] / p.scale : 0.f;
     const int q_low = q - lane;            // the warp's first row
     float m = -INFINITY, l = 0.f;          // m: what the row's exponentials are taken against; -infinity until the row has seen a key
     bool ok = true;
-    const int steps = to[t] - from[t] + 1;
-    for (int i = 0; i < steps && ok; ++i) {
-      const int k0 = (from[t] + i) * SA_T;
-      ok = sa_wait(&s_full[t], (uint32_t)i & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
+    for (int i = 0; i < n && ok; ++i) {
+      const int k0 = (j0 + i) * SA_T;
+      ok = sa_wait(s_full, (uint32_t)i & 1u, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
       if (!ok) break;
       tc_fence_after();
       uint32_t x[128];
@@ -395,22 +356,20 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       tmem_st32(t_s + 32u, *reinterpret_cast<uint32_t(*)[32]>(&x[32]));
       tmem_st_wait();
       tc_fence_before();
-      sa_warp_arrive(&p_full[t], lane);
+      sa_warp_arrive(p_full, lane);
     }
-    if (t == 0 ? has0 : has1) {           // without a step, Q has to be there before its place is written
-      if (ok) ok = sa_wait(steps > 0 ? &o_full[t] : &q_full[t], 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);
-      tc_fence_after();
-    }
+    if (ok) ok = sa_wait(n > 0 ? o_full : q_full, 0, abort_flag, p, FFK_ERR_TIMEOUT_EPILOGUE);      // without a key, Q has to be there before its place is written
+    tc_fence_after();
     if (ok) {
-      const bool stored = t * SA_T + r < rows_cta && q < p.S;
+      const bool stored = q < p.S;
       const float inv = empty || !(l != 0.f) ? 0.f : 1.f / l;
       if (stored && p.lse) p.lse[((long long)b * p.H + h) * p.S + q] = empty ? 0.f : m + __log2f(l);
-      // O goes out through the query tile's place: the last product has read that
-      uint8_t *tile = smem + C::OFF_Q + t * C::TILE;
+      // O goes out through the queries' place: the last product has read that
+      uint8_t *tile = smem + C::OFF_Q;
 #pragma unroll 1
       for (int c = 0; c < DT / 32; ++c) {
         uint32_t o[32];
-        if (steps > 0) {
+        if (n > 0) {
           tmem_ld32(t_o + (uint32_t)(c * 32), o);
           tmem_ld_wait();
         }
@@ -420,7 +379,7 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         sa_tile_row(tile, r, c * 32, o, inv);
       }
-      if (t * SA_T < rows_cta && q0 + t * SA_T < p.S) sa_tile_out<C::PANELS>(tile, &tmO, q0 + t * SA_T, h, b, 1 + t, 128, warp == 4 + 4 * t && lane == 0);
+      sa_tile_out<C::PANELS>(tile, &tmO, q0, h, b, 1, 128, threadIdx.x == 128);
       tc_fence_before();
     }
   }
@@ -429,7 +388,7 @@ span_attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)C::TM_COLS) : "memory");
   }
 }
 
@@ -462,10 +421,8 @@ FFK_API int ffk_span_attention_fwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
   if ((r = sa_head_map(&to, d->O, d->D, d->S, d->ldo, d->H, d->B))) return r;
   SpanArgs a = {};
   sa_args(d, a, ffk_span_attention_err());
-  // two query tiles per CTA share the K and V tiles and the tensor core; one where that would leave SMs without work
   const long long heads = (long long)d->B * d->H;
-  a.tiles = heads * ((d->S + 255) / 256) >= 148 ? 2 : 1;
-  const long long grid = heads * ((d->S + SA_T * a.tiles - 1) / (SA_T * a.tiles));
+  const long long grid = heads * ((d->S + SA_T - 1) / SA_T);
   if (heads > 0x7fffffffll || grid > 0x7fffffffll) return -2;
   FfkTraffic traffic((long long)d->B * d->S * d->D * 2 * (2 * d->H + 2 * d->KH));
   const bool cap = d->cap > 0.f, bias = d->slopes != nullptr;
