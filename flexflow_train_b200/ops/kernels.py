@@ -389,8 +389,8 @@ def attention_spans(documents, prompt=None, *, causal=True, out=None):
     """The first and last token that each token of packed sequences sees: int32 [B, S, 2], the mask of `span_attention_fwd`.
 
     documents [B, S] int32: a document is a run of equal numbers in a row; a negative number is padding, which sees nothing (first 0,
-    last -1).  A token sees its own document: up to itself if `causal`, to the end otherwise.  prompt [B, S] (bool or uint8, with
-    `causal` only): the flagged tokens that a document begins with are seen by all of its tokens."""
+    last -1).  A token sees its own document: up to itself if `causal`, to the end otherwise.  prompt [B, S] (bool or uint8):
+    the flagged tokens that a document begins with are seen by all of its tokens (which they are anyway unless `causal`)."""
     shape = documents.shape
     if len(shape) != 2 or documents.dtype is not torch.int32:
         raise KernelError("attention_spans: documents is an int32 [batch, sequence] tensor")
@@ -398,8 +398,6 @@ def attention_spans(documents, prompt=None, *, causal=True, out=None):
     if prompt is not None:
         if prompt.dtype not in (torch.bool, torch.uint8) or prompt.shape != shape:
             raise KernelError("attention_spans: prompt holds one bool or uint8 flag per token")
-        if not causal:
-            raise KernelError("attention_spans: a prompt is seen by all of its document anyway unless the mask is causal")
     if out is None:
         out = torch.empty(B, S, 2, dtype=torch.int32, device=documents.device)
     if out.dtype is not torch.int32 or out.shape != (B, S, 2):
@@ -491,7 +489,7 @@ def span_attention_fwd(q, k, v, out, lse, spans, *, B, S, H, KH, D, scale, cap=0
     fp32 receives the base-2 log-sum-exp of x (0 for an empty span), which `span_attention_bwd` needs.
 
     What tokens hold that no query sees does not matter, NaN and infinity included.  A NaN or infinity in a token that some query does see
-    may reach other queries of its neighbourhood (up to 256 tokens that are computed together)."""
+    may reach other queries of its neighbourhood (up to 128 tokens that are computed together)."""
     what = "span_attention_fwd"
     at, slope, stat = _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes)
     rows, wide, narrow = B * S, H * D, KH * D

@@ -44,6 +44,14 @@ def test_spans_follow_the_definition(B, S, mean, form):
     assert torch.equal(got.cpu(), spans_of(doc, prompt, causal=form != "both"))
 
 
+@pytest.mark.parametrize("S,mean", [(7, 2), (1024, 90), (2500, 700)])
+def test_prompts_of_documents_that_are_seen_from_both_sides(S, mean):
+    doc = random_documents(3, S, mean, seed=S)
+    prompt = torch.rand(3, S, generator=torch.Generator().manual_seed(S)) < 0.9
+    got = K.attention_spans(doc.cuda(), prompt.cuda(), causal=False).cpu()
+    assert torch.equal(got, spans_of(doc, prompt, causal=False)) and torch.equal(got, spans_of(doc, None, causal=False))
+
+
 def test_spans_of_runs_that_cross_many_blocks_and_of_flags_that_end_there():
     S = 6000
     doc = torch.zeros(4, S, dtype=torch.int32)
