@@ -5,12 +5,15 @@
 // The tensors are cut into pieces of PIECE elements, listed in device memory once when the list is made (address, destination, length,
 // type); a block takes pieces in steps of the grid.  Squares of one 16-byte vector are added in 32 bits, vectors in 64: that costs one
 // conversion and one 64-bit addition per vector and keeps the sum of 1e9 elements exact to a few 1e-8.  A vector whose squares leave the
-// range of 32 bits (elements beyond 1e18, or below 1e-16 and not zero, infinities, NaN) is squared in 64 bits.  Each block leaves one partial sum; whoever needs
-// the norm adds the partial sums in their fixed order, so the result does not depend on which block came first, and there is no counter
-// to reset.  The clipping kernel's blocks each add them up (at most 1184 numbers from L2), which saves a launch between the passes.
+// range of 32 bits (elements beyond 1e18, or below 1e-16 and not zero, infinities, NaN) is squared in 64 bits.  Each block leaves one partial
+// sum; whoever needs the norm adds the partial sums in their fixed order, so the result does not depend on which block came first, and there
+// is no counter to reset.  The clipping kernel's blocks each add them up (at most 1184 numbers from L2), which saves a launch between the
+// passes.  A clipped element is rounded once, when it is stored.
 //
 // What bounds it: HBM, read once for the norm and read again and written for the clipping.  The second pass goes over the pieces in the
-// opposite order: it begins with what the first left in L2.
+// opposite order: it begins with what the first left in L2.  403 million bf16 elements (805 MB) in the tensors of eight layers of width 2048:
+// norm 114 us (7.1 TB/s, reads only), with the clipping 385 us (three passes over the gradients at the copy rate: 370); 6.3 million fp32
+// elements: 20 us.
 #include <cuda_fp16.h>
 
 #include "common.cuh"

@@ -11,7 +11,8 @@
 // bytes, or one element where the width or an address does not allow that), up to 16 warps (8 of single elements); wider rows give N pieces.  More pieces and fewer
 // warps cost registers and with them the loads under way: 32768 x 1024 backward 60 us with one warp and four pieces.  Backward's blocks stay
 // for many rows: a thread keeps the columns it owns of dgamma in registers and the block leaves one partial row, which the fold adds in a
-// fixed order.  Rows too wide for registers take the kernels at the end, which read a row twice.
+// fixed order.  Rows too wide for registers take the kernels at the end, which read a row twice.  32768 x 2048 bf16 with residual: forward 80
+// us (6.7 TB/s), backward 98 (5.5 TB/s) and 5 for the fold; 4004 x 1001 fp32, single elements: 29 both ways; 128 x 512 bf16 forward: 2.1.
 #include "common.cuh"
 
 namespace {

@@ -9,6 +9,7 @@
 // What bounds it: launch and load latency (12 bytes a token).  A block takes SEG tokens of one row; what it needs of the rest of the row
 // is one number each -- where the run at its first token began, where the run at its last token ends, where that run's flags end -- and
 // the block looks for those by itself, in steps of its width, so blocks share nothing and there is one launch and no scratch.
+// 8 x 256: 1.7 us; 16 x 16384 in documents of about 1500 with prompts: 8.7 us, of which two searches of up to 2048 places each way.
 #include "common.cuh"
 
 namespace {
