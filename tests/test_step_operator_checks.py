@@ -78,7 +78,7 @@ def test_spans_refuse():
     refused("int32", lambda: K.attention_spans(doc[0]))
     refused("prompt", lambda: K.attention_spans(doc, torch.zeros(2, 7, dtype=torch.bool)))
     refused("prompt", lambda: K.attention_spans(doc, torch.zeros(2, 8)))
-    refused("anyway", lambda: K.attention_spans(doc, torch.zeros(2, 8, dtype=torch.bool), causal=False))
+    refused("CPU tensor", lambda: K.attention_spans(doc, torch.zeros(2, 8, dtype=torch.bool), causal=False))
     refused("out is", lambda: K.attention_spans(doc, out=torch.zeros(2, 8, dtype=torch.int32)))
     both = torch.zeros(2, 8, 2, dtype=torch.int32)
     refused("share memory", lambda: K.attention_spans(both.view(-1)[:16].view(2, 8), out=both))
