@@ -16,6 +16,7 @@
 //
 // Rounded to bf16: P and dS (the type that the products take), and dQ, dK, dV once, when they are stored.  delta is taken of the O that
 // forward stored; its rounding and that of dS are what sets the gradients' error (2.5e-3 to 2.7e-3 of their norm, 1.7e-3 with both in fp32).
+// dS as the sum of two bf16 operands (16 bits of it, 1.8e-3) costs a fourth of the pass: 8 x 2048 packed 510 -> 648 us, 8192 causal 1046 -> 1301.
 //
 // What bounds it: a tile pair of a long sequence takes about 8300 cycles in both kernels together (8192 causal, cap), of which the seven
 // products fill 3584 at the tensor core's rate; the rest is the element-wise chain (tensor-memory load, cap, exponential, mask, dS, store,
