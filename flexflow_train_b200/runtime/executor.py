@@ -1675,7 +1675,11 @@ class Executable:
             return
         sl = slice(start, None)
         shadow = self.shadow[sl] if self.shadow is not None else None
-        norm = K.gradient_norm(self.grad_list) if self.grad_list is not None else None
+        norm = None
+        if o.max_grad_norm > 0:
+            if self.grad_list is None:
+                raise ValueError("max_grad_norm was 0 when the executable was built: its step cannot clip")
+            norm = K.gradient_norm(self.grad_list)
         if o.kind == "adam":
             K.adam_update(self.master[sl], self.opt_m[sl], self.opt_v[sl], self.grads[sl], shadow, 0.0, o.beta1, o.beta2, o.epsilon,
                           o.weight_decay, 1.0, alpha_tensor=self.alpha_tensor, grad_norm=norm, max_grad_norm=o.max_grad_norm)

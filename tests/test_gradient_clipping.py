@@ -105,6 +105,23 @@ def test_step_on_the_gpu(dtype, kind):
 
 
 @gpu
+def test_a_limit_changed_after_the_build():
+    """Taken away, the step does not clip; brought in, it is refused."""
+    make = lambda limit: api.compile("mlp", MLP, config=api.FFConfig(compute_dtype="fp32", use_cuda_graph=False),  # noqa: E731
+                                     optimizer=OptimizerConfig(kind="sgd", lr=0.5, max_grad_norm=limit))
+    plain, other = make(0.0), make(1e-3)
+    other.load_state_dict(copy.deepcopy(plain.state_dict()))
+    x, y = batch(classes_of(plain))
+    other.executable.cfg.optimizer.max_grad_norm = 0.0
+    plain.train_step(x, y)
+    other.train_step(x, y)
+    assert torch.equal(plain.executable.master, other.executable.master)
+    plain.executable.cfg.optimizer.max_grad_norm = 1.0
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        plain.train_step(x, y)
+
+
+@gpu
 def test_tables_are_part_of_the_norm():
     """Plain SGD keeps embedding tables out of the arena; with clipping they are in it."""
     cfg = {"batch_size": 64, "embedding_dim": 16, "embedding_bag_size": 1, "embedding_size": [500, 300],
