@@ -413,7 +413,9 @@ def attention_spans(documents, prompt=None, *, causal=True, out=None):
     if po % 8:
         raise KernelError("attention_spans: out must start on an 8-byte boundary")
     stream = _launch_stream(documents, prompt, out)
-    _check(_nlib().ffk_attention_spans(pd, pp, po, B, S, 1 if causal else 0, stream), "ffk_attention_spans")
+    room = _nlib().ffk_attention_spans_scratch(B, S) if S > 8192 else 0        # long rows: what their pieces say to one another
+    scratch = torch.empty(room, dtype=torch.int32, device=documents.device) if room else None
+    _check(_nlib().ffk_attention_spans(pd, pp, po, _p(scratch), B, S, 1 if causal else 0, stream), "ffk_attention_spans")
     return out
 
 
@@ -779,7 +781,8 @@ def _new_ops_decl(l):
         "ffk_rmsnorm_fwd": ([P, P, P, P, P, P, I, I, F, I, S], c_int),
         "ffk_rmsnorm_bwd": ([P, P, P, P, P, P, P, P, I, I, I, I, S], c_int),
         "ffk_rmsnorm_bwd_scratch": ([I, I], c_longlong),
-        "ffk_attention_spans": ([P, P, P, I, I, I, S], c_int),
+        "ffk_attention_spans": ([P, P, P, P, I, I, I, S], c_int),
+        "ffk_attention_spans_scratch": ([I, I], c_longlong),
         "ffk_span_attention_fwd": ([ctypes.c_char_p, S], c_int),
         "ffk_span_attention_bwd": ([ctypes.c_char_p, S], c_int),
         "ffk_span_attention_bwd_scratch_floats": ([I, I, I], c_longlong),

@@ -44,6 +44,20 @@ def test_spans_follow_the_definition(B, S, mean, form):
     assert torch.equal(got.cpu(), spans_of(doc, prompt, causal=form != "both"))
 
 
+@pytest.mark.parametrize("S,mean", [(17 * 1024, 900), (17 * 1024 + 1, 30000), (40000, 6000), (20000, 1)])
+@pytest.mark.parametrize("form", ["causal", "prompt", "both"])
+def test_spans_of_long_rows(S, mean, form):
+    """Rows whose pieces are told of one another by a launch of their own."""
+    doc = random_documents(2, S, mean, seed=S)
+    prompt = None
+    if form == "prompt":                     # a document's flags end in its own piece, at a piece's border, pieces later, or with it
+        prompt = torch.ones(2, S, dtype=torch.bool)
+        prompt[0, torch.randint(0, S, (max(1, S // 5000),), generator=torch.Generator().manual_seed(S))] = False
+        prompt[0, 5 * 1024] = prompt[0, 9 * 1024 - 1] = False
+    got = K.attention_spans(doc.cuda(), None if prompt is None else prompt.cuda(), causal=form != "both")
+    assert torch.equal(got.cpu(), spans_of(doc, prompt, causal=form != "both"))
+
+
 @pytest.mark.parametrize("S,mean", [(7, 2), (1024, 90), (2500, 700)])
 def test_prompts_of_documents_that_are_seen_from_both_sides(S, mean):
     doc = random_documents(3, S, mean, seed=S)
