@@ -377,6 +377,8 @@ int rms_resident(K kernel, int threads, size_t smem) {
   int n = 0;
   return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess ? n : 1;
 }
+// steps of a loop past the end of rows or columns stay within 32 bits
+bool rms_sizes_ok(int rows, int cols) { return rows <= 0x7fffffff - 4096 && cols <= (1 << 30); }
 bool rms_aligned(const void *p) { return (((uintptr_t)p) & 15) == 0; }
 
 template <typename T, int V, int N, int WARPS>
@@ -432,7 +434,7 @@ FFK_API int ffk_rmsnorm_fwd(const void *a, const void *b, const void *gamma, voi
                             cudaStream_t st) {
   if (dt != 0 && dt != 1) return -2;
   if (rows <= 0) return 0;
-  if (cols <= 0) return -2;
+  if (cols <= 0 || !rms_sizes_ok(rows, cols)) return -2;
   const int es = dt == 1 ? 2 : 4;
   FfkTraffic traffic((long long)rows * cols * es * (b ? xsum ? 4 : 3 : 2));
   const RmsForm f = rms_form(cols, es, rms_aligned(a) && rms_aligned(b) && rms_aligned(gamma) && rms_aligned(xsum) && rms_aligned(y));
@@ -444,7 +446,7 @@ FFK_API int ffk_rmsnorm_fwd(const void *a, const void *b, const void *gamma, voi
 
 // floats of scratch: the partial rows of dgamma, for either form of the addresses
 FFK_API long long ffk_rmsnorm_bwd_scratch(int rows, int cols) {
-  if (rows <= 0 || cols <= 0) return 0;
+  if (rows <= 0 || cols <= 0 || !rms_sizes_ok(rows, cols)) return 0;
   long long most = 0;
   for (int es = 2; es <= 4; es += 2)
     for (int whole = 0; whole < 2; ++whole) {
@@ -459,6 +461,7 @@ FFK_API int ffk_rmsnorm_bwd(const void *dy, const void *h, const void *gamma, co
                             int rows, int cols, int dt, int accumulate_params, cudaStream_t st) {
   if (dt != 0 && dt != 1) return -2;
   if (cols <= 0) return rows <= 0 ? 0 : -2;
+  if (!rms_sizes_ok(rows, cols)) return -2;
   const int es = dt == 1 ? 2 : 4;
   int grid = 0;
   if (dgamma && rows > 0 && !partial) return -2;

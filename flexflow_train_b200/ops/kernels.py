@@ -824,8 +824,8 @@ def _rms_check(what, a, gamma, rstd, same):
         es = 4
     else:
         raise KernelError(f"{what}: bf16 or fp32 rows expected, got {dtype}")
-    if cols < 1 or rows > 2**31 - 1 or cols > 2**31 - 1:
-        raise KernelError(f"{what}: rows of {cols} elements")
+    if cols < 1 or rows > 2**31 - 4097 or cols > 2**30:
+        raise KernelError(f"{what}: {rows} rows of {cols} elements (up to 2^31 - 4097 rows of 1 to 2^30)")
     whole = a.is_contiguous()
     for t in same:
         if t is not None:

@@ -97,6 +97,8 @@ def test_rmsnorm_refuses():
     refused("with a residual", lambda: K.rmsnorm_fwd(x, g, 1e-6, xsum=x.clone()))
     refused("rstd", lambda: K.rmsnorm_fwd(x, g, 1e-6, rstd=r[:3]))
     refused("elements", lambda: K.rmsnorm_fwd(torch.zeros(4, 0), torch.zeros(0), 1e-6))
+    for shape in ((2**31 - 4096, 1), (1, 2**30 + 1)):              # loops' steps past the end would leave 32 bits
+        refused("elements", lambda: K.rmsnorm_fwd(torch.zeros(1, 1).expand(shape), g, 1e-6))  # noqa: B023
     flat = torch.zeros(300)
     refused("share memory", lambda: K.rmsnorm_fwd(flat[:128].view(4, 32), g, 1e-6, out=flat[32:160].view(4, 32)))
     same = torch.zeros(4, 32)
