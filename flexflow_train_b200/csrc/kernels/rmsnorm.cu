@@ -12,7 +12,7 @@
 // warps cost registers and with them the loads under way: 32768 x 1024 backward 60 us with one warp and four pieces.  Backward's blocks stay
 // for many rows: a thread keeps the columns it owns of dgamma in registers and the block leaves one partial row, which the fold adds in a
 // fixed order.  Rows too wide for registers take the kernels at the end, which read a row twice.  32768 x 2048 bf16 with residual: forward 80
-// us (6.7 TB/s), backward 98 (5.5 TB/s) and 5 for the fold; 4004 x 1001 fp32, single elements: 29 both ways; 128 x 512 bf16 forward: 2.1.
+// us (6.7 TB/s), backward 92 with the fold (5.8 TB/s); 4004 x 1001 fp32, single elements: 29 both ways; 128 x 512 bf16 forward: 2.1.
 #include "common.cuh"
 
 namespace {
@@ -143,13 +143,29 @@ __global__ void __launch_bounds__(rms_threads(WARPS)) rms_fwd_kernel(const T *a,
   }
 }
 
+__device__ __forceinline__ uint32_t smem_place(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes from global to shared memory while the thread goes on; the end of a group of them; the wait for all but the latest LEFT groups
+__device__ __forceinline__ void rms_fetch(uint32_t to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void rms_fetch_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void rms_fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// Pieces of 16 bytes come through shared memory, each thread's own: the next row is under way while this one is reduced and written, without a
+// barrier among threads or registers for it.  32768 x 2048 bf16: 92 us with the fold, 102 with loads into registers; 8192 x 4096: 51
+// and 62; 2048 x 8192: 34 and 41; two rows ahead: the same within 2 %.
+template <int V, int N, int WARPS>
+constexpr size_t rms_bwd_smem() { return V == 1 ? 0 : (size_t)2 * N * 3 * 16 * rms_threads(WARPS); }
+
 // dh may be dy or dsum.  `partial`: [gridDim.x][cols]
 template <typename T, int V, int N, int WARPS>
 __global__ void __launch_bounds__(rms_threads(WARPS)) rms_bwd_kernel(const T *dy, const T *h, const T *gamma, const float *rstd, const T *dsum, T *dh,
                                                       float *__restrict__ partial, int rows, int cols) {
   pdl_entry(dh);
   __shared__ float red[2 * rms_threads(WARPS) / 32];
-  extern __shared__ float part[];            // several rows a block: its sum of dgamma, [cols]
+  extern __shared__ float4 rms_smem[];       // pieces on their way; then (several rows a block) its sum of dgamma, [cols]
+  float *part = reinterpret_cast<float *>(rms_smem);
   constexpr int GROUPS = rms_threads(WARPS) / (WARPS * 32);
   const int slot = threadIdx.x % (WARPS * 32), group = threadIdx.x / (WARPS * 32);
   const float inv = 1.f / (float)cols;
@@ -164,9 +180,42 @@ __global__ void __launch_bounds__(rms_threads(WARPS)) rms_bwd_kernel(const T *dy
     for (int j = 0; j < V; ++j) acc[i][j] = 0.f;
   }
   int parity = 0;
-  for (long long row = (long long)blockIdx.x * GROUPS + group; row < rows; row += (long long)gridDim.x * GROUPS) {
+  const long long step = (long long)gridDim.x * GROUPS;
+  long long row = (long long)blockIdx.x * GROUPS + group;
+  constexpr int THREADS = rms_threads(WARPS);
+  int stage = 0;
+  float rs_next = 0.f;
+  // place of piece i of dy (0), h (1), dsum (2)
+  auto place = [&](int at, int i, int what) { return ((at * N + i) * 3 + what) * THREADS + (int)threadIdx.x; };
+  auto fetch = [&](long long r, int at) {
+    if (r < rows) {
+      const long long base = r * cols;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = (i * WARPS * 32 + slot) * V;
+        if (c < cols) {
+          rms_fetch(smem_place(&rms_smem[place(at, i, 0)]), dy + base + c);
+          rms_fetch(smem_place(&rms_smem[place(at, i, 1)]), h + base + c);
+          if (dsum) rms_fetch(smem_place(&rms_smem[place(at, i, 2)]), dsum + base + c);
+        }
+      }
+    }
+    rms_fetch_end();
+  };
+  auto take = [&](Piece<T, V> &to, int i, int what) { to.load(reinterpret_cast<const T *>(&rms_smem[place(stage, i, what)])); };
+  if constexpr (V > 1) {
+    fetch(row, 0);
+    if (row < rows) rs_next = rstd[row];
+  }
+  for (; row < rows; row += step) {
     const long long base = row * cols;
     Piece<T, V> py[N], ph[N], ps[N];
+    float rs = rs_next;
+    if constexpr (V > 1) {
+      if (row + step < rows) rs_next = rstd[row + step];
+      fetch(row + step, stage ^ 1);
+      rms_fetch_wait<1>();
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int c = (i * WARPS * 32 + slot) * V;
@@ -174,12 +223,17 @@ __global__ void __launch_bounds__(rms_threads(WARPS)) rms_bwd_kernel(const T *dy
       ph[i].zero();
       ps[i].zero();
       if (c < cols) {
-        py[i].load(dy + base + c);
-        ph[i].load(h + base + c);
-        if (N * V < 32 && dsum) ps[i].load(dsum + base + c);
+        if constexpr (V > 1) {
+          take(py[i], i, 0);
+          take(ph[i], i, 1);
+        } else {
+          py[i].load(dy + base + c);
+          ph[i].load(h + base + c);
+          if (dsum) ps[i].load(dsum + base + c);
+        }
       }
     }
-    const float rs = rstd[row];
+    if constexpr (V == 1) rs = rstd[row];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -202,10 +256,14 @@ __global__ void __launch_bounds__(rms_threads(WARPS)) rms_bwd_kernel(const T *dy
       const int c = (i * WARPS * 32 + slot) * V;
       if (c < cols) {
         float y[V], x[V], g[V], s[V];
+        if constexpr (V > 1) {            // again: registers for them would cost resident blocks
+          take(py[i], i, 0);
+          take(ph[i], i, 1);
+          if (dsum) take(ps[i], i, 2);
+        }
         py[i].get(y);
         ph[i].get(x);
         pg[i].get(g);
-        if (N * V >= 32 && dsum) ps[i].load(dsum + base + c);      // the widest rows: the other three fill the registers
         ps[i].get(s);
 #pragma unroll
         for (int j = 0; j < V; ++j) y[j] = fmaf(rs, fmaf(y[j], g[j], -x[j] * k), s[j]);
@@ -213,7 +271,9 @@ __global__ void __launch_bounds__(rms_threads(WARPS)) rms_bwd_kernel(const T *dy
         py[i].store(dh + base + c);
       }
     }
+    stage ^= 1;
   }
+  if constexpr (V > 1) rms_fetch_wait<0>();
   if (!partial) return;
   float *out = partial + (long long)blockIdx.x * cols;
   if constexpr (GROUPS == 1) {
@@ -226,7 +286,8 @@ __global__ void __launch_bounds__(rms_threads(WARPS)) rms_bwd_kernel(const T *dy
       }
     }
   } else {
-    // the groups add up their columns one after the other
+    // the groups add up their columns one after the other, where their pieces were
+    __syncthreads();
     for (int w = 0; w < GROUPS; ++w) {
       if (group == w) {
 #pragma unroll
@@ -364,10 +425,12 @@ int rms_fwd_grid(const RmsForm &f, int rows, int &threads) {
   const int per = threads / (f.warps * 32), want = (rows + per - 1) / per;
   return want < 148 * 8 ? want : 148 * 8;
 }
-// backward's blocks stay for their rows: as many as are resident at once, at most RMS_BWD_PER_SM per SM
+// backward's blocks stay for their rows: as many as are resident at once, at most RMS_BWD_PER_SM per SM of single elements; of whole pieces half
+// of that, which the row ahead keeps busy (32768 x 2048 bf16: 92 us with 4, 97 with 6, 114 with 2; 4004 x 1001 fp32: 18.5 with 8, 20 with 4)
 constexpr int RMS_BWD_PER_SM = 8;
 int rms_bwd_grid(const RmsForm &f, int rows, int per_sm) {
-  if (per_sm > RMS_BWD_PER_SM) per_sm = RMS_BWD_PER_SM;
+  const int at_most = f.v > 1 ? RMS_BWD_PER_SM / 2 : RMS_BWD_PER_SM;
+  if (per_sm > at_most) per_sm = at_most;
   const int groups = f.n == 0 ? 1 : rms_threads(f.warps) / (f.warps * 32);
   const int want = (rows + groups - 1) / groups, most = 148 * (per_sm < 1 ? 1 : per_sm);
   return want < most ? want : most;
@@ -392,9 +455,13 @@ int rms_bwd_run(const void *dy, const void *h, const void *gamma, const float *r
                 int &grid, cudaStream_t st) {
   constexpr int threads = rms_threads(WARPS);
   constexpr bool several = threads > WARPS * 32;
-  static const int per_sm = rms_resident(rms_bwd_kernel<T, V, N, WARPS>, threads, several ? (size_t)V * N * WARPS * 128 : 0);
+  constexpr size_t sums = several ? (size_t)V * N * WARPS * 128 : 0, smem = sums > rms_bwd_smem<V, N, WARPS>() ? sums : rms_bwd_smem<V, N, WARPS>();
+  static unsigned long long done = 0;
+  const cudaError_t e = ffk_allow_smem(rms_bwd_kernel<T, V, N, WARPS>, (int)smem, done);
+  if (e != cudaSuccess) return (int)e;
+  static const int per_sm = rms_resident(rms_bwd_kernel<T, V, N, WARPS>, threads, smem);
   grid = rms_bwd_grid({V, WARPS, N}, rows, per_sm);
-  return ffk_launch(rms_bwd_kernel<T, V, N, WARPS>, grid, threads, several ? (size_t)cols * 4 : 0, st, (const T *)dy, (const T *)h, (const T *)gamma,
+  return ffk_launch(rms_bwd_kernel<T, V, N, WARPS>, grid, threads, smem, st, (const T *)dy, (const T *)h, (const T *)gamma,
                     rstd, (const T *)dsum, (T *)dh, partial, rows, cols);
 }
 #define RMS_FORMS(RUN, T, V, ...)                            \
