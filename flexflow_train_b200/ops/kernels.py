@@ -440,31 +440,33 @@ def _span_sizes(what, spans, lse, B, S, H, KH, D, scale, cap, slopes):
     if S > 2**30:
         raise KernelError(f"{what}: sequences of up to 2^30 tokens")
     at = spans.data_ptr() if spans is not None else 1
-    if at % 8 or spans.dtype is not torch.int32 or spans.shape != (B, S, 2) or not spans.is_contiguous():
+    if at % 8 or spans.dtype is not _I32 or spans.shape != (B, S, 2) or not spans.is_contiguous():
         raise KernelError(f"{what}: spans is a contiguous int32 [B, S, 2] tensor (attention_spans)")
     if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous()):
         raise KernelError(f"{what}: slopes holds one fp32 value per query head")
-    if lse is None or lse.dtype is not torch.float32 or lse.shape != (B, H, S) or not lse.is_contiguous():
+    if lse is None or lse.dtype is not _F32 or lse.shape != (B, H, S) or not lse.is_contiguous():
         raise KernelError(f"{what}: lse must be a contiguous fp32 [B, H, S] tensor")
     return at, 0 if slopes is None else slopes.data_ptr(), lse.data_ptr()
 
 
 _INF = float("inf")
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
 def _span_place(what, name, t, rows, width):
     """A [B*S, >= width] bf16 matrix with unit column stride whose rows TMA can address: (address, pitch, width, end, name), pitch and
     width in elements."""
-    if t is None or t.dtype is not torch.bfloat16 or t.dim() != 2:
+    stride = t.stride() if t is not None else ()
+    if len(stride) != 2 or t.dtype is not _BF16:
         raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
+    ld, one = stride
     n, columns = t.shape
-    ld, one = t.stride()
     if n != rows or columns < width or (one != 1 and columns > 1):
         raise KernelError(f"{what}: {name} must be a bf16 matrix [batch*seq, heads*head_dim] with unit column stride")
     if rows <= 1:
         ld = width                       # a single row has no pitch
     p = t.data_ptr()
-    if ld < width or ld % 8 or p % 16:
+    if ld < width or ld & 7 or p & 15:
         raise KernelError(f"{what}: {name} must start on a 16-byte boundary, at a pitch of a multiple of 8 elements that holds its heads")
     return p, ld, width, p + 2 * ((rows - 1) * ld + width), name
 
