@@ -49,8 +49,10 @@ struct SpanArgs {
   float *lse;
   const float *delta;
   const int4 *summary;
-  bf16 *dQ, *dK, *dV;
-  long long lddq, lddk, lddv;
+  bf16 *dK, *dV;
+  long long lddk, lddv;
+  const bf16 *Q, *K, *V;           // of the kernels that do not go through tensor maps
+  long long ldq, ldk, ldv;
   int wide;                        // results' rows lie on 32-byte boundaries
   int *err;
 };
@@ -140,6 +142,13 @@ __device__ __forceinline__ bool sa_cap(uint32_t (&x)[N], const SpanArgs &p, bool
 __device__ __forceinline__ void sa_cap_any(uint32_t (&x)[32], const SpanArgs &p) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(sa_tanh_any(__uint_as_float(x[i]) * p.to_z) * p.from_z);
+}
+// one score, the same way
+__device__ __forceinline__ float sa_cap_one(float s, const SpanArgs &p) {
+  const float w = s * s;
+  if (fabsf(s) <= p.lim2) return s * fmaf(fmaf(w, p.t2[2], p.t2[1]), w, p.t2[0]);
+  if (fabsf(s) <= p.lim4) return s * fmaf(fmaf(fmaf(fmaf(w, p.t4[4], p.t4[3]), w, p.t4[2]), w, p.t4[1]), w, p.t4[0]);
+  return sa_tanh_any(s * p.to_z) * p.from_z;
 }
 // The bias: d0 = position of the first column less the row's (distances are whole numbers: exact), side: -1 / 1 where no column of the warp
 // lies right / left of its row, 0 otherwise; slope: the head's, over the scale

@@ -15,14 +15,15 @@
 // part (thread = one row and 32 of the columns); in the first kernel warp 3 brings each query tile's lse, delta and spans.
 //
 // Rounded to bf16: P and dS (the type that the products take), and dQ, dK, dV once, when they are stored.  delta is taken of the O that
-// forward stored; its rounding and that of dS are what sets the gradients' error (2.5e-3 to 2.7e-3 of their norm, 1.7e-3 with both in fp32).
+// forward stored, but for queries that see few keys; its rounding and that of dS are what sets the gradients' error (2.5e-3 to 2.7e-3 of their
+// norm, 1.7e-3 with both in fp32).
 // dS as the sum of two bf16 operands (16 bits of it, 1.8e-3) costs a fourth of the pass: 8 x 2048 packed 510 -> 648 us, 8192 causal 1046 -> 1301.
 //
 // What bounds it: a tile pair of a long sequence takes about 8300 cycles in both kernels together (8192 causal, cap), of which the seven
 // products fill 3584 at the tensor core's rate; the rest is the element-wise chain (tensor-memory load, cap, exponential, mask, dS, store,
 // barrier), which the 16 warps that registers allow issue in 41 to 45 % of the cycles.  8192 causal, 16 heads of 128, 4 key heads, cap: 1040 us
-// (660 TFLOP/s of the formula's five products), without a cap 860 (800).  8 x 2048 in documents of about 700, 16 heads of 128, cap: delta 28
-// (4.8 TB/s), dK / dV 237, dQ 199; without a cap 435 in all.  Tried and slower: dQ as two CTAs an SM with tiles of 64 keys (8192 causal: 1180), or
+// (660 TFLOP/s of the formula's five products), without a cap 860 (800).  8 x 2048 in documents of about 700, 16 heads of 128, cap: delta 45,
+// dK / dV 237, dQ 199; without a cap 450 in all.  Tried and slower: dQ as two CTAs an SM with tiles of 64 keys (8192 causal: 1180), or
 // going on with the next block of the grid as dK / dV does (its registers do not suffice).
 //
 // Every wait is bounded (tcgen05.cuh).
@@ -40,10 +41,62 @@ __device__ __forceinline__ void sa_times_slope(uint32_t (&y)[32], int c, float e
 }
 
 // ---------------------------------------------------------------------------------------------- delta and summaries
-// L lanes (16 bytes each) per (row, head); blocks from `delta_blocks` on: a warp per 128 queries.  Summary: smallest first key and largest
-// last key of the queries that see any, largest first key and smallest last key of all (an empty span among them: nothing is seen by all).
+// The delta of a query that sees few keys is sum_k P dP over them, from Q, K, V and dO, instead of dO . O: its gradients are differences of a few
+// products, and the rounding of O to bf16 would be a fair part of them (one head, a sequence of 2 tokens: dQ off by up to its own size; of 3:
+// 2.6e-2; of 8: 5e-3, as much as the other roundings).  It costs two dot products a key: backward of 8 x 2048, 16 heads of 128, documents of
+// about 700: 524 -> 538 us, of 60: 293 -> 318, of 5: 260 -> 341; with up to 16 keys, a warp per 128 queries: 574, 556, 734 (documents of 12).
+constexpr int SAB_FEW = 8;
+
+__device__ __forceinline__ bool sa_few(int2 s) { return s.x <= s.y && s.y - s.x < SAB_FEW; }
+
+__device__ __forceinline__ float sa_dot8(uint4 a, uint4 b) {
+  const uint32_t aa[4] = {a.x, a.y, a.z, a.w}, bb[4] = {b.x, b.y, b.z, b.w};
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = unpack_bf162(aa[i]), y = unpack_bf162(bb[i]);
+    s = fmaf(x.x, y.x, fmaf(x.y, y.y, s));
+  }
+  return s;
+}
+
+// L lanes (the group at `peers` of their warp), 16 bytes of the head from column c on each
 template <int L>
-__global__ void __launch_bounds__(256) span_attn_prep_kernel(const bf16 *dO, long long lddo, const bf16 *O, long long ldo, float *__restrict__ delta,
+__device__ __forceinline__ float span_attn_few(uint4 ov, const SpanArgs &p, unsigned row, int h, int c, int2 span, uint32_t peers) {
+  const int b = (int)(row / (unsigned)p.S), q = (int)(row - (unsigned)b * p.S);
+  const int kh = h / (p.H / p.KH);
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const long long first = (long long)b * p.S;
+  const uint4 qv = c < p.D ? *reinterpret_cast<const uint4 *>(p.Q + (first + q) * p.ldq + (long long)h * p.D + c) : zero;
+  const float lse = p.lse[((long long)b * p.H + h) * p.S + q], slope = p.slopes ? p.slopes[h] * SA_LOG2E : 0.f;
+  const bf16 *K = p.K + (first + span.x) * p.ldk + (long long)kh * p.D + c, *V = p.V + (first + span.x) * p.ldv + (long long)kh * p.D + c;
+  float sum = 0.f, total = 0.f;
+#pragma unroll 1
+  for (int k = span.x; k <= span.y; ++k, K += p.ldk, V += p.ldv) {
+    uint4 kv = zero, vv = zero;
+    if (c < p.D) {
+      kv = *reinterpret_cast<const uint4 *>(K);
+      vv = *reinterpret_cast<const uint4 *>(V);
+    }
+    float x = sa_dot8(qv, kv), dp = sa_dot8(ov, vv);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      x += __shfl_xor_sync(peers, x, o);
+      dp += __shfl_xor_sync(peers, dp, o);
+    }
+    if (p.to_z > 0.f) x = sa_cap_one(x, p);
+    const float e = sa_exp2(fmaf(x, p.factor, -slope * (float)abs(q - k)) - lse);
+    sum = fmaf(e, dp, sum);
+    total += e;
+  }
+  return total > 0.f ? sum / total : 0.f;
+}
+
+// Blocks up to `delta_blocks`: delta, L lanes (16 bytes each) per (row, head).  From there on a warp per 128 queries, their summary: smallest first
+// key and largest last key of the queries that see any, largest first key and smallest last key of all (an empty span among them: nothing is
+// seen by all).
+template <int L>
+__global__ void __launch_bounds__(256, 6) span_attn_prep_kernel(const bf16 *dO, long long lddo, const bf16 *O, long long ldo, float *__restrict__ delta,
                                                              int4 *__restrict__ summary, int delta_blocks, const SpanArgs p) {
   pdl_entry();
   const int lane = threadIdx.x & 31;
@@ -51,24 +104,24 @@ __global__ void __launch_bounds__(256) span_attn_prep_kernel(const bf16 *dO, lon
     // (row, head) pairs are counted in 32 bits (checked at the launch): 64-bit divisions had bounded this kernel
     const unsigned at = blockIdx.x * (256 / L) + threadIdx.x / L, total = (unsigned)p.B * p.S * p.H;
     const int c = (threadIdx.x % L) * 8;
-    const bool here = at < total;
+    if (at >= total) return;               // whole groups
     const unsigned row32 = at / (unsigned)p.H;
     const int h = (int)(at - row32 * p.H);
     const long long row = row32;
-    float s = 0.f;
-    if (here && c < p.D) {
-      const uint4 u = *reinterpret_cast<const uint4 *>(dO + row * lddo + (long long)h * p.D + c);
-      const uint4 w = *reinterpret_cast<const uint4 *>(O + row * ldo + (long long)h * p.D + c);
-      const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = unpack_bf162(uu[i]), o = unpack_bf162(ww[i]);
-        s = fmaf(a.x, o.x, fmaf(a.y, o.y, s));
-      }
+    const uint32_t peers = ((1u << L) - 1u) << (lane / L * L);
+    uint4 u = make_uint4(0, 0, 0, 0), w = u;
+    if (c < p.D) {
+      u = *reinterpret_cast<const uint4 *>(dO + row * lddo + (long long)h * p.D + c);
+      w = *reinterpret_cast<const uint4 *>(O + row * ldo + (long long)h * p.D + c);
     }
+    int2 span = p.spans[row];
+    span.x = max(span.x, 0);
+    span.y = min(span.y, p.S - 1);
+    float s = sa_dot8(u, w);               // for all: O's load does not wait for the span's
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (here && c == 0) {
+    for (int o = L / 2; o > 0; o >>= 1) s += __shfl_xor_sync(peers, s, o);
+    if (sa_few(span)) s = span_attn_few<L>(u, p, row32, h, c, span, peers);
+    if (c == 0) {
       const unsigned b = row32 / (unsigned)p.S, q = row32 - b * p.S;
       delta[((long long)b * p.H + h) * p.S + q] = s;
     }
@@ -980,6 +1033,7 @@ FFK_API int ffk_span_attention_bwd(const FfkSpanAttnDesc *d, cudaStream_t st) {
   a.dK = (bf16 *)d->dK; a.lddk = d->lddk; a.dV = (bf16 *)d->dV; a.lddv = d->lddv;
   a.wide = sa_wide(d->dK, d->lddk, d->D) && sa_wide(d->dV, d->lddv, d->D);
   FfkTraffic traffic((long long)d->B * d->S * d->D * 4 * (d->H + d->KH));
+  a.Q = (const bf16 *)d->Q; a.ldq = d->ldq; a.K = (const bf16 *)d->K; a.ldk = d->ldk; a.V = (const bf16 *)d->V; a.ldv = d->ldv;
   const unsigned blocks = (unsigned)(delta_blocks + sum_blocks);
   r = lanes == 8 ? ffk_launch(span_attn_prep_kernel<8>, blocks, 256, 0, st, (const bf16 *)d->dO, d->lddo, (const bf16 *)d->O, d->ldo, delta, summary,
                               (int)delta_blocks, a)

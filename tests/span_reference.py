@@ -23,9 +23,10 @@ def visible(spans, S):
     return (at[None, None] >= spans[..., :1]) & (at[None, None] <= spans[..., 1:])          # [B, S, S]
 
 
-def reference(q, k, v, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None, dout=None):
+def reference(q, k, v, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None, dout=None, few=0):
     """Values and bounds of out (and lse), and with `dout` of dq, dk, dv: {name: (value, bound)}, matrices of [B*S, heads*D] in 64 bits.
-    Rows that nothing may touch (tokens that nobody sees, queries with empty spans) may hold NaN."""
+    Rows that nothing may touch (tokens that nobody sees, queries with empty spans) may hold NaN.  few: queries that see so many keys at most have
+    a delta in 32 bits, no rounded O in it."""
     seen = visible(spans, S)
     some = seen.any(-1)                                       # queries that see a key
     heads = lambda t, n: t.double().reshape(B, S, n, D).permute(0, 2, 1, 3)  # noqa: E731
@@ -54,7 +55,8 @@ def reference(q, k, v, spans, *, B, S, H, KH, D, scale, cap=0.0, slopes=None, do
     delta = (do * out).sum(-1, keepdim=True)
     ds = p * c * (dp - delta)
     whole = p * (do.abs() @ v.abs().transpose(-1, -2) + (do.abs() * out.abs()).sum(-1, keepdim=True))
-    e_ds = U * ds.abs() + p * c * (do.abs() * e_out).sum(-1, keepdim=True) + (SLACK * c + (TANH if cap > 0 else 0.0)) * whole
+    many = (seen.sum(-1) > few)[:, None, :, None]
+    e_ds = U * ds.abs() + p * c * many * (do.abs() * e_out).sum(-1, keepdim=True) + (SLACK * c + (TANH if cap > 0 else 0.0)) * whole
     dq, dk, dv = scale * ds @ k, share(scale * ds.transpose(-1, -2) @ q), share(p.transpose(-1, -2) @ do)
     m_dv = share(p.transpose(-1, -2) @ do.abs())
     tiny = 1e-30

@@ -158,6 +158,28 @@ def test_attention_and_gradients_against_the_formula(B, S, H, KH, D, kind, cap, 
     check(run(q, k, v, dout, spans, **sizes), reference(q, k, v, spans, dout=dout, **sizes))
 
 
+FEW = 8
+
+
+@pytest.mark.parametrize("S,mean", [(1, 1), (2, 2), (3, 3), (5, 2), (8, 8), (131, 3), (400, 2)])
+@pytest.mark.parametrize("H,KH,D,kind,cap,bias", [(1, 1, 64, "full", 0.0, False), (1, 1, 32, "causal", 0.0, True), (4, 2, 128, "both", 20.0, False),
+                                                  (3, 1, 72, "documents", 0.5, True), (2, 2, 8, "documents", 0.0, False)])
+def test_queries_that_see_few_keys(S, mean, H, KH, D, kind, cap, bias):
+    """Their gradients are differences of a few products: the bound has no rounding of O in it."""
+    B = 3
+    if kind in ("both", "documents"):
+        spans = K.attention_spans(random_documents(B, S, mean, seed=S).cuda(), causal=kind == "documents")
+    elif S > FEW:                            # windows
+        at = torch.arange(S, dtype=torch.int32, device="cuda").expand(B, S)
+        spans = torch.stack([at - (3 if kind == "full" else 7), at + (4 if kind == "full" else 0)], -1).contiguous()
+    else:
+        spans = mask(kind, B, S, seed=S)
+    slopes = torch.linspace(0.1, 1.0, H, device="cuda") if bias else None
+    _, q, k, v, dout = make(B, S, H, KH, D, seed=S + D)
+    sizes = dict(B=B, S=S, H=H, KH=KH, D=D, scale=1.0 / math.sqrt(D), cap=cap, slopes=slopes)
+    check(run(q, k, v, dout, spans, **sizes), reference(q, k, v, spans, dout=dout, few=FEW, **sizes))
+
+
 @pytest.mark.parametrize("cap,scale", [(0.0, 2.0), (3.0, 1.0), (30.0, 4.0)])
 def test_scores_far_apart(cap, scale):
     """Maxima that move by much more than 2^8 from tile to tile, and scores at the cap's flat end."""
