@@ -397,3 +397,48 @@ def test_the_first_calls_of_a_process_may_be_captured():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stdout + r.stderr
+
+
+def test_calls_on_two_streams_at_once():
+    """Passes of different head dims and masks side by side give the bits that they give alone."""
+    jobs = []
+    for D, KH, S, cap in ((64, 2, 700, 0.0), (128, 4, 900, 30.0)):
+        B, H = 2, 4
+        _, q, k, v, dout = make(B, S, H, KH, D, seed=D)
+        spans = K.attention_spans(random_documents(B, S, 150, seed=D).cuda())
+        sizes = dict(B=B, S=S, H=H, KH=KH, D=D, scale=1.0 / math.sqrt(D), cap=cap, slopes=None)
+        jobs.append((q, k, v, dout, spans, sizes, run(q, k, v, dout, spans, **sizes), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for q, k, v, dout, spans, sizes, _, stream in jobs:
+            B, S, H, KH, D = (sizes[n] for n in ("B", "S", "H", "KH", "D"))
+            with torch.cuda.stream(stream):
+                out, lse = torch.empty(B * S, H * D, dtype=torch.bfloat16, device="cuda"), torch.empty(B, H, S, device="cuda")
+                dq, dk, dv = (torch.empty(B * S, n * D, dtype=torch.bfloat16, device="cuda") for n in (H, KH, KH))
+                scratch = torch.empty(K.span_attention_bwd_scratch_floats(B, H, S), device="cuda")
+                K.span_attention_fwd(q, k, v, out, lse, spans, **sizes)
+                K.span_attention_bwd(q, k, v, out, lse, dout, dq, dk, dv, scratch, spans, **sizes)
+            got.append({"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv, "scratch": scratch})
+        torch.cuda.synchronize()
+        for (*_, want, _stream), g in zip(jobs, got):
+            assert all(torch.equal(g[n], want[n]) for n in want)
+    assert K.span_attention_last_error() == 0
+
+
+def test_spans_of_long_rows_replayed():
+    """Their pieces' summaries lie in memory of the graph's own."""
+    S = 20000
+    doc = random_documents(2, S, 4000, seed=1).cuda()
+    want, other = K.attention_spans(doc), K.attention_spans(torch.zeros_like(doc))
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        K.attention_spans(doc, out=out)
+    graph.replay()
+    assert torch.equal(out, want)
+    doc.zero_()
+    between = K.attention_spans(torch.ones_like(doc))            # an eager call has a scratch of its own
+    graph.replay()
+    assert torch.equal(out, other) and torch.equal(between, other)
